@@ -16,6 +16,7 @@ FT_OK = 0
 FT_MASKED_CE_SKIP = 0xFFFFFFFF
 FT_SUM_SQUARES_CHUNK = 4096
 FT_GEMM_F32, FT_GEMM_F16, FT_GEMM_F16X2 = 0, 1, 2
+FT_TYPE_F32, FT_TYPE_F16 = 0, 1
 FT_LINEARS = 7
 FT_ERR_COMM = 5
 FT_COMM_ID_BYTES = 128
@@ -43,6 +44,15 @@ class FtAdamParams(C.Structure):
     _fields_ = [
         ("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
         ("weight_decay", C.c_float), ("t", C.c_float), ("_pad", C.c_float * 2),
+    ]
+
+
+class FtLinearCeParams(C.Structure):
+    _fields_ = [
+        ("rows", C.c_uint32), ("hidden", C.c_uint32), ("vocab", C.c_uint32),
+        ("weight_vocab_major", C.c_uint32), ("hidden_type", C.c_uint32), ("weight_type", C.c_uint32),
+        ("grad_hidden_type", C.c_uint32), ("grad_weight_type", C.c_uint32),
+        ("vocab_piece", C.c_uint32), ("grad_scale", C.c_float),
     ]
 
 
@@ -109,6 +119,12 @@ PROTOTYPES = {
     "ft_sum_squares_partial": [_P, _P, _Z, _P, _Z, C.POINTER(_Z)],
     "ft_clip_grad_by_norm": [_P, _P, _Z, _F],
     "ft_adamw_update": [_P, _P, _P, _P, _P, _Z, C.POINTER(FtAdamParams)],
+    "ft_linear_cross_entropy_workspace": [_P, C.POINTER(FtLinearCeParams), _I, _I, C.POINTER(_Z)],
+    "ft_linear_cross_entropy": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, C.POINTER(FtLinearCeParams)],
+    "ft_grad_list_create": [_P, _Z, C.POINTER(_P), C.POINTER(_Z), C.POINTER(_I), C.POINTER(_P)],
+    "ft_grad_list_destroy": [_P],
+    "ft_global_grad_norm": [_P, _P, _F, _P],
+    "ft_clip_grad_global_norm": [_P, _P, _P, _F, _F, _P],
     "ft_embedding_gather": [_P, _P, _P, _P, _I, _I, _I],
     "ft_argmax_rows": [_P, _P, _P, _I, _I],
     "ft_model_create": [_P, C.POINTER(FtModelConfig), C.POINTER(_P)],

@@ -31,7 +31,8 @@ extern "C" const char* ft_build_info(void) {
          "gemm_tcgen05_f16 (TMA + TMEM)\n"
          "attention_fwd_simt_f32\nattention_bwd_simt_f32\n"
          "rms_norm\nrms_norm_backward\nrope\nsilu_gate\nmasked_cross_entropy\n"
-         "sum_squares\nadamw\napply_fused\nembedding_gather\n";
+         "sum_squares\nadamw\napply_fused\nembedding_gather\n"
+         "linear_cross_entropy\nglobal_grad_norm\n";
 }
 
 extern "C" int ft_ctx_create(int device, void* stream, FtContext** out) {

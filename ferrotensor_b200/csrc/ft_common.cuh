@@ -153,6 +153,22 @@ inline cudaError_t ft_launch_ex(FtContext* ctx, void (*kernel)(KArgs...), dim3 g
 // calls safe; growth synchronises the stream before the old block is released.
 int ft_scratch(FtContext* ctx, size_t bytes, void** out);
 
+// Makes the context's device current for a scope.  Launches and attribute queries need it when
+// the calling thread works on several devices.
+struct FtDeviceScope {
+  int prev = -1;
+  bool restore = false;
+  explicit FtDeviceScope(const FtContext* ctx) {
+    if (cudaGetDevice(&prev) == cudaSuccess && prev != ctx->device)
+      restore = cudaSetDevice(ctx->device) == cudaSuccess;
+  }
+  ~FtDeviceScope() {
+    if (restore) cudaSetDevice(prev);
+  }
+  FtDeviceScope(const FtDeviceScope&) = delete;
+  FtDeviceScope& operator=(const FtDeviceScope&) = delete;
+};
+
 static inline size_t ft_align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 static inline int ft_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 

@@ -1,0 +1,86 @@
+// What the files of the linear cross entropy share: the problem, the row bookkeeping in the
+// workspace and the way the workspace is cut up.
+#pragma once
+
+#include <algorithm>
+
+#include "ft_common.cuh"
+
+namespace ft_ce {
+
+// |g| is at most max |s w|; the power of two that brings that bound into [2^13, 2^14) keeps a
+// probability down to 2^-27 in f16's normal range with a factor of four to spare at the top.
+constexpr int G_EXP = 14;
+
+// Written by k_ce_gather, read by every kernel after it.
+struct Head {
+  int count;          // supervised rows
+  float g_scale;      // power of two that g carries while it is held in f16
+  float g_unscale;
+};
+
+// Per packed row, except where noted.
+struct Rows {
+  Head* head;
+  int* place;         // [source row] its packed row, -1 for a skipped one
+  int* source;        // its row in the caller's tensors
+  uint32_t* target;
+  float* weight;      // grad_scale * weights[row]
+  float2* stat;       // running {maximum, sum of exponentials against it}
+  float* picked;      // logit of the target
+  float* lse;
+};
+
+struct Problem {
+  FtLinearCeParams p;
+  int T, H, V;
+  bool grad_hidden, grad_weight;
+};
+
+struct Tensors {
+  const void *hidden, *weight;
+  const uint32_t* targets;
+  const float* weights;
+  float* row_loss;
+  void *grad_hidden, *grad_weight;
+};
+
+// Cuts 256-byte aligned pieces off a block; with a null base it only adds up their sizes.
+class Carver {
+ public:
+  explicit Carver(void* base) : base_((uintptr_t)base), at_(ft_align_up((uintptr_t)base, 256)) {}
+  template <typename T>
+  T* take(size_t count) {
+    T* p = (T*)at_;
+    at_ += ft_align_up(count * sizeof(T), 256);
+    return p;
+  }
+  // 256 bytes more than the sum: the base may begin anywhere
+  size_t bytes() const { return (size_t)(at_ - base_) + 256; }
+
+ private:
+  uintptr_t base_, at_;
+};
+
+inline Rows carve_rows(Carver& c, int T) {
+  Rows r;
+  r.head = c.take<Head>(1);
+  r.place = c.take<int>(T);
+  r.source = c.take<int>(T);
+  r.target = c.take<uint32_t>(T);
+  r.weight = c.take<float>(T);
+  r.stat = c.take<float2>(T);
+  r.picked = c.take<float>(T);
+  r.lse = c.take<float>(T);
+  return r;
+}
+
+// Rows that a block of k_ce_gather packs.  Each block reads all targets, so the number of blocks is
+// bounded: 1024 of them read at most 1024 x 4 x rows bytes, a small share of any product's time.
+inline int gather_rows(int T) { return std::max(8, ft_cdiv(T, 1024)); }
+
+// Reference point for exponentials of a row whose maximum is m: a row that is -inf throughout
+// would otherwise meet (-inf) - (-inf).
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+}  // namespace ft_ce

@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import FtAdamParams, FtAttnParams, FtError, call
+from ._lib import FtAdamParams, FtAttnParams, FtError, FtLinearCeParams, call
 
 MASKED_CE_SKIP = _lib.FT_MASKED_CE_SKIP
 SUM_SQUARES_CHUNK = _lib.FT_SUM_SQUARES_CHUNK
@@ -111,6 +111,14 @@ class CudaContext:
         n = C.c_uint64()
         call("ft_ctx_launch_count", self.handle, C.byref(n))
         return n.value
+
+    def temporary(self, nbytes: int) -> torch.Tensor:
+        """Device memory for one call: allocated on the context's stream, so that it may be released
+        as soon as the call has been made, whatever stream is current."""
+        if torch.cuda.current_stream(self.device) == self.stream:
+            return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        with torch.cuda.stream(self.stream):
+            return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
 
     def adapter_info(self) -> str:
         p = torch.cuda.get_device_properties(self.device)
@@ -257,6 +265,43 @@ class AdamParams:
 def _require(cond: bool, msg: str) -> None:
     if not cond:
         raise FtError(1, msg)
+
+
+_TYPE_CODE = {DType.F32: _lib.FT_TYPE_F32, DType.FP16: _lib.FT_TYPE_F16}
+
+
+class GradientList:
+    """The tensors that a norm or a clip runs over (F32 or FP16, any shapes), laid out once for the
+    device.  It keeps the tensors alive; every call reads their values anew."""
+
+    def __init__(self, ctx: CudaContext, tensors: Sequence[UnifiedTensor]):
+        self.ctx, self.tensors, self.handle = ctx, list(tensors), None
+        for i, t in enumerate(self.tensors):
+            _require(t.dtype in _TYPE_CODE, f"GradientList: tensor {i} is {t.dtype}, expected F32 or FP16")
+            _require(t.storage.device == ctx.device, f"GradientList: tensor {i} is on {t.storage.device}")
+            _require(t.size_in_bytes() <= t.storage.numel() * t.storage.element_size(),
+                     f"GradientList: tensor {i} is larger than its buffer")
+        n = len(self.tensors)
+        ptrs = (C.c_void_p * n)(*[t.storage.data_ptr() for t in self.tensors])
+        counts = (C.c_size_t * n)(*[t.numel() for t in self.tensors])
+        types = (C.c_int * n)(*[_TYPE_CODE[t.dtype] for t in self.tensors])
+        handle = C.c_void_p()
+        call("ft_grad_list_create", ctx.handle, n, ptrs, counts, types, C.byref(handle))
+        self.handle = handle
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+    def close(self) -> None:
+        if self.handle and self.ctx.handle:
+            call("ft_grad_list_destroy", self.handle)
+        self.handle = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class ComputeEngine:
@@ -425,6 +470,84 @@ class ComputeEngine:
                  "masked_cross_entropy: shape mismatch")
         call("ft_masked_cross_entropy_weighted", ctx.handle, logits.ptr, targets.ptr, weights.ptr,
              grad.ptr, row_loss.ptr, rows, vocab)
+
+    # ---- lfm.rs:597-623 and training.rs:207-258 in one: no logits are kept
+    def linear_cross_entropy(self, ctx, hidden, weight, targets, weights, row_loss, grad_hidden=None,
+                             grad_weight=None, grad_scale=1.0, vocab_piece=0, workspace=None):
+        """Row losses of `hidden` [..., hidden] x `weight` [hidden, vocab] against `targets`, and on
+        request the gradients of sum(grad_scale * weights * loss) with respect to either operand.
+        Operands and gradients are F32 or FP16 each.  `workspace` (any UnifiedTensor with
+        `linear_cross_entropy_workspace` bytes) saves the call an allocation."""
+        self._linear_ce(ctx, hidden, weight, targets, weights, row_loss, grad_hidden, grad_weight, grad_scale,
+                        vocab_piece, workspace, 0)
+
+    def linear_cross_entropy_bt(self, ctx, hidden, weight, targets, weights, row_loss, grad_hidden=None,
+                                grad_weight=None, grad_scale=1.0, vocab_piece=0, workspace=None):
+        """The same with `weight` (and its gradient) as [vocab, hidden], the layout of an embedding."""
+        self._linear_ce(ctx, hidden, weight, targets, weights, row_loss, grad_hidden, grad_weight, grad_scale,
+                        vocab_piece, workspace, 1)
+
+    def linear_cross_entropy_workspace(self, ctx, hidden, weight, grad_hidden=None, grad_weight=None,
+                                       vocab_piece=0, vocab_major=False) -> int:
+        """Bytes of workspace that a call with these tensors needs in the context's GEMM mode."""
+        p = self._linear_ce_params(hidden, weight, grad_hidden, grad_weight, 1.0, vocab_piece, int(vocab_major))
+        n = C.c_size_t()
+        call("ft_linear_cross_entropy_workspace", ctx.handle, C.byref(p), grad_hidden is not None,
+             grad_weight is not None, C.byref(n))
+        return n.value
+
+    @staticmethod
+    def _linear_ce_params(hidden, weight, grad_hidden, grad_weight, grad_scale, vocab_piece, vocab_major):
+        _require(len(weight.shape) == 2, "linear_cross_entropy: weight must be 2-D")
+        vocab, h = weight.shape if vocab_major else weight.shape[::-1]
+        _require(len(hidden.shape) >= 1 and hidden.shape[-1] == h, "linear_cross_entropy: hidden and weight do not fit")
+        rows = _numel(hidden.shape[:-1])
+        for t, like, name in ((hidden, None, "hidden"), (weight, None, "weight"), (grad_hidden, hidden, "grad_hidden"),
+                              (grad_weight, weight, "grad_weight")):
+            if t is None:
+                continue
+            _require(t.dtype in _TYPE_CODE, f"linear_cross_entropy: {name} must be F32 or FP16")
+            _require(like is None or t.numel() == like.numel(), f"linear_cross_entropy: {name} has the wrong size")
+        code = [_TYPE_CODE[t.dtype] if t is not None else 0 for t in (hidden, weight, grad_hidden, grad_weight)]
+        _require(0 <= vocab_piece < 1 << 32, "linear_cross_entropy: vocab_piece is out of range")
+        _require(max(rows, h, vocab) < 1 << 32, "linear_cross_entropy: a dimension is out of range")
+        return FtLinearCeParams(rows, h, vocab, vocab_major, *code, vocab_piece, grad_scale)
+
+    def _linear_ce(self, ctx, hidden, weight, targets, weights, row_loss, grad_hidden, grad_weight, grad_scale,
+                   vocab_piece, workspace, vocab_major):
+        p = self._linear_ce_params(hidden, weight, grad_hidden, grad_weight, grad_scale, vocab_piece, vocab_major)
+        _require(targets.dtype is DType.U32 and targets.numel() == p.rows, "linear_cross_entropy: one U32 target per row")
+        _require(row_loss.dtype is DType.F32 and row_loss.numel() == p.rows, "linear_cross_entropy: one F32 loss per row")
+        _require(weights is None or (weights.dtype is DType.F32 and weights.numel() == p.rows),
+                 "linear_cross_entropy: one F32 weight per row")
+        if workspace is None:
+            n = C.c_size_t()
+            call("ft_linear_cross_entropy_workspace", ctx.handle, C.byref(p), grad_hidden is not None,
+                 grad_weight is not None, C.byref(n))
+            workspace = ctx.temporary(n.value)
+        else:
+            workspace = workspace.storage
+        call("ft_linear_cross_entropy", ctx.handle, hidden.ptr, weight.ptr, targets.ptr,
+             weights.ptr if weights is not None else None, row_loss.ptr,
+             grad_hidden.ptr if grad_hidden is not None else None,
+             grad_weight.ptr if grad_weight is not None else None,
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), C.byref(p))
+
+    # ---- trainer/lib.rs:328-343: the norm over all gradients, and the clip by it
+    def global_grad_norm(self, ctx, grads: GradientList, norm_out, grad_scale=1.0):
+        """norm_out (F32, 4 values): {norm, 1 or 0 when it is not finite, grad_scale, unused}."""
+        _require(norm_out.dtype is DType.F32 and norm_out.numel() >= 4, "global_grad_norm: norm_out holds 4 F32 values")
+        call("ft_global_grad_norm", ctx.handle, grads.handle, float(grad_scale), norm_out.ptr)
+
+    def clip_grad_global_norm(self, ctx, grads: GradientList, max_norm, norm_out=None, grad_scale=1.0,
+                              out: Optional[GradientList] = None):
+        """Scales every gradient by grad_scale and, when the norm exceeds max_norm > 0, by
+        max_norm / (norm + 1e-6): in place, or into the tensors of `out`.  A norm that is not finite
+        writes nothing but norm_out = {norm, applied, factor, unused}."""
+        _require(norm_out is None or (norm_out.dtype is DType.F32 and norm_out.numel() >= 4),
+                 "clip_grad_global_norm: norm_out holds 4 F32 values")
+        call("ft_clip_grad_global_norm", ctx.handle, grads.handle, out.handle if out is not None else None,
+             float(grad_scale), float(max_norm), norm_out.ptr if norm_out is not None else None)
 
     # ---- misc.rs:20-34
     def argmax_rows(self, ctx, input, out_idx):

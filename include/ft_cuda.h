@@ -201,6 +201,51 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
                                      const uint32_t* targets, const float* weights, float* grad,
                                      float* row_loss, int rows, int vocab);
 
+/* Storage type of an operand that may be either. */
+#define FT_TYPE_F32 0
+#define FT_TYPE_F16 1
+
+/* ---- linear cross entropy: the output projection and ft_masked_cross_entropy_weighted in one
+ * (ferrotensor-graph/src/lfm.rs:597-623, engine/training.rs:207-258), for a vocabulary too large
+ * to keep the logits.  With z[t, v] = sum_k hidden[t, k] W(k, v) and lse_t = log sum_v exp z[t, v]:
+ *   row_loss[t] = lse_t - z[t, targets[t]]
+ *   g[t, v]     = grad_scale * weights[t] * (exp(z[t, v] - lse_t) - (v == targets[t]))
+ *   grad_hidden = g W^T,   grad_weight = hidden^T g (in the layout of the weight)
+ * targets[t] == FT_MASKED_CE_SKIP gives zero loss and a zero gradient, whatever the row holds
+ * (its hidden values are not read); another target >= vocab gives zero loss and the gradient
+ * without its one-hot term, as ft_masked_cross_entropy_weighted does.
+ *   hidden      [rows, hidden]  hidden_type
+ *   weight      weight_type, [hidden, vocab] as ft_matmul's b, or with weight_vocab_major
+ *               [vocab, hidden] as ft_matmul_bt's
+ *   weights     f32 [rows]; may be NULL when no gradient is asked for
+ *   row_loss    f32 [rows]
+ *   grad_hidden [rows, hidden] grad_hidden_type, or NULL
+ *   grad_weight grad_weight_type, shaped like the weight, or NULL
+ * The context's GEMM mode chooses the arithmetic of the products: FT_GEMM_F32 exact f32 FMA,
+ * FT_GEMM_F16 operands and g rounded to f16, FT_GEMM_F16X2 f32 operands and g carried as two f16
+ * halves.  (f16 operands are exact in every mode; sums are f32 in every mode.)
+ * The vocabulary is worked through in pieces of vocab_piece columns (0: chosen by size), of which
+ * only one piece of g exists at a time; workspace holds it and must have the bytes that
+ * ft_linear_cross_entropy_workspace gives for the same arguments, context and GEMM mode.  The
+ * call allocates nothing, keeps nothing there for a later call, and may be captured into a
+ * graph; calls that overlap on the GPU need workspaces of their own.  Outputs may overlap no
+ * input, no other output and not the workspace.
+ * Limits: rows <= 2^24, hidden <= 2^16, vocab <= 2^24. */
+typedef struct FtLinearCeParams {
+  uint32_t rows, hidden, vocab;
+  uint32_t weight_vocab_major;
+  uint32_t hidden_type, weight_type;           /* FT_TYPE_*                              */
+  uint32_t grad_hidden_type, grad_weight_type;
+  uint32_t vocab_piece;
+  float grad_scale;
+} FtLinearCeParams;
+int ft_linear_cross_entropy_workspace(FtContext* ctx, const FtLinearCeParams* p,
+                                      int want_grad_hidden, int want_grad_weight, size_t* bytes);
+int ft_linear_cross_entropy(FtContext* ctx, const void* hidden, const void* weight,
+                            const uint32_t* targets, const float* weights, float* row_loss,
+                            void* grad_hidden, void* grad_weight, void* workspace,
+                            size_t workspace_bytes, const FtLinearCeParams* p);
+
 /* ---- optimizer side: engine/training.rs:15-32,54-77,161-171,263-290;
  * kernels.wgsl:355-387,661-670,713-735. */
 typedef struct FtAdamParams {
@@ -213,6 +258,32 @@ int ft_sum_squares_partial(FtContext* ctx, const float* x, size_t n, float* out,
 int ft_clip_grad_by_norm(FtContext* ctx, float* g, size_t n, float scale);
 int ft_adamw_update(FtContext* ctx, float* w, const float* g, float* m, float* v, size_t n,
                     const FtAdamParams* p);
+
+/* ---- global gradient norm and clipping over many tensors: the trainer's global_grad_norm and
+ * clip (ferrotensor-trainer/src/lib.rs:328-343) without its read-back and its launches for each
+ * tensor.  A list names `count` tensors (device pointer, elements, FT_TYPE_*; aligned to their
+ * element size, empty ones allowed, FT_ERR_INVALID otherwise).  The tensors stay the caller's and
+ * must live as long as the list; their values are read anew by every call.  Creating a list
+ * allocates and copies (not inside a stream capture), calls on it do neither.  A list belongs to
+ * its context: calls on it run in the order of the context's stream, and graphs that hold calls
+ * on one list must not run at the same time.
+ * norm_out: device f32[4] = {norm, applied, factor, unused}, as ft_model_apply_gradients:
+ *   norm    = |grad_scale| * sqrt(sum of all squares), squares and sums in f64
+ *   applied = 1, or 0 when the norm is not finite in f32
+ *   factor  = grad_scale, times max_norm / (norm + 1e-6) when norm > max_norm > 0
+ * ft_global_grad_norm only measures (factor = grad_scale).  ft_clip_grad_global_norm also writes
+ * factor * g to the tensors of `out` (same counts, its own types; out == grads or NULL: in
+ * place).  Nothing is written when the norm is not finite, nor in place when the factor is 1.
+ * The tensors of `out` may not overlap one another, and may overlap only the tensor of `grads`
+ * that they replace, exactly and in the same type.  norm_out may be NULL for the clip and may
+ * overlap no tensor of either list.  Results do not depend on scheduling. */
+typedef struct FtGradList FtGradList;
+int ft_grad_list_create(FtContext* ctx, size_t count, void* const* ptrs, const size_t* elements,
+                        const int* types, FtGradList** out);
+int ft_grad_list_destroy(FtGradList* list);
+int ft_global_grad_norm(FtContext* ctx, FtGradList* grads, float grad_scale, float* norm_out);
+int ft_clip_grad_global_norm(FtContext* ctx, FtGradList* grads, FtGradList* out, float grad_scale,
+                             float max_norm, float* norm_out);
 
 /* engine/misc.rs:20-34 argmax_rows: for each of `rows` rows of `len` f32 values, the index of
  * the largest in f32::total_cmp order, the last index winning ties (a greedy token). */
