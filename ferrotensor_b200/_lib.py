@@ -119,7 +119,7 @@ PROTOTYPES = {
     "ft_sum_squares_partial": [_P, _P, _Z, _P, _Z, C.POINTER(_Z)],
     "ft_clip_grad_by_norm": [_P, _P, _Z, _F],
     "ft_adamw_update": [_P, _P, _P, _P, _P, _Z, C.POINTER(FtAdamParams)],
-    "ft_linear_cross_entropy_workspace": [_P, C.POINTER(FtLinearCeParams), _I, _I, C.POINTER(_Z)],
+    "ft_linear_cross_entropy_workspace": [_P, _P, C.POINTER(FtLinearCeParams), _I, _I, C.POINTER(_Z)],
     "ft_linear_cross_entropy": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, C.POINTER(FtLinearCeParams)],
     "ft_grad_list_create": [_P, _Z, C.POINTER(_P), C.POINTER(_Z), C.POINTER(_I), C.POINTER(_P)],
     "ft_grad_list_destroy": [_P],

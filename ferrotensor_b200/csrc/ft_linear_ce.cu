@@ -39,14 +39,50 @@ __device__ __forceinline__ int block_sum_int(int v, int* red) {
   return s;
 }
 
+// One row -> f16 (and its rounding remainder, when `lo` is given), eight values a lane.
+template <typename TH>
+__device__ __forceinline__ void pack_row(const TH* __restrict__ from, int H, float S, __half* __restrict__ hi, int ld,
+                                         __half* __restrict__ lo, int lane) {
+  const bool vec = (((uintptr_t)from) & 15) == 0;
+  for (int c = lane * 8; c < ld; c += 256) {
+    if constexpr (sizeof(TH) == 2) {
+      if (vec && c + 8 <= H) {
+        *(uint4*)(hi + c) = *(const uint4*)(from + c);
+        continue;
+      }
+    }
+    float v[8];
+    if (vec && c + 8 <= H && sizeof(TH) == 4) {
+      const float4 a = *(const float4*)(from + c), b = *(const float4*)(from + c + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < H ? (float)from[c + k] : 0.f;
+    }
+    __half2 h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = v[2 * k] * S, b = v[2 * k + 1] * S;
+      h[k] = __floats2half2_rn(a, b);
+      const float2 f = __half22float2(h[k]);
+      l[k] = __floats2half2_rn(a - f.x, b - f.y);
+    }
+    *(uint4*)(hi + c) = *(const uint4*)h;
+    if (lo) *(uint4*)(lo + c) = *(const uint4*)l;
+  }
+}
+
 // One block packs rows [blockIdx.x * per, ...).  Every block counts the supervised rows of the
 // whole batch itself (targets are 4 bytes a row and come from L2), which gives it the place of its
 // first row and the total without a launch of its own or a wait on its neighbours.
-template <typename TH>
+// TO = __half: as `planes` f16 planes of `plane_rows` rows, times the power of two of the largest
+// value where they are f32, and with zero rows up to the next multiple of 64 (a K block of dW).
+template <typename TH, typename TO>
 __global__ void __launch_bounds__(GATHER_THREADS)
 k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
             const float* __restrict__ weights, float grad_scale, int rows, int H, int per, Rows rw,
-            float* __restrict__ out, float* __restrict__ row_loss) {
+            TO* __restrict__ out, int ld, int plane_rows, int planes, int w_scaled,
+            float* __restrict__ row_loss) {
   __shared__ int red[GATHER_THREADS / 32];
   __shared__ float redf[GATHER_THREADS / 32];
   __shared__ int src_row[GATHER_THREADS];
@@ -54,6 +90,7 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
   ft_pdl_launch();
   const int r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(rw.head->h_amax, OPERAND_EXP) : 1.f;
   int before = 0, all = 0;
   float big = 0.f;
   for (int i = tid; i < rows; i += GATHER_THREADS) {
@@ -71,15 +108,16 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
     __syncthreads();
     if (tid == 0) {
       for (int w = 1; w < GATHER_THREADS / 32; ++w) big = fmaxf(big, redf[w]);
-      float S = 1.0f;
-      if (big > 0.f && isfinite(big)) {
-        int e;
-        frexpf(big, &e);
-        S = ldexpf(1.0f, G_EXP - e);
-      }
+      const float S = power_for(__float_as_int(big), G_EXP);
       rw.head->count = all;
       rw.head->g_scale = S;
       rw.head->g_unscale = 1.0f / S;
+      if constexpr (sizeof(TO) == 2) {
+        const float wu = w_scaled ? 1.0f / power_for(rw.head->w_amax, OPERAND_EXP) : 1.0f;
+        rw.head->h_unscale = 1.0f / h_scale;
+        rw.head->w_unscale = wu;
+        rw.head->z_scale = wu / h_scale;
+      }
     }
   }
   int at = before;
@@ -109,11 +147,22 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
     __syncthreads();
     for (int k = warp; k < total; k += GATHER_THREADS / 32) {
       const TH* from = hidden + (size_t)src_row[k] * H;
-      float* to = out + (size_t)(at + k) * H;
-      for (int c = lane; c < H; c += 32) to[c] = (float)from[c];
+      TO* to = out + (size_t)(at + k) * ld;
+      if constexpr (sizeof(TO) == 4) {
+        for (int c = lane; c < H; c += 32) to[c] = (float)from[c];
+      } else {
+        pack_row(from, H, h_scale, to, ld, planes == 2 ? to + (size_t)plane_rows * ld : nullptr, lane);
+      }
     }
     at += total;
     __syncthreads();
+  }
+  if constexpr (sizeof(TO) == 2) {
+    const int end = max(64, (all + 63) / 64 * 64);
+    for (int p = 0; p < planes; ++p)
+      for (int r = all + (int)blockIdx.x * (GATHER_THREADS / 32) + warp; r < end; r += gridDim.x * (GATHER_THREADS / 32))
+        for (int c = lane * 8; c < ld; c += 256)
+          *(uint4*)(out + ((size_t)p * plane_rows + r) * ld + c) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -274,6 +323,21 @@ struct ExactPlan {
   size_t bytes;
 };
 
+template <typename TO>
+int launch_gather(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, TO* out, int ld, int plane_rows,
+                  int planes) {
+  const int per = gather_rows(q.T), blocks = ft_cdiv(q.T, per);
+  if (q.p.hidden_type == FT_TYPE_F16)
+    FT_LAUNCH_PDL(ctx, (k_ce_gather<__half, TO>), blocks, GATHER_THREADS, 0, (const __half*)t.hidden, t.targets, t.weights,
+                  q.p.grad_scale, q.T, q.H, per, rw, out, ld, plane_rows, planes,
+                  q.p.weight_type == FT_TYPE_F32 ? 1 : 0, t.row_loss);
+  else
+    FT_LAUNCH_PDL(ctx, (k_ce_gather<float, TO>), blocks, GATHER_THREADS, 0, (const float*)t.hidden, t.targets, t.weights,
+                  q.p.grad_scale, q.T, q.H, per, rw, out, ld, plane_rows, planes,
+                  q.p.weight_type == FT_TYPE_F32 ? 1 : 0, t.row_loss);
+  return FT_OK;
+}
+
 ExactPlan exact_plan(const Problem& q, void* base) {
   ExactPlan pl;
   Carver c(base);
@@ -304,13 +368,7 @@ int launch_exact(FtContext* ctx, const ExactProduct& p, bool b_f16, bool c_f16, 
 int exact_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   const ExactPlan pl = exact_plan(q, ws);
   const int T = q.T, H = q.H, V = q.V;
-  const int per = gather_rows(T), blocks = ft_cdiv(T, per);
-  if (q.p.hidden_type == FT_TYPE_F16)
-    FT_LAUNCH_PDL(ctx, k_ce_gather<__half>, blocks, GATHER_THREADS, 0, (const __half*)t.hidden, t.targets, t.weights,
-                  q.p.grad_scale, T, H, per, pl.rows, pl.hidden, t.row_loss);
-  else
-    FT_LAUNCH_PDL(ctx, k_ce_gather<float>, blocks, GATHER_THREADS, 0, (const float*)t.hidden, t.targets, t.weights,
-                  q.p.grad_scale, T, H, per, pl.rows, pl.hidden, t.row_loss);
+  FT_TRY(launch_gather<float>(ctx, q, t, pl.rows, pl.hidden, H, T, 1));
   const bool w16 = q.p.weight_type == FT_TYPE_F16;
   const long long swk = q.p.weight_vocab_major ? 1 : V, swv = q.p.weight_vocab_major ? H : 1;   // strides of W(k, v)
   const size_t we = w16 ? 2 : 4;
@@ -382,12 +440,17 @@ size_t type_size(uint32_t t) { return t == FT_TYPE_F16 ? 2 : 4; }
 
 }  // namespace
 
-extern "C" int ft_linear_cross_entropy_workspace(FtContext* ctx, const FtLinearCeParams* p, int want_grad_hidden,
-                                                 int want_grad_weight, size_t* bytes) {
+int ft_ce::launch_gather_f16(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, __half* out, int ld,
+                             int plane_rows, int planes) {
+  return launch_gather<__half>(ctx, q, t, rw, out, ld, plane_rows, planes);
+}
+
+extern "C" int ft_linear_cross_entropy_workspace(FtContext* ctx, const void* weight, const FtLinearCeParams* p,
+                                                 int want_grad_hidden, int want_grad_weight, size_t* bytes) {
   FT_TRY(check_params("ft_linear_cross_entropy_workspace", ctx, p));
   FT_REQUIRE(bytes, "ft_linear_cross_entropy_workspace: NULL argument");
   const Problem q = make_problem(*p, want_grad_hidden != 0, want_grad_weight != 0);
-  *bytes = exact_plan(q, nullptr).bytes;
+  *bytes = ctx->gemm_mode == FT_GEMM_F32 ? exact_plan(q, nullptr).bytes : tc_workspace(ctx, q, weight);
   return FT_OK;
 }
 
@@ -400,7 +463,7 @@ extern "C" int ft_linear_cross_entropy(FtContext* ctx, const void* hidden, const
   FT_REQUIRE(weight && (!T || (hidden && targets && row_loss)), "%s: NULL argument", who);
   FT_REQUIRE(weights || !T || (!grad_hidden && !grad_weight), "%s: a gradient needs the rows' weights", who);
   size_t need = 0;
-  FT_TRY(ft_linear_cross_entropy_workspace(ctx, p, grad_hidden != nullptr, grad_weight != nullptr, &need));
+  FT_TRY(ft_linear_cross_entropy_workspace(ctx, weight, p, grad_hidden != nullptr, grad_weight != nullptr, &need));
   FT_REQUIRE(workspace && workspace_bytes >= need, "%s: the workspace has %zu bytes, %zu are needed", who,
              workspace ? workspace_bytes : (size_t)0, need);
   struct Range { const char* name; const void* p; size_t bytes; size_t align; };
@@ -430,5 +493,5 @@ extern "C" int ft_linear_cross_entropy(FtContext* ctx, const void* hidden, const
   }
   const Problem q = make_problem(*p, grad_hidden != nullptr, grad_weight != nullptr);
   const Tensors t = {hidden, weight, targets, weights, row_loss, grad_hidden, grad_weight};
-  return exact_path(ctx, q, t, workspace);
+  return ctx->gemm_mode == FT_GEMM_F32 ? exact_path(ctx, q, t, workspace) : tc_path(ctx, q, t, workspace);
 }

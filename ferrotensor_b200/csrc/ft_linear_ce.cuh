@@ -11,12 +11,26 @@ namespace ft_ce {
 // |g| is at most max |s w|; the power of two that brings that bound into [2^13, 2^14) keeps a
 // probability down to 2^-27 in f16's normal range with a factor of four to spare at the top.
 constexpr int G_EXP = 14;
+// an f32 operand is brought to the same range before it is split into f16 planes
+constexpr int OPERAND_EXP = 14;
+
+// The power of two that brings the magnitude with these bits into [2^(exp-1), 2^exp).
+__device__ __forceinline__ float power_for(int bits, int exp) {
+  const float amax = __int_as_float(bits);
+  if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
+  int e;
+  frexpf(amax, &e);
+  return ldexpf(1.f, min(exp - e, 100));
+}
 
 // Written by k_ce_gather, read by every kernel after it.
 struct Head {
   int count;          // supervised rows
   float g_scale;      // power of two that g carries while it is held in f16
   float g_unscale;
+  float h_scale, h_unscale, w_unscale;   // of the f16 planes of f32 operands, else 1
+  float z_scale;      // h_unscale * w_unscale
+  int h_amax, w_amax; // bits of the f32 operands' largest finite magnitudes
 };
 
 // Per packed row, except where noted.
@@ -78,6 +92,13 @@ inline Rows carve_rows(Carver& c, int T) {
 // Rows that a block of k_ce_gather packs.  Each block reads all targets, so the number of blocks is
 // bounded: 1024 of them read at most 1024 x 4 x rows bytes, a small share of any product's time.
 inline int gather_rows(int T) { return std::max(8, ft_cdiv(T, 1024)); }
+
+// ft_linear_ce_tc.cu
+size_t tc_workspace(const FtContext* ctx, const Problem& q, const void* weight);
+int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws);
+// ft_linear_ce.cu: packs the supervised rows as f16 planes [planes][plane_rows][ld]
+int launch_gather_f16(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, __half* out, int ld,
+                      int plane_rows, int planes);
 
 // Reference point for exponentials of a row whose maximum is m: a row that is -inf throughout
 // would otherwise meet (-inf) - (-inf).

@@ -1,0 +1,828 @@
+// The products of the linear cross entropy on the tensor cores (FT_GEMM_F16 and FT_GEMM_F16X2).
+//
+// One kernel serves all of them: C[256 x 256 tile] = sum over (plane pairs, K) of A . B^T on a CTA
+// pair (tcgen05 cta_group::2), with either operand K-contiguous or M/N-contiguous in memory, so no
+// operand is ever transposed:
+//   logits   A = packed rows,    B = W            K = hidden    epilogue: row statistics, or g
+//   dh       A = g,              B = W            K = a vocabulary piece (in `splits` parts)
+//   dW       A = g, B = rows (W is [vocab, hidden]) or A = rows, B = g ([hidden, vocab])   K = rows
+//
+// Planes: an f16 operand, and an f32 one in FT_GEMM_F16, is one f16 plane.  FT_GEMM_F16X2 carries an
+// f32 operand and g as two planes, hi = f16(x) and lo = f16(x - hi), of which the products hi.hi,
+// hi.lo and lo.hi are summed: 22 bits.  The tensor core adds each group of 16 products into its f32
+// accumulator with the low bits cut off, a loss of up to K/16 x 2^-24 of the sum, so that mode also
+// sums at most SLICE_KB x 64 of K in tensor memory and adds the slices up in registers.
+//
+// Roles and barriers as in ft_gemm_tc.cu's pair kernel: warp 0 loads (TMA), warp 1 of the even CTA
+// issues the products, warps 2..9 drain.  Every wait is bounded; a wait that runs out sets the
+// status word, and all roles fall through.
+#include <math.h>
+#include <string.h>
+
+#include "ft_linear_ce.cuh"
+#include "ft_tc.cuh"
+
+namespace {
+
+using namespace ft_tc;
+using namespace ft_ce;
+
+constexpr int TILE = 256;                 // rows and columns of a pair's tile
+constexpr int STAGES = 6;
+constexpr int OPERAND_BYTES = 128 * BK * 2;
+constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int EPI_OFFSET = STAGES * STAGE_BYTES;      // 8 epilogue warps x 4 KiB
+constexpr int BAR_OFFSET = EPI_OFFSET + 8 * 4096;
+constexpr int SMEM_BYTES = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
+constexpr int SLICE_KB = 8;
+
+enum Epi { EPI_STATS, EPI_GRAD, EPI_STORE };
+
+struct TcProduct {
+  int M, N, K;
+  int live_m, live_k;               // 1: that extent is the number of supervised rows
+  int splits;                       // parts of K, each with a slab of its own
+  int n_fast, band;                 // order of the tiles
+  int terms;                        // plane pairs, the small ones first
+  int a_plane[3], b_plane[3];
+  int a_mn0, b_mn0, k0;             // where M, N and K begin in the operands' tensors...
+  int a_has_k0, b_has_k0;           // ... and which of them k0 applies to
+  // EPI_STATS, EPI_GRAD
+  Rows rw;
+  float2* part;                     // [2 * column tiles][part_ld]
+  int part_ld;
+  int v0, vocab;                    // first vocabulary column of the launch, columns in all
+  int g_planes;
+  // EPI_STORE
+  int out_type;                     // FT_TYPE_*
+  int accumulate;
+  int unscale;                      // multiply by the scales of g and of the rows
+  int out_x0, out_y0;
+  void* direct;                     // when the output breaks a TMA rule: plain stores
+  long long direct_ld;
+};
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t leader_bar, int c0,
+                                                 int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"((uint64_t)map),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   (uint64_t)map),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// the staging tile may be written again: the copies have read it
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Unit { int mt, nt, sp; };
+__device__ __forceinline__ Unit decode_unit(int u, int tiles_m, int tiles_n, const TcProduct& g) {
+  Unit r;
+  if (g.n_fast) {
+    r.nt = u % tiles_n;
+    const int v = u / tiles_n;
+    r.sp = v % g.splits;
+    r.mt = v / g.splits;
+  } else {
+    const int per_band = g.band * tiles_n * g.splits;
+    const int b = u / per_band, in = u - b * per_band;
+    const int rows = min(g.band, tiles_m - b * g.band);
+    r.mt = b * g.band + in % rows;
+    const int v = in / rows;
+    r.nt = v % tiles_n;
+    r.sp = v / tiles_n;
+  }
+  return r;
+}
+
+// The 32 x 32 block of a warp (a row a lane, 32 consecutive f32 columns) -> its staging tile, in the
+// 128-byte swizzle of the output map: 16-byte unit j of row r at unit j ^ (r & 7).
+__device__ __forceinline__ void stage_f32(uint8_t* st, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *(float4*)(st + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+// half `part` (32 columns, 64 bytes) of a 64-column f16 row
+__device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const uint32_t (&h)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *(uint4*)(st + lane * 128 + (((part * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+}
+
+template <int EPI, bool A_MN, bool B_MN, bool SPLIT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+          const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t bar_full = base + BAR_OFFSET;
+  const uint32_t bar_empty = bar_full + STAGES * 8;
+  const uint32_t bar_tfull = bar_empty + STAGES * 8;
+  const uint32_t bar_tempty = bar_tfull + 2 * 8;
+  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + (2 * STAGES + 4) * 8);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + s * 8, 1);
+      mbar_init(bar_empty + s * 8, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_tfull + b * 8, 1);
+      mbar_init(bar_tempty + b * 8, 16);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  ft_pdl_wait();
+  ft_pdl_launch();
+
+  const uint32_t lead_full = mapa_shared(bar_full, 0);
+  const uint32_t lead_tempty = mapa_shared(bar_tempty, 0);
+  const int live = g.rw.head->count;
+  // no supervised row at all still makes one tile (of zeros): gradients are overwritten, not left
+  const int tiles_m = g.live_m ? max(1, (live + TILE - 1) / TILE) : (g.M + TILE - 1) / TILE;
+  const int tiles_n = (g.N + TILE - 1) / TILE;
+  const int units = tiles_m * tiles_n * g.splits;
+  const int kb_all = g.live_k ? max(1, (live + BK - 1) / BK) : (g.K + BK - 1) / BK;
+  const int slice = SPLIT ? SLICE_KB : kb_all;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both CTAs)
+    if (elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      const int ak0 = g.a_has_k0 ? g.k0 : 0, bk0 = g.b_has_k0 ? g.k0 : 0;
+      for (int u = pair; u < units && !*abort_flag; u += npairs) {
+        const Unit un = decode_unit(u, tiles_m, tiles_n, g);
+        const int kb0 = (int)((long long)kb_all * un.sp / g.splits), kb1 = (int)((long long)kb_all * (un.sp + 1) / g.splits);
+        const int am = g.a_mn0 + un.mt * TILE + (int)rank * 128, bn = g.b_mn0 + un.nt * TILE + (int)rank * 128;
+        for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice) {
+          const int s1 = min(kb1, s0 + slice);
+          for (int t = 0; t < g.terms; ++t) {
+            const int pa = g.a_plane[t], pb = g.b_plane[t];
+            for (int kb = s0; kb < s1; ++kb) {
+              if (!mbar_wait(bar_empty + stage * 8, phase ^ 1, abort_flag, status, 21)) break;
+              const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OPERAND_BYTES;
+              const uint32_t bar = lead_full + stage * 8;
+              if (rank == 0) mbar_expect_tx(bar_full + stage * 8, 2 * STAGE_BYTES);
+              if constexpr (A_MN) {
+                tma_load_3d_pair(sa, &map_a, bar, am, ak0 + kb * BK, pa);
+                tma_load_3d_pair(sa + 8192, &map_a, bar, am + 64, ak0 + kb * BK, pa);
+              } else {
+                tma_load_3d_pair(sa, &map_a, bar, ak0 + kb * BK, am, pa);
+              }
+              if constexpr (B_MN) {
+                tma_load_3d_pair(sb, &map_b, bar, bn, bk0 + kb * BK, pb);
+                tma_load_3d_pair(sb + 8192, &map_b, bar, bn + 64, bk0 + kb * BK, pb);
+              } else {
+                tma_load_3d_pair(sb, &map_b, bar, bk0 + kb * BK, bn, pb);
+              }
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (leader only)
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = make_idesc(256, 256, 0, 0) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16);
+      uint32_t stage = 0, phase = 0;
+      int local = 0;
+      for (int u = pair; u < units && !*abort_flag; u += npairs) {
+        const Unit un = decode_unit(u, tiles_m, tiles_n, g);
+        const int kb0 = (int)((long long)kb_all * un.sp / g.splits), kb1 = (int)((long long)kb_all * (un.sp + 1) / g.splits);
+        for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice, ++local) {
+          const int todo = (min(kb1, s0 + slice) - s0) * g.terms;
+          const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+          if (!mbar_wait(bar_tempty + buf * 8, acc_phase ^ 1, abort_flag, status, 22)) break;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + buf * TILE;
+          for (int i = 0; i < todo; ++i) {
+            if (!mbar_wait(bar_full + stage * 8, phase, abort_flag, status, 23)) break;
+            tc_fence_after();
+            const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OPERAND_BYTES;
+            const uint64_t da = A_MN ? make_desc_mn_sw128(sa, 8192) : make_desc_sw128(sa);
+            const uint64_t db = B_MN ? make_desc_mn_sw128(sb, 8192) : make_desc_sw128(sb);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k)
+              tc_mma_f16_pair(d_tmem, da + (uint64_t)(k * (A_MN ? 128 : 2)), db + (uint64_t)(k * (B_MN ? 128 : 2)), idesc,
+                              (i > 0 || k > 0) ? 1u : 0u);
+            tc_commit_pair(bar_empty + stage * 8, 3);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          if (*abort_flag) break;
+          tc_commit_pair(bar_tfull + buf * 8, 3);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ epilogue (both CTAs)
+    // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the two warps of a quadrant take 128
+    // columns each, in four chunks of 32.
+    const int quad = warp & 3, grp = (warp - 2) >> 2;
+    uint8_t* st = gbase + EPI_OFFSET + (warp - 2) * 4096;
+    const uint32_t st_addr = smem_u32(st);
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * 128;
+    const float z_scale = g.rw.head->z_scale;                      // accumulator -> logit
+    const float c2 = z_scale * 1.4426950408889634f;                // accumulator -> log2 units
+    // rows that a store may reach: all of a tile where the rows are packed ones (their buffers end with
+    // a tile), else those of the output
+    const int rows_end = g.live_m ? tiles_m * TILE : g.M;
+    int local = 0;
+    for (int u = pair; u < units && !*abort_flag; u += npairs) {
+      const Unit un = decode_unit(u, tiles_m, tiles_n, g);
+      const int kb0 = (int)((long long)kb_all * un.sp / g.splits), kb1 = (int)((long long)kb_all * (un.sp + 1) / g.splits);
+      const int row = un.mt * TILE + (int)rank * 128 + quad * 32 + lane;
+      const int col = un.nt * TILE + grp * 128;                    // first column of this warp, from the launch's first
+      uint32_t target = FT_MASKED_CE_SKIP;
+      float lse2 = 0.f, wg = 0.f, alpha = 1.f;
+      if constexpr (EPI != EPI_STORE) {
+        if (row < live) {
+          target = g.rw.target[row] - (uint32_t)(g.v0 + col);      // relative to this warp's columns
+          if constexpr (EPI == EPI_GRAD) {
+            lse2 = g.rw.lse[row];
+            wg = g.rw.weight[row] * g.rw.head->g_scale;
+          }
+        }
+      } else {
+        if (g.unscale) alpha = g.rw.head->g_unscale * g.rw.head->h_unscale;
+      }
+      float run_m = -INFINITY, run_s = 0.f;
+      const int y0 = un.mt * TILE + (int)rank * 128 + quad * 32;   // first row of this warp
+      uint32_t low[SPLIT && EPI == EPI_GRAD ? 2 : 1][16];          // the second plane, until its store
+
+      auto store_f16_pair = [&](int x, int y, int plane) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&map_o, st_addr, x, y, plane);
+          bulk_commit();
+        }
+      };
+      // what happens to chunk i (columns col + 32 i .. + 31) of the finished sum
+      auto finish = [&](int i, float (&v)[32]) {
+        const int c0 = col + 32 * i;
+        if constexpr (EPI == EPI_STATS) {
+          const int left = g.vocab - (g.v0 + c0);                  // columns of the chunk inside the vocabulary
+          if (left < 32) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (k >= left) v[k] = -INFINITY;
+          }
+          float m = v[0];
+#pragma unroll
+          for (int k = 1; k < 32; ++k) m = fmaxf(m, v[k]);
+          m = fmaxf(run_m, m * c2);
+          const float ref = finite_max(m);
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            s0 += ex2(fmaf(v[k], c2, -ref));
+            s1 += ex2(fmaf(v[k + 1], c2, -ref));
+          }
+          run_s = run_s * ex2(run_m - ref) + (s0 + s1);
+          run_m = m;
+          const uint32_t y = target - 32u * (uint32_t)i;
+          if (y < 32u) {
+            float z = 0.f;
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (y == (uint32_t)k) z = v[k];
+            g.rw.picked[row] = z * c2;
+          }
+        } else if constexpr (EPI == EPI_GRAD) {
+          uint32_t hi[16];
+          const uint32_t y = target - 32u * (uint32_t)i;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            float p0 = ex2(fmaf(v[k], c2, -lse2)), p1 = ex2(fmaf(v[k + 1], c2, -lse2));
+            if (y == (uint32_t)k) p0 -= 1.f;
+            if (y == (uint32_t)(k + 1)) p1 -= 1.f;
+            p0 *= wg;
+            p1 *= wg;
+            // rows behind the last supervised one hold zeros: they are part of dW's K
+            if (row >= live) p0 = p1 = 0.f;
+            hi[k >> 1] = pack_h2(p0, p1);
+            if constexpr (SPLIT) {
+              const float2 f = __half22float2(*(const __half2*)&hi[k >> 1]);
+              low[i & 1][k >> 1] = pack_h2(p0 - f.x, p1 - f.y);
+            }
+          }
+          // two chunks make the 64 columns of a store
+          if ((i & 1) == 0) {
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();
+          }
+          stage_f16(st, lane, i & 1, hi);
+          if (i & 1) {
+            store_f16_pair(c0 - 32, y0, 0);
+            if constexpr (SPLIT) {
+              if (lane == 0) bulk_wait_read();
+              __syncwarp();
+              stage_f16(st, lane, 0, low[0]);
+              stage_f16(st, lane, 1, low[1]);
+              store_f16_pair(c0 - 32, y0, 1);
+            }
+          }
+        } else {
+          if (c0 >= g.N || y0 >= rows_end) return;                 // the whole block lies outside
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] *= alpha;
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+          if (g.direct == nullptr && g.out_type == FT_TYPE_F16) {
+            uint32_t h[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) h[k >> 1] = pack_h2(v[k], v[k + 1]);
+            // 32 columns are 64 bytes: a tile of its own swizzle (64-byte rows)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *(uint4*)(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+          } else {
+            stage_f32(st, lane, v);
+          }
+          if (g.direct == nullptr) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (g.accumulate) tma_add_3d(&map_o, st_addr, g.out_x0 + c0, g.out_y0 + y0, un.sp);
+              else tma_store_3d(&map_o, st_addr, g.out_x0 + c0, g.out_y0 + y0, un.sp);
+              bulk_commit();
+            }
+          } else {
+            // a pitch or a base that TMA cannot address: a row at a time, a column a lane
+            __syncwarp();
+            if (c0 + lane < g.N) {
+              for (int r = 0; r < 32 && y0 + r < rows_end; ++r) {
+                const float x = *(const float*)(st + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                const long long at = (long long)(g.out_y0 + y0 + r) * g.direct_ld + g.out_x0 + c0 + lane;
+                if (g.out_type == FT_TYPE_F16) ((__half*)g.direct)[at] = __float2half_rn(x);
+                else ((float*)g.direct)[at] = x;
+              }
+            }
+            __syncwarp();
+          }
+        }
+      };
+
+      if constexpr (SPLIT) {
+        float acc[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) acc[i][k] = 0.f;
+        for (int s0 = kb0; s0 < kb1; s0 += slice, ++local) {
+          const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+          if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t r[32];
+            tc_ld32(t_lane + buf * TILE + i * 32, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[i][k] += __uint_as_float(r[k]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(lead_tempty + buf * 8);
+        }
+        if (*abort_flag) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) finish(i, acc[i]);
+      } else {
+        const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+        ++local;
+        if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[32];
+          tc_ld32(t_lane + buf * TILE + i * 32, *(uint32_t(*)[32])v);
+          tc_wait_ld();
+          if (i == 3) {
+            // all four chunks are in registers: the accumulator may be overwritten
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(lead_tempty + buf * 8);
+          }
+          finish(i, v);
+        }
+      }
+      if constexpr (EPI == EPI_STATS) g.part[(size_t)(un.nt * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+    }
+    // what was stored is complete before the launch ends
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    __syncthreads();
+  }
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------ around the products
+// Joins the column tiles' {maximum, sum} of 32 rows, tiles over 16 warps in a fixed order, and writes
+// the row's log-sum-exp (in log2 units, as the gradient's epilogue wants it) and its loss.
+constexpr int LOSS_WARPS = 16;
+__global__ void __launch_bounds__(32 * LOSS_WARPS)
+k_ce_loss(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int vocab, float* __restrict__ row_loss) {
+  __shared__ float2 red[LOSS_WARPS][32];
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  const int live = rw.head->count;
+  if (blockIdx.x * 32 >= live) return;
+  float m = -INFINITY, s = 0.f;
+  for (int p = warp; p < parts; p += LOSS_WARPS) {
+    const float2 v = part[(size_t)p * part_ld + row];
+    const float mn = fmaxf(m, v.x), ref = finite_max(mn);
+    s = s * ex2(m - ref) + v.y * ex2(v.x - ref);
+    m = mn;
+  }
+  red[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (warp != 0 || row >= live) return;
+  float M = -INFINITY;
+  for (int w = 0; w < LOSS_WARPS; ++w) M = fmaxf(M, red[w][lane].x);
+  const float ref = finite_max(M);
+  float S = 0.f;
+  for (int w = 0; w < LOSS_WARPS; ++w) S += red[w][lane].y * ex2(red[w][lane].x - ref);
+  const float l2 = log2f(S);
+  rw.lse[row] = ref + l2;
+  // (ref - picked) first: a row that is sure of its target loses nothing to the size of its logits
+  row_loss[rw.source[row]] =
+      rw.target[row] < (uint32_t)vocab ? ((ref - rw.picked[row]) + l2) * 0.6931471805599453f : 0.f;
+}
+
+// Largest finite magnitude of W (first `w_blocks` blocks) and of the supervised rows (the others).
+__global__ void __launch_bounds__(256)
+k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* __restrict__ hidden,
+          const uint32_t* __restrict__ targets, int rows, int H, Head* __restrict__ head) {
+  ft_pdl_wait();
+  ft_pdl_launch();
+  float m = 0.f;
+  if ((int)blockIdx.x < w_blocks) {
+    const long long step = (long long)w_blocks * 256;
+    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (((uintptr_t)w & 15) == 0) {
+      for (; i < n / 4; i += step) {
+        const float4 v = ((const float4*)w)[i];
+        const float a = fmaxf(fabsf(v.x), fabsf(v.y)), b = fmaxf(fabsf(v.z), fabsf(v.w));
+        if (fmaxf(a, b) < INFINITY && a + b == a + b) m = fmaxf(m, fmaxf(a, b));
+        else {
+          const float e[4] = {v.x, v.y, v.z, v.w};
+          for (float x : e) if (fabsf(x) < INFINITY) m = fmaxf(m, fabsf(x));
+        }
+      }
+      i = n / 4 * 4 + (long long)blockIdx.x * 256 + threadIdx.x;
+    }
+    for (; i < n; i += step)
+      if (fabsf(w[i]) < INFINITY) m = fmaxf(m, fabsf(w[i]));
+  } else {
+    for (int r = blockIdx.x - w_blocks; r < rows; r += gridDim.x - w_blocks) {
+      if (targets[r] == FT_MASKED_CE_SKIP) continue;
+      for (int c = threadIdx.x; c < H; c += 256) {
+        const float x = fabsf(hidden[(size_t)r * H + c]);
+        if (x < INFINITY) m = fmaxf(m, x);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0 && m > 0.f)
+    atomicMax((int)blockIdx.x < w_blocks ? &head->w_amax : &head->h_amax, __float_as_int(m));
+}
+
+// W [rows, cols] -> f16 planes [planes][rows][ld], times the power of two of its largest value
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_ce_weight(const T* __restrict__ w, int rows, int cols, __half* __restrict__ out, int ld, int planes,
+            const Head* __restrict__ head) {
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const float S = sizeof(T) == 4 ? power_for(head->w_amax, OPERAND_EXP) : 1.f;
+  const size_t plane = (size_t)rows * ld;
+  const int units = ld / 8;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * units; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / units), c = (int)(i % units) * 8;
+    const T* p = w + (size_t)r * cols + c;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      const float a = c + k < cols ? (float)p[k] * S : 0.f, b = c + k + 1 < cols ? (float)p[k + 1] * S : 0.f;
+      hi[k >> 1] = pack_h2(a, b);
+      const float2 f = __half22float2(*(const __half2*)&hi[k >> 1]);
+      lo[k >> 1] = pack_h2(a - f.x, b - f.y);
+    }
+    *(uint4*)(out + (size_t)r * ld + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (planes == 2) *(uint4*)(out + plane + (size_t)r * ld + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+
+// grad_hidden[r] = unscale * (sum of the splits' slabs) at the row's packed place, zero where skipped
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_ce_scatter(const float* __restrict__ acc, size_t slab, int splits, int ld, Rows rw, int H, int rows, T* __restrict__ out) {
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const float alpha = rw.head->g_unscale * rw.head->w_unscale;
+  const int units = ld / 4;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * units; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / units), c = (int)(i % units) * 4;
+    const int at = rw.place[r];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at >= 0) {
+      const float* p = acc + (size_t)at * ld + c;
+      v = *(const float4*)p;
+      for (int s = 1; s < splits; ++s) {
+        const float4 x = *(const float4*)(p + s * slab);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      }
+    }
+    T* o = out + (size_t)r * H + c;
+    const float e[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < H) {
+        if constexpr (sizeof(T) == 2) o[k] = __float2half_rn(e[k]);
+        else o[k] = e[k];
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------ host side
+int make_map3(FtContext* ctx, CUtensorMap* map, const void* ptr, bool f32, uint64_t inner, uint64_t rows, uint64_t planes,
+              uint64_t ld, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+  auto encode = (PFN_cuTensorMapEncodeTiled_v12000)ctx->encode_tiled;
+  if (!encode) {
+    ft_set_error("linear_cross_entropy: cuTensorMapEncodeTiled is not available from this driver");
+    return FT_ERR_UNSUPPORTED;
+  }
+  const uint64_t size = f32 ? 4 : 2;
+  cuuint64_t dims[3] = {inner, rows, planes};
+  cuuint64_t strides[2] = {ld * size, rows * ld * size};
+  cuuint32_t box[3] = {box_inner, box_rows, 1}, step[3] = {1, 1, 1};
+  const CUresult r = encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                            const_cast<void*>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    ft_set_error("linear_cross_entropy: cuTensorMapEncodeTiled failed with %d (%llu x %llu, pitch %llu)", (int)r,
+                 (unsigned long long)inner, (unsigned long long)rows, (unsigned long long)ld);
+    return FT_ERR_UNSUPPORTED;
+  }
+  return FT_OK;
+}
+
+template <int EPI, bool A_MN, bool B_MN, bool SPLIT>
+int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g) {
+  auto kernel = k_ce_gemm<EPI, A_MN, B_MN, SPLIT>;
+  static bool ready[FT_MAX_DEVICES] = {};
+  static int most[FT_MAX_DEVICES] = {};
+  if (!ready[ctx->device]) {
+    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctx->sm_count & ~1));
+    cfg.blockDim = dim3(GEMM_THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    FT_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    most[ctx->device] = std::max(1, std::min(n, ctx->sm_count / 2));
+    ready[ctx->device] = true;
+  }
+  const long long units = (long long)ft_cdiv(g.M, TILE) * ft_cdiv(g.N, TILE) * g.splits;
+  const int pairs = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
+  FT_LAUNCH_PDL(ctx, (k_ce_gemm<EPI, A_MN, B_MN, SPLIT>), 2 * pairs, GEMM_THREADS, SMEM_BYTES, a, b, o, g, ctx->status_dev);
+  return FT_OK;
+}
+
+template <int EPI, bool A_MN, bool B_MN>
+int launch_gemm(FtContext* ctx, bool split, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g) {
+  return split ? launch_gemm<EPI, A_MN, B_MN, true>(ctx, a, b, o, g) : launch_gemm<EPI, A_MN, B_MN, false>(ctx, a, b, o, g);
+}
+
+// plane pairs of a product, the smallest first: sums grow as late as they can
+void set_terms(TcProduct& g, int pa, int pb) {
+  g.terms = 0;
+  auto add = [&](int a, int b) { g.a_plane[g.terms] = a; g.b_plane[g.terms] = b; ++g.terms; };
+  if (pa == 2) add(1, 0);
+  if (pb == 2) add(0, 1);
+  add(0, 0);
+}
+
+constexpr size_t G_PIECE_BYTES = (size_t)256 << 20;
+
+struct TcPlan {
+  Rows rows;
+  __half *h, *w, *grad;
+  float2* part;
+  float* acc;
+  int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld, parts;
+  bool w_staged;
+  size_t bytes;
+};
+
+TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void* base) {
+  TcPlan pl = {};
+  Carver c(base);
+  const bool two = ctx->gemm_mode == FT_GEMM_F16X2;
+  pl.rows = carve_rows(c, q.T);
+  pl.Tp = (int)ft_align_up((size_t)std::max(q.T, 1), TILE);
+  pl.h_ld = (int)ft_align_up((size_t)q.H, 8);
+  pl.h_planes = two && q.p.hidden_type == FT_TYPE_F32 ? 2 : 1;
+  pl.w_planes = two && q.p.weight_type == FT_TYPE_F32 ? 2 : 1;
+  pl.g_planes = two ? 2 : 1;
+  pl.w_rows = q.p.weight_vocab_major ? q.V : q.H;
+  pl.w_cols = q.p.weight_vocab_major ? q.H : q.V;
+  pl.w_staged = q.p.weight_type == FT_TYPE_F32 || pl.w_cols % 8 != 0 || ((uintptr_t)weight & 15) != 0;
+  pl.w_ld = (int)ft_align_up((size_t)pl.w_cols, 8);
+  pl.h = c.take<__half>((size_t)pl.h_planes * pl.Tp * pl.h_ld);
+  pl.w = pl.w_staged ? c.take<__half>((size_t)pl.w_planes * pl.w_rows * pl.w_ld) : nullptr;
+  pl.parts = 2 * ft_cdiv(q.V, TILE);
+  const size_t part_bytes = (size_t)pl.parts * pl.Tp * sizeof(float2);
+  size_t grad_bytes = 0;
+  if (q.grad_hidden || q.grad_weight) {
+    const size_t column = (size_t)pl.Tp * 2 * pl.g_planes;
+    size_t cols = q.p.vocab_piece ? q.p.vocab_piece : std::max<size_t>(TILE, G_PIECE_BYTES / column);
+    const int pieces = ft_cdiv(q.V, (long long)std::min<size_t>(cols, (size_t)q.V));
+    // equal pieces of whole tiles
+    pl.piece = (int)ft_align_up((size_t)ft_cdiv(q.V, pieces), TILE);
+    grad_bytes = column * pl.piece;
+  }
+  // the statistics of the column tiles are done with before the first piece of g is written
+  char* shared = c.take<char>(std::max(part_bytes, grad_bytes));
+  pl.part = (float2*)shared;
+  pl.grad = (__half*)shared;
+  pl.splits = 1;
+  if (q.grad_hidden) {
+    // K parts: as many as fill the pairs in whole waves, each at least 1024 deep and 64 MB of slabs
+    pl.acc_ld = (int)ft_align_up((size_t)q.H, 4);
+    const int pairs = std::max(1, ctx->sm_count / 2);
+    const long long tiles = (long long)(pl.Tp / TILE) * ft_cdiv(q.H, TILE);
+    double best = 1e30;
+    for (int s = 1; s <= 64 && s * 1024 <= std::max(1024, pl.piece); ++s) {
+      if (s > 1 && (size_t)s * pl.Tp * pl.acc_ld * 4 > ((size_t)256 << 20)) break;
+      const double waves = (double)((tiles * s + pairs - 1) / pairs) / s;
+      if (waves < best * 0.97) { best = waves; pl.splits = s; }
+    }
+    pl.acc = c.take<float>((size_t)pl.splits * pl.Tp * pl.acc_ld);
+  }
+  pl.bytes = c.bytes();
+  return pl;
+}
+
+}  // namespace
+
+namespace ft_ce {
+
+size_t tc_workspace(const FtContext* ctx, const Problem& q, const void* weight) { return tc_plan(ctx, q, weight, nullptr).bytes; }
+
+int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
+  const TcPlan pl = tc_plan(ctx, q, t.weight, ws);
+  const int T = q.T, H = q.H, V = q.V;
+  const bool vm = q.p.weight_vocab_major != 0, two = pl.g_planes == 2;
+  const bool h32 = q.p.hidden_type == FT_TYPE_F32, w32 = q.p.weight_type == FT_TYPE_F32;
+  if (h32 || w32) {
+    FT_CUDA(cudaMemsetAsync(pl.rows.head, 0, sizeof(Head), ctx->stream));
+    const int wb = w32 ? ctx->sm_count * 4 : 0, hb = h32 ? std::min(T, ctx->sm_count * 4) : 0;
+    FT_LAUNCH_PDL(ctx, k_ce_amax, wb + hb, 256, 0, (const float*)t.weight, (long long)pl.w_rows * pl.w_cols, wb,
+                  (const float*)t.hidden, t.targets, T, H, pl.rows.head);
+  }
+  FT_TRY(launch_gather_f16(ctx, q, t, pl.rows, pl.h, pl.h_ld, pl.Tp, pl.h_planes));
+  const void* w = t.weight;
+  if (pl.w_staged) {
+    w = pl.w;
+    const int grid = (int)std::min<long long>(ft_cdiv((long long)pl.w_rows * (pl.w_ld / 8), 256), (long long)ctx->sm_count * 16);
+    if (w32)
+      FT_LAUNCH_PDL(ctx, k_ce_weight<float>, grid, 256, 0, (const float*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
+                    pl.w_planes, pl.rows.head);
+    else
+      FT_LAUNCH_PDL(ctx, k_ce_weight<__half>, grid, 256, 0, (const __half*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
+                    pl.w_planes, pl.rows.head);
+  }
+  // K-contiguous operands come in boxes of 64 x 128 rows, M/N-contiguous ones in two of 64 x 64
+  CUtensorMap h_k, w_k, w_mn;
+  FT_TRY(make_map3(ctx, &h_k, pl.h, false, H, pl.Tp, pl.h_planes, pl.h_ld, 64, 128));
+  FT_TRY(make_map3(ctx, &w_k, w, false, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, 64, 128));
+  FT_TRY(make_map3(ctx, &w_mn, w, false, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, 64, 64));
+
+  TcProduct z = {};
+  z.M = T; z.K = H; z.live_m = 1; z.splits = 1;
+  z.band = 32;
+  set_terms(z, pl.h_planes, pl.w_planes);
+  z.rw = pl.rows; z.part = pl.part; z.part_ld = pl.Tp; z.vocab = V; z.g_planes = pl.g_planes;
+  z.N = V;
+  if (vm) FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z)));
+  else FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z)));
+  FT_LAUNCH_PDL(ctx, k_ce_loss, ft_cdiv(T, 32), 32 * LOSS_WARPS, 0, pl.part, pl.Tp, pl.parts, pl.rows, V, t.row_loss);
+  if (!t.grad_hidden && !t.grad_weight) return FT_OK;
+
+  CUtensorMap g_out, g_k, g_mn, acc_out, h_mn, dw_out;
+  FT_TRY(make_map3(ctx, &g_out, pl.grad, false, pl.piece, pl.Tp, pl.g_planes, pl.piece, 64, 32));
+  if (t.grad_hidden) FT_TRY(make_map3(ctx, &acc_out, pl.acc, true, pl.acc_ld, pl.Tp, pl.splits, pl.acc_ld, 32, 32));
+  FT_TRY(make_map3(ctx, &h_mn, pl.h, false, H, pl.Tp, pl.h_planes, pl.h_ld, 64, 64));
+  const bool dw16 = q.p.grad_weight_type == FT_TYPE_F16;
+  const bool dw_tma = t.grad_weight && ((uintptr_t)t.grad_weight & 15) == 0 && pl.w_cols % (dw16 ? 8 : 4) == 0;
+  if (dw_tma)
+    FT_TRY(make_map3(ctx, &dw_out, t.grad_weight, !dw16, pl.w_cols, pl.w_rows, 1, pl.w_cols, 32, 32,
+                     dw16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B));
+  for (int v0 = 0; v0 < V; v0 += pl.piece) {
+    const int cols = std::min(pl.piece, V - v0);
+    z.N = cols; z.v0 = v0; z.b_mn0 = v0;
+    if (vm) FT_TRY((launch_gemm<EPI_GRAD, false, false>(ctx, two, h_k, w_k, g_out, z)));
+    else FT_TRY((launch_gemm<EPI_GRAD, false, true>(ctx, two, h_k, w_mn, g_out, z)));
+    // as operands, the piece ends with the vocabulary: what lies behind reads as zero
+    if (v0 == 0 || cols != pl.piece) {
+      FT_TRY(make_map3(ctx, &g_k, pl.grad, false, cols, pl.Tp, pl.g_planes, pl.piece, 64, 128));
+      FT_TRY(make_map3(ctx, &g_mn, pl.grad, false, cols, pl.Tp, pl.g_planes, pl.piece, 64, 64));
+    }
+    if (t.grad_hidden) {
+      TcProduct p = {};
+      p.rw = pl.rows;
+      p.M = T; p.N = H; p.K = cols; p.live_m = 1;
+      p.splits = std::min(pl.splits, ft_cdiv(cols, BK));
+      p.n_fast = 1; p.band = 1;
+      set_terms(p, pl.g_planes, pl.w_planes);
+      p.k0 = v0; p.b_has_k0 = 1;
+      p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
+      if (vm) FT_TRY((launch_gemm<EPI_STORE, false, true>(ctx, two, g_k, w_mn, acc_out, p)));
+      else FT_TRY((launch_gemm<EPI_STORE, false, false>(ctx, two, g_k, w_k, acc_out, p)));
+    }
+    if (t.grad_weight) {
+      TcProduct p = {};
+      p.rw = pl.rows;
+      p.K = T; p.live_k = 1; p.splits = 1;
+      p.unscale = 1;
+      p.out_type = (int)q.p.grad_weight_type;
+      if (!dw_tma) { p.direct = t.grad_weight; p.direct_ld = pl.w_cols; }
+      if (vm) {
+        p.M = cols; p.N = H; p.out_y0 = v0;
+        set_terms(p, pl.g_planes, pl.h_planes);
+      } else {
+        p.M = H; p.N = cols; p.out_x0 = v0;
+        set_terms(p, pl.h_planes, pl.g_planes);
+      }
+      p.n_fast = p.M >= p.N; p.band = ft_cdiv(p.M, TILE);
+      FT_TRY((launch_gemm<EPI_STORE, true, true>(ctx, two, vm ? g_mn : h_mn, vm ? h_mn : g_mn, dw_tma ? dw_out : g_mn, p)));
+    }
+  }
+  if (t.grad_hidden) {
+    const size_t slab = (size_t)pl.Tp * pl.acc_ld;
+    const int grid = (int)std::min<long long>(ft_cdiv((long long)T * (pl.acc_ld / 4), 256), (long long)ctx->sm_count * 16);
+    if (q.p.grad_hidden_type == FT_TYPE_F16)
+      FT_LAUNCH_PDL(ctx, k_ce_scatter<__half>, grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, H, T, (__half*)t.grad_hidden);
+    else
+      FT_LAUNCH_PDL(ctx, k_ce_scatter<float>, grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, H, T, (float*)t.grad_hidden);
+  }
+  return FT_OK;
+}
+
+}  // namespace ft_ce

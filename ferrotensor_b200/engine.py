@@ -492,7 +492,7 @@ class ComputeEngine:
         """Bytes of workspace that a call with these tensors needs in the context's GEMM mode."""
         p = self._linear_ce_params(hidden, weight, grad_hidden, grad_weight, 1.0, vocab_piece, int(vocab_major))
         n = C.c_size_t()
-        call("ft_linear_cross_entropy_workspace", ctx.handle, C.byref(p), grad_hidden is not None,
+        call("ft_linear_cross_entropy_workspace", ctx.handle, weight.ptr, C.byref(p), grad_hidden is not None,
              grad_weight is not None, C.byref(n))
         return n.value
 
@@ -522,7 +522,7 @@ class ComputeEngine:
                  "linear_cross_entropy: one F32 weight per row")
         if workspace is None:
             n = C.c_size_t()
-            call("ft_linear_cross_entropy_workspace", ctx.handle, C.byref(p), grad_hidden is not None,
+            call("ft_linear_cross_entropy_workspace", ctx.handle, weight.ptr, C.byref(p), grad_hidden is not None,
                  grad_weight is not None, C.byref(n))
             workspace = ctx.temporary(n.value)
         else:

@@ -226,7 +226,8 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  * halves.  (f16 operands are exact in every mode; sums are f32 in every mode.)
  * The vocabulary is worked through in pieces of vocab_piece columns (0: chosen by size), of which
  * only one piece of g exists at a time; workspace holds it and must have the bytes that
- * ft_linear_cross_entropy_workspace gives for the same arguments, context and GEMM mode.  The
+ * ft_linear_cross_entropy_workspace gives for the same arguments, context and GEMM mode (of the
+ * weight it looks at the alignment alone).  The
  * call allocates nothing, keeps nothing there for a later call, and may be captured into a
  * graph; calls that overlap on the GPU need workspaces of their own.  Outputs may overlap no
  * input, no other output and not the workspace.
@@ -239,8 +240,9 @@ typedef struct FtLinearCeParams {
   uint32_t vocab_piece;
   float grad_scale;
 } FtLinearCeParams;
-int ft_linear_cross_entropy_workspace(FtContext* ctx, const FtLinearCeParams* p,
-                                      int want_grad_hidden, int want_grad_weight, size_t* bytes);
+int ft_linear_cross_entropy_workspace(FtContext* ctx, const void* weight,
+                                      const FtLinearCeParams* p, int want_grad_hidden,
+                                      int want_grad_weight, size_t* bytes);
 int ft_linear_cross_entropy(FtContext* ctx, const void* hidden, const void* weight,
                             const uint32_t* targets, const float* weights, float* row_loss,
                             void* grad_hidden, void* grad_weight, void* workspace,

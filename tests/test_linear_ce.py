@@ -77,14 +77,18 @@ def test_refusals(lib, params, call, message):
 def test_workspace_grows_with_what_is_asked(lib):
     fake = C.create_string_buffer(1 << 16)
     h = C.cast(fake, C.c_void_p)
-    got = []
-    for gh, gw in ((0, 0), (1, 0), (1, 1)):
-        n = C.c_size_t()
-        assert lib.ft_linear_cross_entropy_workspace(h, C.byref(_params(rows=4096)), gh, gw, C.byref(n)) == 0
-        got.append(n.value)
-    assert 0 < got[0] <= got[1] <= got[2]
-    assert lib.ft_linear_cross_entropy_workspace(h, C.byref(_params(hidden=0)), 0, 0, C.byref(n)) == 1
-    assert lib.ft_linear_cross_entropy_workspace(h, C.byref(_params()), 0, 0, None) == 1
+    n = C.c_size_t()
+    for mode in range(3):
+        assert lib.ft_ctx_set_gemm_mode(h, mode) == 0
+        for rows, hidden, vocab, piece in ((0, 1, 1, 0), (1, 1, 1, 0), (4096, 64, 1000, 0), (4096, 65, 100003, 1), (1 << 24, 1 << 16, 1 << 24, 7)):
+            got = []
+            for gh, gw in ((0, 0), (1, 0), (1, 1)):
+                p = _params(rows=rows, hidden=hidden, vocab=vocab, vocab_piece=piece)
+                assert lib.ft_linear_cross_entropy_workspace(h, None, C.byref(p), gh, gw, C.byref(n)) == 0
+                got.append(n.value)
+            assert 0 < got[0] <= got[1] <= got[2] < 1 << 60
+    assert lib.ft_linear_cross_entropy_workspace(h, None, C.byref(_params(hidden=0)), 0, 0, C.byref(n)) == 1
+    assert lib.ft_linear_cross_entropy_workspace(h, None, C.byref(_params()), 0, 0, None) == 1
 
 
 def test_struct_layout_matches_header(tmp_path):
