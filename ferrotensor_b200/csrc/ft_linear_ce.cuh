@@ -42,6 +42,7 @@ struct Rows {
   float* weight;      // grad_scale * weights[row]
   float2* stat;       // running {maximum, sum of exponentials against it}
   float* picked;      // logit of the target
+  float* exact;       // the same from f32 products, beside the tensor cores' sum
   float* lse;
 };
 
@@ -85,6 +86,7 @@ inline Rows carve_rows(Carver& c, int T) {
   r.weight = c.take<float>(T);
   r.stat = c.take<float2>(T);
   r.picked = c.take<float>(T);
+  r.exact = c.take<float>(T);
   r.lse = c.take<float>(T);
   return r;
 }

@@ -37,6 +37,8 @@ constexpr int SMEM_BYTES = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
 constexpr int SLICE_KB = 8;
 
 enum Epi { EPI_STATS, EPI_GRAD, EPI_STORE };
+// The statistics' launch has two warps more, for the targets' logits.
+constexpr int threads_of(int epi) { return epi == EPI_STATS ? GEMM_THREADS + 64 : GEMM_THREADS; }
 
 struct TcProduct {
   int M, N, K;
@@ -53,6 +55,11 @@ struct TcProduct {
   int part_ld;
   int v0, vocab;                    // first vocabulary column of the launch, columns in all
   int g_planes;
+  // EPI_STATS: the operands again, for the targets' logits
+  const __half *h, *w;              // value (k, plane) of a row at h + row * h_ld + plane * h_plane + k,
+  long long h_ld, h_plane;          // W(k, v) at w + k * w_sk + v * w_sv + plane * w_plane
+  long long w_sk, w_sv, w_plane;
+  int h_planes, w_planes;
   // EPI_STORE
   int out_type;                     // FT_TYPE_*
   int accumulate;
@@ -124,8 +131,29 @@ __device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const
     *(uint4*)(st + lane * 128 + (((part * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
 }
 
+// h_row . W(:, target) on f32 FMA, one row a warp.  The tensor core's sums are cut off, not rounded (see
+// above): 4e-6 of a logit at K = 256, 4e-5 at 2048.  For most logits that is noise under the softmax,
+// but the loss of a row that is sure of its target is as exact, relative to itself, as that one
+// logit is exact in absolute terms.  [hidden, vocab] weights cost a 32-byte sector for every 2
+// bytes here; beside the products nobody waits for them.
+__device__ __forceinline__ float target_dot(const TcProduct& g, int row, uint32_t target, int lane) {
+  const __half* h = g.h + (long long)row * g.h_ld;
+  const __half* w = g.w + (long long)target * g.w_sv;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int k = lane; k < g.K; k += 32) {
+    float a = __half2float(h[k]), b = __half2float(w[k * g.w_sk]);
+    if (g.h_planes == 2) a += __half2float(h[g.h_plane + k]);
+    if (g.w_planes == 2) b += __half2float(w[g.w_plane + k * g.w_sk]);
+    acc = fmaf(a, b, acc);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  return acc;
+}
+
 template <int EPI, bool A_MN, bool B_MN, bool SPLIT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
   extern __shared__ uint8_t smem_raw[];
@@ -249,6 +277,15 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
     }
     __syncwarp();
+  } else if (EPI == EPI_STATS && warp >= GEMM_THREADS / 32) {
+    // ------------------------------------------------------------------ the targets' logits
+    const float c2 = g.rw.head->z_scale * 1.4426950408889634f;
+    for (int r = (int)blockIdx.x * 2 + warp - GEMM_THREADS / 32; r < live; r += (int)gridDim.x * 2) {
+      const uint32_t y = g.rw.target[r];
+      if (y >= (uint32_t)g.vocab) continue;
+      const float z = target_dot(g, r, y, lane);
+      if (lane == 0) g.rw.exact[r] = z * c2;
+    }
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
     // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the two warps of a quadrant take 128
@@ -493,9 +530,16 @@ k_ce_loss(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
   for (int w = 0; w < LOSS_WARPS; ++w) S += red[w][lane].y * ex2(red[w][lane].x - ref);
   const float l2 = log2f(S);
   rw.lse[row] = ref + l2;
-  // (ref - picked) first: a row that is sure of its target loses nothing to the size of its logits
-  row_loss[rw.source[row]] =
-      rw.target[row] < (uint32_t)vocab ? ((ref - rw.picked[row]) + l2) * 0.6931471805599453f : 0.f;
+  float loss = 0.f;
+  if (rw.target[row] < (uint32_t)vocab) {
+    // the sum with the target's logit z replaced by its exact value z + d:
+    //   loss = log(e^(lse - z) + e^d - 1) - d = (lse - z) - d + log(1 + p (e^d - 1)),  p = e^(z - lse)
+    // (ref - z) first: a row that is sure of its target loses nothing to the size of its logits
+    const float z = rw.picked[row], above = ((ref - z) + l2) * 0.6931471805599453f;
+    const float d = (rw.exact[row] - z) * 0.6931471805599453f;
+    loss = above - d + log1pf(expf(-above) * expm1f(d));
+  }
+  row_loss[rw.source[row]] = loss;
 }
 
 // Largest finite magnitude of W (first `w_blocks` blocks) and of the supervised rows (the others).
@@ -626,7 +670,7 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
     FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctx->sm_count & ~1));
-    cfg.blockDim = dim3(GEMM_THREADS);
+    cfg.blockDim = dim3(threads_of(EPI));
     cfg.dynamicSmemBytes = SMEM_BYTES;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -640,7 +684,13 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   }
   const long long units = (long long)ft_cdiv(g.M, TILE) * ft_cdiv(g.N, TILE) * g.splits;
   const int pairs = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
-  FT_LAUNCH_PDL(ctx, (k_ce_gemm<EPI, A_MN, B_MN, SPLIT>), 2 * pairs, GEMM_THREADS, SMEM_BYTES, a, b, o, g, ctx->status_dev);
+  const char* const names[3] = {"k_ce_gemm<statistics>", "k_ce_gemm<g>", A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>"};
+  if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
+  cudaError_t e = ft_launch_ex(ctx, kernel, 2 * pairs, threads_of(EPI), SMEM_BYTES, a, b, o, g, ctx->status_dev);
+  if (ctx->profile_all) ft_prof_end(ctx);
+  ctx->launches++;
+  if (e == cudaSuccess) e = cudaPeekAtLastError();
+  if (e != cudaSuccess) return ft_cuda_fail(e, "k_ce_gemm", __FILE__, __LINE__);
   return FT_OK;
 }
 
@@ -760,6 +810,9 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   set_terms(z, pl.h_planes, pl.w_planes);
   z.rw = pl.rows; z.part = pl.part; z.part_ld = pl.Tp; z.vocab = V; z.g_planes = pl.g_planes;
   z.N = V;
+  z.h = pl.h; z.h_ld = pl.h_ld; z.h_plane = (long long)pl.Tp * pl.h_ld; z.h_planes = pl.h_planes;
+  z.w = (const __half*)w; z.w_plane = (long long)pl.w_rows * pl.w_ld; z.w_planes = pl.w_planes;
+  z.w_sk = vm ? 1 : pl.w_ld; z.w_sv = vm ? pl.w_ld : 1;
   if (vm) FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z)));
   else FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z)));
   FT_LAUNCH_PDL(ctx, k_ce_loss, ft_cdiv(T, 32), 32 * LOSS_WARPS, 0, pl.part, pl.Tp, pl.parts, pl.rows, V, t.row_loss);
