@@ -8,12 +8,14 @@
 // the sums and writes the scaled values.  Both walk a table of chunks (at most CHUNK elements of
 // one tensor each) that lies on the device since the list was made.  HBM-bound: a value is read
 // once for the norm and once for the scaling, which walks the chunks in the reverse order so that
-// its first reads find in L2 what the norm read last.
+// its first reads find in L2 what the norm read last.  A list of a few thousand values is bound by
+// its launches: k_list_small does both in one.
 #include <math.h>
 #include <string.h>
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "ft_common.cuh"
@@ -22,7 +24,12 @@ namespace {
 
 constexpr int LIST_THREADS = 256;
 constexpr int CHUNK = 8192;            // elements; a thread's share of one is eight 16-byte loads of f32
-constexpr int LIST_BLOCKS_PER_SM = 8;
+constexpr int LIST_BLOCKS_PER_SM = 4;  // of k_list_squares: 128 KB of loads in flight a multiprocessor
+constexpr int SCALE_BLOCKS_PER_SM = 4;
+
+// A list that makes at most SMALL_CHUNKS chunks of SMALL_CHUNK values: one block, a warp a chunk,
+// two chunks a warp at most, whose values stay in registers between the two steps.
+constexpr int SMALL_CHUNK = 256, SMALL_CHUNKS = 64, SMALL_THREADS = 1024;
 
 struct Chunk {
   void* p;
@@ -30,21 +37,91 @@ struct Chunk {
   uint32_t type;
 };
 
+// Eight values at a 16-byte boundary.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
+  const uint4 a = *(const uint4*)p;
+  const __half2* h = (const __half2*)&a;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+// Four values at a boundary of four.
+__device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
+__device__ __forceinline__ float4 load4(const __half* p) {
+  const uint2 a = *(const uint2*)p;
+  const float2 x = __half22float2(*(const __half2*)&a.x), y = __half22float2(*(const __half2*)&a.y);
+  return make_float4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *(float4*)p = v; }
+__device__ __forceinline__ void store4(__half* p, float4 v) {
+  const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+  *(uint2*)p = make_uint2(*(const uint32_t*)&x, *(const uint32_t*)&y);
+}
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
+
+// Elements before the first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ uint32_t ahead_of_boundary(const T* p, uint32_t n) {
+  return min(n, (uint32_t)((16 - ((uintptr_t)p & 15)) & 15) / (uint32_t)sizeof(T));
+}
+
 // Squares are taken and summed in f64: an f32 square leaves the f32 range for |g| above 1.8e19 or
-// below 1e-19.
-__device__ __forceinline__ double sum_squares_chunk(const Chunk& c) {
+// below 1e-19.  Squares of f16 values are exact in f32 and far from its ends, so eight of them are
+// added there first (conversions to f64 would bound the f16 rate otherwise).
+__device__ __forceinline__ double squares8(const float (&v)[8], float) {
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fma((double)v[i], (double)v[i], s);
+  return s;
+}
+__device__ __forceinline__ double squares8(const float (&v)[8], __half) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fmaf(v[i], v[i], s);
+  return (double)s;
+}
+
+template <typename T>
+__device__ __forceinline__ double sum_squares(const T* __restrict__ x, uint32_t n) {
   double acc = 0.0;
-  if (c.type == FT_TYPE_F32) {
-    const float* x = (const float*)c.p;
-    for (uint32_t i = threadIdx.x; i < c.n; i += LIST_THREADS) acc = fma((double)x[i], (double)x[i], acc);
-  } else {
-    const __half* x = (const __half*)c.p;
-    for (uint32_t i = threadIdx.x; i < c.n; i += LIST_THREADS) {
-      const double v = (double)__half2float(x[i]);
-      acc = fma(v, v, acc);
+  const uint32_t head = ahead_of_boundary(x, n);
+  if (threadIdx.x < head) {
+    const double v = (double)(float)x[threadIdx.x];
+    acc = v * v;
+  }
+  const T* body = x + head;
+  const uint32_t groups = (n - head) / 8;
+  // all loads of a thread's share first
+  float v[CHUNK / 8 / LIST_THREADS][8];
+#pragma unroll
+  for (int k = 0; k < CHUNK / 8 / LIST_THREADS; ++k) {
+    const uint32_t g = threadIdx.x + k * LIST_THREADS;
+    if (g < groups) load8(body + 8 * g, v[k]);
+    else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
     }
   }
+#pragma unroll
+  for (int k = 0; k < CHUNK / 8 / LIST_THREADS; ++k) acc += squares8(v[k], T());
+  const uint32_t tail = head + 8 * groups + threadIdx.x;
+  if (tail < n) {
+    const double t = (double)(float)x[tail];
+    acc = fma(t, t, acc);
+  }
   return acc;
+}
+
+__device__ __forceinline__ double sum_squares_chunk(const Chunk& c) {
+  return c.type == FT_TYPE_F32 ? sum_squares((const float*)c.p, c.n) : sum_squares((const __half*)c.p, c.n);
 }
 
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {
@@ -59,24 +136,93 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
   return s;
 }
 
-__global__ void __launch_bounds__(LIST_THREADS)
+__global__ void __launch_bounds__(LIST_THREADS, LIST_BLOCKS_PER_SM)
 k_list_squares(const Chunk* __restrict__ chunks, int count, double* __restrict__ partials) {
   __shared__ double red[LIST_THREADS / 32];
   ft_pdl_wait();
   ft_pdl_launch();
   double acc = 0.0;
-  for (int c = blockIdx.x; c < count; c += gridDim.x) acc += sum_squares_chunk(chunks[c]);
+  Chunk now = {};
+  if ((int)blockIdx.x < count) now = chunks[blockIdx.x];
+  for (int c = blockIdx.x; c < count; c += gridDim.x) {
+    // the next chunk's place is on its way while this one's values are
+    Chunk next = {};
+    if (c + (int)gridDim.x < count) next = chunks[c + gridDim.x];
+    acc += sum_squares_chunk(now);
+    now = next;
+  }
   acc = block_sum_f64(acc, red);
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
-__device__ __forceinline__ float load_one(const Chunk& c, uint32_t i) {
-  return c.type == FT_TYPE_F32 ? ((const float*)c.p)[i] : __half2float(((const __half*)c.p)[i]);
+// out = f x over one chunk: four values a lane, so that a warp's loads and stores are whole lines in
+// either type, where both sides reach a boundary of four values at the same element, else one.
+template <typename TI, typename TO>
+__device__ __forceinline__ void scale_chunk(const TI* x, TO* out, uint32_t n, float f) {
+  constexpr int BATCH = 4;
+  const uint32_t head = min(n, (uint32_t)((4 * sizeof(TI) - ((uintptr_t)x & (4 * sizeof(TI) - 1))) & (4 * sizeof(TI) - 1)) / (uint32_t)sizeof(TI));
+  if (((uintptr_t)(out + head) & (4 * sizeof(TO) - 1)) == 0) {
+    if (threadIdx.x < head) store1(out + threadIdx.x, f * (float)x[threadIdx.x]);
+    const uint32_t groups = (n - head) / 4;
+#pragma unroll 1
+    for (uint32_t g = threadIdx.x; g < groups; g += BATCH * LIST_THREADS) {
+      // (one base and constant offsets: indices of their own cost two registers each)
+      const TI* xb = x + head + 4 * (size_t)g;
+      TO* ob = out + head + 4 * (size_t)g;
+      const int left = (int)((groups - g + LIST_THREADS - 1) / LIST_THREADS);
+      float4 v[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (k < left) v[k] = load4(xb + 4 * k * LIST_THREADS);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (k < left) store4(ob + 4 * k * LIST_THREADS, make_float4(f * v[k].x, f * v[k].y, f * v[k].z, f * v[k].w));
+    }
+    const uint32_t tail = head + 4 * groups + threadIdx.x;
+    if (tail < n) store1(out + tail, f * (float)x[tail]);
+  } else {
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < n; i += BATCH * LIST_THREADS) {
+      const TI* xb = x + i;
+      TO* ob = out + i;
+      const int left = (int)((n - i + LIST_THREADS - 1) / LIST_THREADS);
+      float v[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (k < left) v[k] = (float)xb[k * LIST_THREADS];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (k < left) store1(ob + k * LIST_THREADS, f * v[k]);
+    }
+  }
+}
+
+// What follows from the sum of squares.
+struct Verdict {
+  float norm, factor;
+  bool finite;
+  __device__ __forceinline__ void publish(float* o) const {
+    o[0] = norm;
+    o[1] = finite ? 1.f : 0.f;
+    o[2] = factor;
+  }
+};
+__device__ __forceinline__ Verdict judge(double squares, float grad_scale, float max_norm) {
+  const double norm = sqrt(squares) * fabs((double)grad_scale);
+  Verdict d;
+  d.norm = (float)norm;
+  d.finite = isfinite(d.norm);
+  d.factor = grad_scale;
+  if (d.finite && max_norm > 0.f && norm > (double)max_norm)
+    d.factor = (float)((double)grad_scale * (double)max_norm / (norm + 1e-6));
+  return d;
 }
 
 // Every block joins the partial sums itself (the same order everywhere), block 0 publishes.
-// out == NULL: measure only.
-__global__ void __launch_bounds__(LIST_THREADS)
+// out == NULL: measure only.  TI, TO: the types of all chunks; void: each chunk's own.  (The four pairs
+// of types in one body spill 300 to 700 bytes a thread, so only lists of both types take it.)
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(LIST_THREADS, SCALE_BLOCKS_PER_SM)
 k_list_scale(const Chunk* __restrict__ chunks, const Chunk* __restrict__ out, int count,
              const double* __restrict__ partials, int parts, float grad_scale, float max_norm,
              float* __restrict__ norm_out, int in_place) {
@@ -85,27 +231,82 @@ k_list_scale(const Chunk* __restrict__ chunks, const Chunk* __restrict__ out, in
   ft_pdl_launch();
   double acc = 0.0;
   for (int i = threadIdx.x; i < parts; i += LIST_THREADS) acc += partials[i];
-  const double norm = sqrt(block_sum_f64(acc, red)) * fabs((double)grad_scale);
-  const bool finite = isfinite((float)norm);
-  float factor = grad_scale;
-  if (finite && max_norm > 0.f && norm > (double)max_norm)
-    factor = (float)((double)grad_scale * (double)max_norm / (norm + 1e-6));
-  if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) {
-    norm_out[0] = (float)norm;
-    norm_out[1] = finite ? 1.f : 0.f;
-    norm_out[2] = factor;
-  }
-  if (!out || !finite || (in_place && factor == 1.0f)) return;
-  for (int k = blockIdx.x; k < count; k += gridDim.x) {
-    const int c = count - 1 - k;
-    const Chunk src = chunks[c], dst = out[c];
-    if (dst.type == FT_TYPE_F32) {
-      for (uint32_t i = threadIdx.x; i < src.n; i += LIST_THREADS) ((float*)dst.p)[i] = factor * load_one(src, i);
+  const Verdict d = judge(block_sum_f64(acc, red), grad_scale, max_norm);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) d.publish(norm_out);
+  if (!out || !d.finite || (in_place && d.factor == 1.0f)) return;
+  const float factor = d.factor;
+  Chunk src = {}, dst = {};
+  int c = count - 1 - (int)blockIdx.x;
+  if (c >= 0) { src = chunks[c]; dst = out[c]; }
+  while (c >= 0) {
+    // the next chunk's place is on its way while this one's values are
+    c -= (int)gridDim.x;
+    Chunk next_src = {}, next_dst = {};
+    if (c >= 0) { next_src = chunks[c]; next_dst = out[c]; }
+    if constexpr (!std::is_void<TI>::value) {
+      scale_chunk((const TI*)src.p, (TO*)dst.p, src.n, factor);
+    } else if (src.type == FT_TYPE_F32) {
+      if (dst.type == FT_TYPE_F32) scale_chunk((const float*)src.p, (float*)dst.p, src.n, factor);
+      else scale_chunk((const float*)src.p, (__half*)dst.p, src.n, factor);
     } else {
-      for (uint32_t i = threadIdx.x; i < src.n; i += LIST_THREADS)
-        ((__half*)dst.p)[i] = __float2half_rn(factor * load_one(src, i));
+      if (dst.type == FT_TYPE_F32) scale_chunk((const __half*)src.p, (float*)dst.p, src.n, factor);
+      else scale_chunk((const __half*)src.p, (__half*)dst.p, src.n, factor);
     }
+    src = next_src;
+    dst = next_dst;
   }
+}
+
+__device__ __forceinline__ float load_any(const Chunk& c, int i) {
+  return c.type == FT_TYPE_F32 ? ((const float*)c.p)[i] : __half2float(((const __half*)c.p)[i]);
+}
+
+__global__ void __launch_bounds__(SMALL_THREADS)
+k_list_small(const Chunk* __restrict__ chunks, const Chunk* __restrict__ out, int count, float grad_scale,
+             float max_norm, float* __restrict__ norm_out, int in_place) {
+  __shared__ double red[SMALL_THREADS / 32];
+  constexpr int WARPS = SMALL_THREADS / 32, PER = SMALL_CHUNKS / WARPS, VALUES = SMALL_CHUNK / 32;
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float v[PER][VALUES];
+  Chunk dst[PER];
+  double acc = 0.0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int c = warp + j * WARPS;
+    Chunk src = {};
+    dst[j] = Chunk{};
+    if (c < count) {
+      src = chunks[c];
+      if (out) dst[j] = out[c];
+    }
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) v[j][k] = lane + 32 * k < (int)src.n ? load_any(src, lane + 32 * k) : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) acc = fma((double)v[j][k], (double)v[j][k], acc);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0) red[warp] = acc;
+  __syncthreads();
+  double sum = red[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const Verdict d = judge(sum, grad_scale, max_norm);
+  if (threadIdx.x == 0 && norm_out) d.publish(norm_out);
+  if (!out || !d.finite || (in_place && d.factor == 1.0f)) return;
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) {
+      const int i = lane + 32 * k;
+      if (i >= (int)dst[j].n) continue;
+      if (dst[j].type == FT_TYPE_F32) ((float*)dst[j].p)[i] = d.factor * v[j][k];
+      else ((__half*)dst[j].p)[i] = __float2half_rn(d.factor * v[j][k]);
+    }
 }
 
 struct Span {
@@ -123,7 +324,9 @@ struct FtGradList {
   std::vector<int> types;
   std::vector<Span> spans;      // of the tensors that are not empty, by address
   bool disjoint = true;
+  int type = -1;                // FT_TYPE_* of every tensor, -1 for a list of both
   int chunks = 0;
+  bool small = false;           // chunks of SMALL_CHUNK for k_list_small, else of CHUNK
   Chunk* table = nullptr;       // [chunks] on the device
   double* partials = nullptr;   // one sum for each block of k_list_squares
 };
@@ -158,10 +361,14 @@ int create_list(FtContext* ctx, size_t count, void* const* ptrs, const size_t* e
   l->elements.assign(elements, elements + count);
   l->types.assign(types, types + count);
   std::vector<Chunk> host;
+  size_t pieces = 0;
+  for (size_t i = 0; i < count; ++i) pieces += (elements[i] + SMALL_CHUNK - 1) / SMALL_CHUNK;
+  l->small = pieces <= SMALL_CHUNKS;
+  const size_t chunk = l->small ? SMALL_CHUNK : CHUNK;
   for (size_t i = 0; i < count; ++i) {
     const size_t size = types[i] == FT_TYPE_F32 ? 4 : 2;
-    for (size_t at = 0; at < elements[i]; at += CHUNK)
-      host.push_back({(char*)ptrs[i] + at * size, (uint32_t)std::min<size_t>(CHUNK, elements[i] - at), (uint32_t)types[i]});
+    for (size_t at = 0; at < elements[i]; at += chunk)
+      host.push_back({(char*)ptrs[i] + at * size, (uint32_t)std::min<size_t>(chunk, elements[i] - at), (uint32_t)types[i]});
     if (elements[i])
       l->spans.push_back({(uintptr_t)ptrs[i], (uintptr_t)ptrs[i] + elements[i] * size, i});
     FT_REQUIRE(host.size() < 0x7fffffffull, "ft_grad_list_create: too many elements");
@@ -173,6 +380,7 @@ int create_list(FtContext* ctx, size_t count, void* const* ptrs, const size_t* e
     reach = std::max(reach, s.end);
   }
   l->chunks = (int)host.size();
+  if (count && std::count(l->types.begin(), l->types.end(), types[0]) == (long)count) l->type = types[0];
   FT_CUDA(cudaMalloc((void**)&l->table, std::max<size_t>(1, host.size()) * sizeof(Chunk)));
   FT_CUDA(cudaMalloc((void**)&l->partials, (size_t)list_grid(l) * sizeof(double)));
   if (!host.empty()) {
@@ -188,13 +396,28 @@ void free_list(FtGradList* l) {
   delete l;
 }
 
-int launch_list(FtContext* ctx, FtGradList* l, const Chunk* out, float grad_scale, float max_norm, float* norm_out,
-                bool in_place) {
-  const int grid = list_grid(l);
-  FT_LAUNCH_PDL(ctx, k_list_squares, grid, LIST_THREADS, 0, l->table, l->chunks, l->partials);
-  FT_LAUNCH_PDL(ctx, k_list_scale, out ? grid : 1, LIST_THREADS, 0, l->table, out, l->chunks, l->partials, grid,
-                grad_scale, max_norm, norm_out, in_place ? 1 : 0);
+template <typename TI, typename TO>
+int launch_scale(FtContext* ctx, FtGradList* l, const FtGradList* out, float grad_scale, float max_norm, float* norm_out) {
+  const int grid = out ? std::max(1, std::min(l->chunks, ctx->sm_count * SCALE_BLOCKS_PER_SM)) : 1;
+  FT_LAUNCH_PDL(ctx, (k_list_scale<TI, TO>), grid, LIST_THREADS, 0, l->table, out ? out->table : nullptr, l->chunks,
+                l->partials, list_grid(l), grad_scale, max_norm, norm_out, out == l ? 1 : 0);
   return FT_OK;
+}
+
+int launch_list(FtContext* ctx, FtGradList* l, const FtGradList* out, float grad_scale, float max_norm, float* norm_out) {
+  if (l->small) {   // so is `out`: that follows from the counts alone
+    FT_LAUNCH_PDL(ctx, k_list_small, 1, SMALL_THREADS, 0, l->table, out ? out->table : nullptr, l->chunks, grad_scale,
+                  max_norm, norm_out, out == l ? 1 : 0);
+    return FT_OK;
+  }
+  FT_LAUNCH_PDL(ctx, k_list_squares, list_grid(l), LIST_THREADS, 0, l->table, l->chunks, l->partials);
+  const int from = l->type, to = out ? out->type : -1;
+  if (from < 0 || to < 0) return launch_scale<void, void>(ctx, l, out, grad_scale, max_norm, norm_out);
+  if (from == FT_TYPE_F32)
+    return to == FT_TYPE_F32 ? launch_scale<float, float>(ctx, l, out, grad_scale, max_norm, norm_out)
+                             : launch_scale<float, __half>(ctx, l, out, grad_scale, max_norm, norm_out);
+  return to == FT_TYPE_F32 ? launch_scale<__half, float>(ctx, l, out, grad_scale, max_norm, norm_out)
+                           : launch_scale<__half, __half>(ctx, l, out, grad_scale, max_norm, norm_out);
 }
 
 }  // namespace
@@ -245,7 +468,7 @@ extern "C" int ft_global_grad_norm(FtContext* ctx, FtGradList* grads, float grad
   FT_REQUIRE(!overlaps_any(grads->spans, grads->disjoint, (uintptr_t)norm_out, (uintptr_t)(norm_out + 4)),
              "ft_global_grad_norm: norm_out overlaps a gradient");
   FtDeviceScope on(ctx);
-  return launch_list(ctx, grads, nullptr, grad_scale, 0.f, norm_out, false);
+  return launch_list(ctx, grads, nullptr, grad_scale, 0.f, norm_out);
 }
 
 extern "C" int ft_clip_grad_global_norm(FtContext* ctx, FtGradList* grads, FtGradList* out, float grad_scale,
@@ -279,5 +502,5 @@ extern "C" int ft_clip_grad_global_norm(FtContext* ctx, FtGradList* grads, FtGra
                "%s: norm_out overlaps a tensor", who);
   }
   FtDeviceScope on(ctx);
-  return launch_list(ctx, grads, out->table, grad_scale, max_norm, norm_out, out == grads);
+  return launch_list(ctx, grads, out, grad_scale, max_norm, norm_out);
 }

@@ -91,7 +91,7 @@ def _check_values(out, src, factor):
         assert ((o.double() - want).abs() <= tol).all()
 
 
-SHAPES = [[1], [0, 5, 0], [3, 1, 8192, 8193, 7], [100000, 33], [16] * 400, [2 * 8192 * 1300 + 5], [31] * 3 + [70001] * 9]
+SHAPES = [[1], [0, 5, 0], [256] * 64, [256] * 63 + [257], [16384], [100] * 40, [3, 1, 8192, 8193, 7], [100000, 33], [16] * 400, [2 * 8192 * 1300 + 5], [31] * 3 + [70001] * 9]
 
 
 @gpu
