@@ -40,10 +40,12 @@ struct Rows {
   int* source;        // its row in the caller's tensors
   uint32_t* target;
   float* weight;      // grad_scale * weights[row]
-  float2* stat;       // running {maximum, sum of exponentials against it}
+  float2* stat;       // running {maximum, sum of exponentials against it}; E, at the end: factors of dh's two terms
   float* picked;      // logit of the target
   float* exact;       // the same from f32 products, beside the tensor cores' sum
   float* lse;
+  float* base;        // E: the point R that the row's sums are scaled against, in log2 units
+  float2* kept;       // E: {value, reference point} of the target
 };
 
 struct Problem {
@@ -88,6 +90,8 @@ inline Rows carve_rows(Carver& c, int T) {
   r.picked = c.take<float>(T);
   r.exact = c.take<float>(T);
   r.lse = c.take<float>(T);
+  r.base = c.take<float>(T);
+  r.kept = c.take<float2>(T);
   return r;
 }
 

@@ -1,17 +1,26 @@
 // The products of the linear cross entropy on the tensor cores (FT_GEMM_F16 and FT_GEMM_F16X2).
 //
-// One kernel serves all of them: C[256 x 256 tile] = sum over (plane pairs, K) of A . B^T on a CTA
+// One kernel serves all of them: C[256 x tile_n tile] = sum over (plane pairs, K) of A . B^T on a CTA
 // pair (tcgen05 cta_group::2), with either operand K-contiguous or M/N-contiguous in memory, so no
 // operand is ever transposed:
-//   logits   A = packed rows,    B = W            K = hidden    epilogue: row statistics, or g
-//   dh       A = g,              B = W            K = a vocabulary piece (in `splits` parts)
+//   logits   A = packed rows,    B = W            K = hidden    epilogue: row statistics, E, or g
+//   dh       A = E or g,         B = W            K = a vocabulary piece (in `splits` parts)
 //   dW       A = g, B = rows (W is [vocab, hidden]) or A = rows, B = g ([hidden, vocab])   K = rows
 //
+// dW's K runs over rows, so its operand g must be normalised, which needs every row's log-sum-exp
+// first: the logits are computed twice.  dh alone does not need that.  The pass that finds the
+// statistics writes E = 2^(z2 - ref) for each column tile (z2 in log2 units, ref the row's maximum in
+// that tile: E has f16's full precision whatever the row's normaliser turns out to be), and the
+// product E W is drained from tensor memory once a tile of K and scaled there, in f32, by the
+// row's 2^(ref - R).  R is the row's maximum when its first piece was done; the rest of the
+// normaliser and the one-hot term, -w W(:, y), are applied by the pass that unpacks the rows.
+// That saves a third of the multiplications of a frozen head's gradient.
+//
 // Planes: an f16 operand, and an f32 one in FT_GEMM_F16, is one f16 plane.  FT_GEMM_F16X2 carries an
-// f32 operand and g as two planes, hi = f16(x) and lo = f16(x - hi), of which the products hi.hi,
-// hi.lo and lo.hi are summed: 22 bits.  The tensor core adds each group of 16 products into its f32
-// accumulator with the low bits cut off, a loss of up to K/16 x 2^-24 of the sum, so that mode also
-// sums at most SLICE_KB x 64 of K in tensor memory and adds the slices up in registers.
+// f32 operand and g (or E) as two planes, hi = f16(x) and lo = f16(x - hi), of which the products
+// hi.hi, hi.lo and lo.hi are summed: 22 bits.  The tensor core adds each group of 16 products into
+// its f32 accumulator with the low bits cut off, a loss of up to K/16 x 2^-24 of the sum, so that mode
+// also sums at most 512 of K in tensor memory and adds the slices up in registers.
 //
 // Roles and barriers as in ft_gemm_tc.cu's pair kernel: warp 0 loads (TMA), warp 1 of the even CTA
 // issues the products, warps 2..9 drain.  Every wait is bounded; a wait that runs out sets the
@@ -33,29 +42,37 @@ constexpr int OPERAND_BYTES = 128 * BK * 2;
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int EPI_OFFSET = STAGES * STAGE_BYTES;      // 8 epilogue warps x 4 KiB
 constexpr int BAR_OFFSET = EPI_OFFSET + 8 * 4096;
-constexpr int SMEM_BYTES = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
-constexpr int SLICE_KB = 8;
+constexpr int BARRIERS = 2 * STAGES + 8;              // full, empty, tfull[2], tempty[2], one a quadrant
+constexpr int SMEM_BYTES = BAR_OFFSET + BARRIERS * 8 + 16 + 1024;
 
-enum Epi { EPI_STATS, EPI_GRAD, EPI_STORE };
-// The statistics' launch has two warps more, for the targets' logits.
-constexpr int threads_of(int epi) { return epi == EPI_STATS ? GEMM_THREADS + 64 : GEMM_THREADS; }
+// STATS: row statistics.  EXP: statistics and E.  GRAD: g.  STORE: the sum.  FACTOR: the sum with every
+// TILE of K scaled by its row's factor.
+enum Epi { EPI_STATS, EPI_EXP, EPI_GRAD, EPI_STORE, EPI_FACTOR };
+// The statistics' launches have two warps more, for the targets' logits.
+constexpr int threads_of(int epi) { return epi <= EPI_EXP ? GEMM_THREADS + 64 : GEMM_THREADS; }
+// k-blocks of 64 that are summed in tensor memory; 0: all
+constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
 
 struct TcProduct {
   int M, N, K;
   int live_m, live_k;               // 1: that extent is the number of supervised rows
   int splits;                       // parts of K, each with a slab of its own
+  int tile_n;                       // columns of a tile: a multiple of 32 up to TILE
   int n_fast, band;                 // order of the tiles
+  int a_second;                     // whether the odd CTA's rows are loaded (not: at most 128 rows, nobody reads them)
+  int stage_tx;                     // bytes of a stage, both CTAs
   int terms;                        // plane pairs, the small ones first
   int a_plane[3], b_plane[3];
   int a_mn0, b_mn0, k0;             // where M, N and K begin in the operands' tensors...
   int a_has_k0, b_has_k0;           // ... and which of them k0 applies to
   // EPI_STATS, EPI_GRAD
   Rows rw;
-  float2* part;                     // [2 * column tiles][part_ld]
+  float2* part;                     // [2 * column tiles][part_ld]: {maximum in log2 units, sum}
   int part_ld;
+  __half* wy;                       // EXP: the targets' columns of W, [planes][part_ld][wy_ld]
+  int wy_ld;
   int v0, vocab;                    // first vocabulary column of the launch, columns in all
-  int g_planes;
-  // EPI_STATS: the operands again, for the targets' logits
+  // EPI_STATS, EPI_EXP: the operands again, for the targets' logits
   const __half *h, *w;              // value (k, plane) of a row at h + row * h_ld + plane * h_plane + k,
   long long h_ld, h_plane;          // W(k, v) at w + k * w_sk + v * w_sv + plane * w_plane
   long long w_sk, w_sv, w_plane;
@@ -101,10 +118,11 @@ struct Unit { int mt, nt, sp; };
 __device__ __forceinline__ Unit decode_unit(int u, int tiles_m, int tiles_n, const TcProduct& g) {
   Unit r;
   if (g.n_fast) {
+    // parts of K slowest: the tiles that run together read the same slice of B
     r.nt = u % tiles_n;
     const int v = u / tiles_n;
-    r.sp = v % g.splits;
-    r.mt = v / g.splits;
+    r.mt = v % tiles_m;
+    r.sp = v / tiles_m;
   } else {
     const int per_band = g.band * tiles_n * g.splits;
     const int b = u / per_band, in = u - b * per_band;
@@ -136,23 +154,42 @@ __device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const
 // but the loss of a row that is sure of its target is as exact, relative to itself, as that one
 // logit is exact in absolute terms.  [hidden, vocab] weights cost a 32-byte sector for every 2
 // bytes here; beside the products nobody waits for them.
+// KEEP: the column goes to wy as well, for the one-hot term of dh.
+template <bool KEEP>
 __device__ __forceinline__ float target_dot(const TcProduct& g, int row, uint32_t target, int lane) {
-  const __half* h = g.h + (long long)row * g.h_ld;
-  const __half* w = g.w + (long long)target * g.w_sv;
+  constexpr int AT_ONCE = 16;   // loads in flight before the first use (and before a store that might alias them)
   float acc = 0.f;
-#pragma unroll 8
-  for (int k = lane; k < g.K; k += 32) {
-    float a = __half2float(h[k]), b = __half2float(w[k * g.w_sk]);
-    if (g.h_planes == 2) a += __half2float(h[g.h_plane + k]);
-    if (g.w_planes == 2) b += __half2float(w[g.w_plane + k * g.w_sk]);
-    acc = fmaf(a, b, acc);
+  for (int pw = 0; pw < g.w_planes; ++pw) {
+    const __half* h = g.h + (long long)row * g.h_ld;
+    const __half* w = g.w + pw * g.w_plane + (long long)target * g.w_sv;
+    __half* keep = KEEP ? g.wy + ((long long)pw * g.part_ld + row) * g.wy_ld : nullptr;
+    for (int k0 = lane; k0 < g.K; k0 += 32 * AT_ONCE) {
+      __half b[AT_ONCE];
+      float a[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int k = k0 + 32 * j;
+        b[j] = k < g.K ? w[k * g.w_sk] : __float2half(0.f);
+        a[j] = k < g.K ? __half2float(h[k]) : 0.f;
+      }
+      if (g.h_planes == 2) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+          if (k0 + 32 * j < g.K) a[j] += __half2float(h[g.h_plane + k0 + 32 * j]);
+      }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        acc = fmaf(a[j], __half2float(b[j]), acc);
+        if (KEEP && k0 + 32 * j < g.K) keep[k0 + 32 * j] = b[j];
+      }
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
   return acc;
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool SPLIT>
+template <int EPI, bool A_MN, bool B_MN, bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
@@ -164,7 +201,8 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const uint32_t bar_empty = bar_full + STAGES * 8;
   const uint32_t bar_tfull = bar_empty + STAGES * 8;
   const uint32_t bar_tempty = bar_tfull + 2 * 8;
-  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + (2 * STAGES + 4) * 8);
+  const uint32_t bar_quad = bar_tempty + 2 * 8;
+  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + BARRIERS * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -180,6 +218,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       mbar_init(bar_tfull + b * 8, 1);
       mbar_init(bar_tempty + b * 8, 16);
     }
+    for (int b = 0; b < 4; ++b) mbar_init(bar_quad + b * 8, 2);   // the two warps of a quadrant
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -201,10 +240,16 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const int live = g.rw.head->count;
   // no supervised row at all still makes one tile (of zeros): gradients are overwritten, not left
   const int tiles_m = g.live_m ? max(1, (live + TILE - 1) / TILE) : (g.M + TILE - 1) / TILE;
-  const int tiles_n = (g.N + TILE - 1) / TILE;
+  const int tile_n = EPI == EPI_EXP || EPI == EPI_GRAD ? TILE : g.tile_n;
+  const int tiles_n = (g.N + tile_n - 1) / tile_n;
   const int units = tiles_m * tiles_n * g.splits;
   const int kb_all = g.live_k ? max(1, (live + BK - 1) / BK) : (g.K + BK - 1) / BK;
-  const int slice = SPLIT ? SLICE_KB : kb_all;
+  constexpr int SLICE = slice_of(EPI, TWO);
+  const int slice = SLICE ? SLICE : kb_all;
+  // FACTOR: parts of K begin with a tile of E
+  constexpr int GRAIN = EPI == EPI_FACTOR ? SLICE : 1;
+  const int grains = (kb_all + GRAIN - 1) / GRAIN;
+  auto k_begin = [&](int sp) { return min(kb_all, GRAIN * (int)((long long)grains * sp / g.splits)); };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
@@ -213,8 +258,8 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       const int ak0 = g.a_has_k0 ? g.k0 : 0, bk0 = g.b_has_k0 ? g.k0 : 0;
       for (int u = pair; u < units && !*abort_flag; u += npairs) {
         const Unit un = decode_unit(u, tiles_m, tiles_n, g);
-        const int kb0 = (int)((long long)kb_all * un.sp / g.splits), kb1 = (int)((long long)kb_all * (un.sp + 1) / g.splits);
-        const int am = g.a_mn0 + un.mt * TILE + (int)rank * 128, bn = g.b_mn0 + un.nt * TILE + (int)rank * 128;
+        const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
+        const int am = g.a_mn0 + un.mt * TILE + (int)rank * 128, bn = g.b_mn0 + un.nt * tile_n + (int)rank * (tile_n / 2);
         for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice) {
           const int s1 = min(kb1, s0 + slice);
           for (int t = 0; t < g.terms; ++t) {
@@ -223,8 +268,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               if (!mbar_wait(bar_empty + stage * 8, phase ^ 1, abort_flag, status, 21)) break;
               const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OPERAND_BYTES;
               const uint32_t bar = lead_full + stage * 8;
-              if (rank == 0) mbar_expect_tx(bar_full + stage * 8, 2 * STAGE_BYTES);
-              if constexpr (A_MN) {
+              if (rank == 0) mbar_expect_tx(bar_full + stage * 8, (uint32_t)g.stage_tx);
+              if (rank != 0 && !g.a_second) {
+              } else if constexpr (A_MN) {
                 tma_load_3d_pair(sa, &map_a, bar, am, ak0 + kb * BK, pa);
                 tma_load_3d_pair(sa + 8192, &map_a, bar, am + 64, ak0 + kb * BK, pa);
               } else {
@@ -232,7 +278,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               }
               if constexpr (B_MN) {
                 tma_load_3d_pair(sb, &map_b, bar, bn, bk0 + kb * BK, pb);
-                tma_load_3d_pair(sb + 8192, &map_b, bar, bn + 64, bk0 + kb * BK, pb);
+                if (tile_n > 128) tma_load_3d_pair(sb + 8192, &map_b, bar, bn + 64, bk0 + kb * BK, pb);
               } else {
                 tma_load_3d_pair(sb, &map_b, bar, bk0 + kb * BK, bn, pb);
               }
@@ -246,12 +292,12 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (leader only)
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = make_idesc(256, 256, 0, 0) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16);
+      const uint32_t idesc = make_idesc(256, tile_n, 0, 0) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16);
       uint32_t stage = 0, phase = 0;
       int local = 0;
       for (int u = pair; u < units && !*abort_flag; u += npairs) {
         const Unit un = decode_unit(u, tiles_m, tiles_n, g);
-        const int kb0 = (int)((long long)kb_all * un.sp / g.splits), kb1 = (int)((long long)kb_all * (un.sp + 1) / g.splits);
+        const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
         for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice, ++local) {
           const int todo = (min(kb1, s0 + slice) - s0) * g.terms;
           const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
@@ -277,37 +323,39 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
     }
     __syncwarp();
-  } else if (EPI == EPI_STATS && warp >= GEMM_THREADS / 32) {
+  } else if (EPI <= EPI_EXP && warp >= GEMM_THREADS / 32) {
     // ------------------------------------------------------------------ the targets' logits
     const float c2 = g.rw.head->z_scale * 1.4426950408889634f;
     for (int r = (int)blockIdx.x * 2 + warp - GEMM_THREADS / 32; r < live; r += (int)gridDim.x * 2) {
       const uint32_t y = g.rw.target[r];
-      if (y >= (uint32_t)g.vocab) continue;
-      const float z = target_dot(g, r, y, lane);
+      if (y - (uint32_t)g.v0 >= (uint32_t)g.N) continue;           // in this launch's columns?
+      const float z = target_dot<EPI == EPI_EXP>(g, r, y, lane);
       if (lane == 0) g.rw.exact[r] = z * c2;
     }
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
-    // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the two warps of a quadrant take 128
-    // columns each, in four chunks of 32.
+    // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the two warps of a quadrant take half of
+    // the columns each, in up to four chunks of 32.
     const int quad = warp & 3, grp = (warp - 2) >> 2;
+    const int half = (tile_n / 32 + 1) / 2, mine = grp ? tile_n / 32 - half : half;
     uint8_t* st = gbase + EPI_OFFSET + (warp - 2) * 4096;
     const uint32_t st_addr = smem_u32(st);
-    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * 128;
-    const float z_scale = g.rw.head->z_scale;                      // accumulator -> logit
-    const float c2 = z_scale * 1.4426950408889634f;                // accumulator -> log2 units
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * half * 32;
+    const float c2 = g.rw.head->z_scale * 1.4426950408889634f;     // accumulator -> logit in log2 units
     // rows that a store may reach: all of a tile where the rows are packed ones (their buffers end with
     // a tile), else those of the output
     const int rows_end = g.live_m ? tiles_m * TILE : g.M;
     int local = 0;
+    uint32_t quad_phase = 0;
     for (int u = pair; u < units && !*abort_flag; u += npairs) {
       const Unit un = decode_unit(u, tiles_m, tiles_n, g);
-      const int kb0 = (int)((long long)kb_all * un.sp / g.splits), kb1 = (int)((long long)kb_all * (un.sp + 1) / g.splits);
-      const int row = un.mt * TILE + (int)rank * 128 + quad * 32 + lane;
-      const int col = un.nt * TILE + grp * 128;                    // first column of this warp, from the launch's first
+      const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
+      const int y0 = un.mt * TILE + (int)rank * 128 + quad * 32;   // first row of this warp
+      const int row = y0 + lane;
+      const int col = un.nt * tile_n + grp * half * 32;            // its first column, from the launch's first
       uint32_t target = FT_MASKED_CE_SKIP;
-      float lse2 = 0.f, wg = 0.f, alpha = 1.f;
-      if constexpr (EPI != EPI_STORE) {
+      float lse2 = 0.f, wg = 0.f, alpha = 1.f, base2 = 0.f;
+      if constexpr (EPI <= EPI_GRAD) {
         if (row < live) {
           target = g.rw.target[row] - (uint32_t)(g.v0 + col);      // relative to this warp's columns
           if constexpr (EPI == EPI_GRAD) {
@@ -315,13 +363,28 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             wg = g.rw.weight[row] * g.rw.head->g_scale;
           }
         }
-      } else {
+      } else if constexpr (EPI == EPI_STORE) {
         if (g.unscale) alpha = g.rw.head->g_unscale * g.rw.head->h_unscale;
+      } else {
+        if (row < live) base2 = g.rw.base[row];
       }
       float run_m = -INFINITY, run_s = 0.f;
-      const int y0 = un.mt * TILE + (int)rank * 128 + quad * 32;   // first row of this warp
-      uint32_t low[SPLIT && EPI == EPI_GRAD ? 2 : 1][16];          // the second plane, until its store
+      uint32_t low[TWO && (EPI == EPI_EXP || EPI == EPI_GRAD) ? 2 : 1][16];   // the second plane, until its store
 
+      auto mask_columns = [&](int c0, float (&v)[32]) {
+        const int left = g.vocab - (g.v0 + c0);                    // columns of the chunk inside the vocabulary
+        if (left < 32) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (k >= left) v[k] = -INFINITY;
+        }
+      };
+      auto max_of = [&](const float (&v)[32]) {
+        float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int k = 4; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], v[k]);
+        return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      };
       auto store_f16_pair = [&](int x, int y, int plane) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -330,30 +393,47 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           bulk_commit();
         }
       };
+      // chunk i of an f16 result (v: its values): two chunks make the 64 columns of a store
+      auto put_f16 = [&](int i, int c0, const float (&v)[32]) {
+        uint32_t hi[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          hi[k >> 1] = pack_h2(v[k], v[k + 1]);
+          if constexpr (TWO) {
+            const float2 f = __half22float2(*(const __half2*)&hi[k >> 1]);
+            low[i & 1][k >> 1] = pack_h2(v[k] - f.x, v[k + 1] - f.y);
+          }
+        }
+        if ((i & 1) == 0) {
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+        }
+        stage_f16(st, lane, i & 1, hi);
+        if (i & 1) {
+          store_f16_pair(c0 - 32, y0, 0);
+          if constexpr (TWO) {
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();
+            stage_f16(st, lane, 0, low[0]);
+            stage_f16(st, lane, 1, low[1]);
+            store_f16_pair(c0 - 32, y0, 1);
+          }
+        }
+      };
+
       // what happens to chunk i (columns col + 32 i .. + 31) of the finished sum
       auto finish = [&](int i, float (&v)[32]) {
         const int c0 = col + 32 * i;
+        const uint32_t y = target - 32u * (uint32_t)i;
         if constexpr (EPI == EPI_STATS) {
-          const int left = g.vocab - (g.v0 + c0);                  // columns of the chunk inside the vocabulary
-          if (left < 32) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (k >= left) v[k] = -INFINITY;
-          }
-          float m = v[0];
-#pragma unroll
-          for (int k = 1; k < 32; ++k) m = fmaxf(m, v[k]);
-          m = fmaxf(run_m, m * c2);
+          mask_columns(c0, v);
+          const float m = fmaxf(run_m, max_of(v) * c2);
           const float ref = finite_max(m);
-          float s0 = 0.f, s1 = 0.f;
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            s0 += ex2(fmaf(v[k], c2, -ref));
-            s1 += ex2(fmaf(v[k + 1], c2, -ref));
-          }
-          run_s = run_s * ex2(run_m - ref) + (s0 + s1);
+          for (int k = 0; k < 32; ++k) s[k & 3] += ex2(fmaf(v[k], c2, -ref));
+          run_s = run_s * ex2(run_m - ref) + ((s[0] + s[1]) + (s[2] + s[3]));
           run_m = m;
-          const uint32_t y = target - 32u * (uint32_t)i;
           if (y < 32u) {
             float z = 0.f;
 #pragma unroll
@@ -361,40 +441,38 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               if (y == (uint32_t)k) z = v[k];
             g.rw.picked[row] = z * c2;
           }
-        } else if constexpr (EPI == EPI_GRAD) {
-          uint32_t hi[16];
-          const uint32_t y = target - 32u * (uint32_t)i;
+        } else if constexpr (EPI == EPI_EXP) {
+          // (run_m is the whole tile's maximum by now)
+          mask_columns(c0, v);
+          const float ref = finite_max(run_m);
+          if (y < 32u) {
+            float z = 0.f;
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            float p0 = ex2(fmaf(v[k], c2, -lse2)), p1 = ex2(fmaf(v[k + 1], c2, -lse2));
-            if (y == (uint32_t)k) p0 -= 1.f;
-            if (y == (uint32_t)(k + 1)) p1 -= 1.f;
-            p0 *= wg;
-            p1 *= wg;
+            for (int k = 0; k < 32; ++k)
+              if (y == (uint32_t)k) z = v[k];
+            const float e = ex2(fmaf(z, c2, -ref));
+            float kept = __half2float(__float2half_rn(e));         // as the product will see it
+            if (TWO) kept += __half2float(__float2half_rn(e - kept));
+            g.rw.picked[row] = z * c2;
+            g.rw.kept[row] = make_float2(kept, ref);
+          }
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            v[k] = ex2(fmaf(v[k], c2, -ref));
+            s[k & 3] += v[k];
+          }
+          run_s += (s[0] + s[1]) + (s[2] + s[3]);
+          put_f16(i, c0, v);
+        } else if constexpr (EPI == EPI_GRAD) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            v[k] = ex2(fmaf(v[k], c2, -lse2));
+            if (y == (uint32_t)k) v[k] -= 1.f;
             // rows behind the last supervised one hold zeros: they are part of dW's K
-            if (row >= live) p0 = p1 = 0.f;
-            hi[k >> 1] = pack_h2(p0, p1);
-            if constexpr (SPLIT) {
-              const float2 f = __half22float2(*(const __half2*)&hi[k >> 1]);
-              low[i & 1][k >> 1] = pack_h2(p0 - f.x, p1 - f.y);
-            }
+            v[k] = row < live ? v[k] * wg : 0.f;
           }
-          // two chunks make the 64 columns of a store
-          if ((i & 1) == 0) {
-            if (lane == 0) bulk_wait_read();
-            __syncwarp();
-          }
-          stage_f16(st, lane, i & 1, hi);
-          if (i & 1) {
-            store_f16_pair(c0 - 32, y0, 0);
-            if constexpr (SPLIT) {
-              if (lane == 0) bulk_wait_read();
-              __syncwarp();
-              stage_f16(st, lane, 0, low[0]);
-              stage_f16(st, lane, 1, low[1]);
-              store_f16_pair(c0 - 32, y0, 1);
-            }
-          }
+          put_f16(i, c0, v);
         } else {
           if (c0 >= g.N || y0 >= rows_end) return;                 // the whole block lies outside
 #pragma unroll
@@ -435,8 +513,31 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
         }
       };
+      // EXP: the maximum over the tile's 256 columns, half of which the quadrant's other warp holds
+      auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_quad + quad * 8);
+        const bool ok = mbar_wait(bar_quad + quad * 8, quad_phase, abort_flag, status, 25);
+        quad_phase ^= 1;
+        return ok;
+      };
+      auto join_max = [&](float m) {
+        float* slot = (float*)(gbase + EPI_OFFSET) + (warp - 2) * 1024;       // the staging tiles, free at this point
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+        slot[lane] = m;
+        if (!meet()) return m;
+        const float other = ((const float*)(gbase + EPI_OFFSET))[((warp - 2) ^ 4) * 1024 + lane];
+        meet();
+        return fmaxf(m, other);
+      };
+      auto release = [&](uint32_t buf) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(lead_tempty + buf * 8);
+      };
 
-      if constexpr (SPLIT) {
+      if constexpr (SLICE > 0) {
         float acc[4][32];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -444,43 +545,67 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           for (int k = 0; k < 32; ++k) acc[i][k] = 0.f;
         for (int s0 = kb0; s0 < kb1; s0 += slice, ++local) {
           const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+          float f = 1.f;
+          if constexpr (EPI == EPI_FACTOR) {
+            // (a difference of two infinities belongs to a row of NaN anyway)
+            if (row < live) f = ex2(finite_max(g.part[(size_t)(2 * (s0 / SLICE)) * g.part_ld + row].x) - base2);
+          }
           if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
+            if (i >= mine) continue;
             uint32_t r[32];
             tc_ld32(t_lane + buf * TILE + i * 32, r);
             tc_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) acc[i][k] += __uint_as_float(r[k]);
+            for (int k = 0; k < 32; ++k)
+              acc[i][k] = EPI == EPI_FACTOR ? fmaf(f, __uint_as_float(r[k]), acc[i][k]) : acc[i][k] + __uint_as_float(r[k]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(lead_tempty + buf * 8);
+          release(buf);
         }
         if (*abort_flag) break;
+        if constexpr (EPI == EPI_EXP) {
+          float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) finish(i, acc[i]);
+          for (int i = 0; i < 4; ++i) {
+            mask_columns(col + 32 * i, acc[i]);
+            m = fmaxf(m, max_of(acc[i]));
+          }
+          run_m = join_max(m * c2);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < mine) finish(i, acc[i]);
       } else {
         const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
         ++local;
         if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
         tc_fence_after();
+        if constexpr (EPI == EPI_EXP) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v[32];
+            tc_ld32(t_lane + buf * TILE + i * 32, *(uint32_t(*)[32])v);
+            tc_wait_ld();
+            mask_columns(col + 32 * i, v);
+            m = fmaxf(m, max_of(v));
+          }
+          run_m = join_max(m * c2);
+        }
+        if (mine == 0) release(buf);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          if (i >= mine) continue;
           float v[32];
           tc_ld32(t_lane + buf * TILE + i * 32, *(uint32_t(*)[32])v);
           tc_wait_ld();
-          if (i == 3) {
-            // all four chunks are in registers: the accumulator may be overwritten
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(lead_tempty + buf * 8);
-          }
+          if (i == mine - 1) release(buf);                         // all chunks have been read
           finish(i, v);
         }
       }
-      if constexpr (EPI == EPI_STATS) g.part[(size_t)(un.nt * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+      if constexpr (EPI <= EPI_EXP) g.part[(size_t)(un.nt * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
     }
     // what was stored is complete before the launch ends
     if (lane == 0) bulk_wait_all();
@@ -501,45 +626,96 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 }
 
 // ------------------------------------------------------------------------------ around the products
-// Joins the column tiles' {maximum, sum} of 32 rows, tiles over 16 warps in a fixed order, and writes
-// the row's log-sum-exp (in log2 units, as the gradient's epilogue wants it) and its loss.
+// Joins the column tiles' {maximum, sum} of 32 rows, tiles over 16 warps in a fixed order, with what
+// the pieces before (not `first`) have left; after the last piece writes the row's log-sum-exp (in
+// log2 units, as the gradient's epilogue wants it) and its loss.
+// With `acc` (E is in use): sets the point R that the row's E W is scaled against.  It stays the maximum
+// of the first piece, and f32 carries what later pieces are above it, unless that is 2^64 or
+// more: then it moves, and the row's sums so far are scaled down.
 constexpr int LOSS_WARPS = 16;
 __global__ void __launch_bounds__(32 * LOSS_WARPS)
-k_ce_loss(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int vocab, float* __restrict__ row_loss) {
+k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int first, int last, int vocab,
+          float* __restrict__ row_loss, float* __restrict__ acc, size_t slab, int splits, int ld, int H) {
   __shared__ float2 red[LOSS_WARPS][32];
+  __shared__ float shrink[32];
   ft_pdl_wait();
   ft_pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   const int live = rw.head->count;
-  if (blockIdx.x * 32 >= live) return;
+  if ((int)blockIdx.x * 32 >= live) return;
   float m = -INFINITY, s = 0.f;
-  for (int p = warp; p < parts; p += LOSS_WARPS) {
-    const float2 v = part[(size_t)p * part_ld + row];
-    const float mn = fmaxf(m, v.x), ref = finite_max(mn);
-    s = s * ex2(m - ref) + v.y * ex2(v.x - ref);
+  constexpr int AT_ONCE = 8;
+  for (int p0 = warp; p0 < parts; p0 += AT_ONCE * LOSS_WARPS) {
+    float2 v[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int p = p0 + j * LOSS_WARPS;
+      v[j] = p < parts ? part[(size_t)p * part_ld + row] : make_float2(-INFINITY, 0.f);
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) mn = fmaxf(mn, v[j].x);
+    const float ref = finite_max(mn);
+    s *= ex2(m - ref);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) s += v[j].y * ex2(v[j].x - ref);
     m = mn;
   }
   red[warp][lane] = make_float2(m, s);
   __syncthreads();
-  if (warp != 0 || row >= live) return;
-  float M = -INFINITY;
-  for (int w = 0; w < LOSS_WARPS; ++w) M = fmaxf(M, red[w][lane].x);
-  const float ref = finite_max(M);
-  float S = 0.f;
-  for (int w = 0; w < LOSS_WARPS; ++w) S += red[w][lane].y * ex2(red[w][lane].x - ref);
-  const float l2 = log2f(S);
-  rw.lse[row] = ref + l2;
-  float loss = 0.f;
-  if (rw.target[row] < (uint32_t)vocab) {
-    // the sum with the target's logit z replaced by its exact value z + d:
-    //   loss = log(e^(lse - z) + e^d - 1) - d = (lse - z) - d + log(1 + p (e^d - 1)),  p = e^(z - lse)
-    // (ref - z) first: a row that is sure of its target loses nothing to the size of its logits
-    const float z = rw.picked[row], above = ((ref - z) + l2) * 0.6931471805599453f;
-    const float d = (rw.exact[row] - z) * 0.6931471805599453f;
-    loss = above - d + log1pf(expf(-above) * expm1f(d));
+  if (warp == 0) {
+    shrink[lane] = 1.f;
+    if (row < live) {
+      const float2 old = first ? make_float2(-INFINITY, 0.f) : rw.stat[row];
+      float M = old.x;
+#pragma unroll
+      for (int w = 0; w < LOSS_WARPS; ++w) M = fmaxf(M, red[w][lane].x);
+      const float ref = finite_max(M);
+      float S = old.y * ex2(old.x - ref);
+#pragma unroll
+      for (int w = 0; w < LOSS_WARPS; ++w) S += red[w][lane].y * ex2(red[w][lane].x - ref);
+      if (!last) rw.stat[row] = make_float2(M, S);
+      if (acc) {
+        if (first) {
+          rw.base[row] = ref;
+        } else if (ref > rw.base[row] + 64.f) {
+          shrink[lane] = ex2(rw.base[row] - ref);
+          rw.base[row] = ref;
+        }
+      }
+      if (last) {
+        const float l2 = log2f(S);
+        rw.lse[row] = ref + l2;
+        float loss = 0.f;
+        if (rw.target[row] < (uint32_t)vocab) {
+          // the sum with the target's logit z replaced by its exact value z + d:
+          //   loss = log(e^(lse - z) + e^d - 1) - d = (lse - z) - d + log(1 + p (e^d - 1)),  p = e^(z - lse)
+          // (ref - z) first: a row that is sure of its target loses nothing to the size of its logits
+          const float z = rw.picked[row], above = ((ref - z) + l2) * 0.6931471805599453f;
+          const float d = (rw.exact[row] - z) * 0.6931471805599453f;
+          loss = above - d + log1pf(expf(-above) * expm1f(d));
+        }
+        row_loss[rw.source[row]] = loss;
+        if (acc) {
+          // the gradient at the target, p - 1, is -(1 - e^-loss), exact for a row that is sure of its
+          // target; what E W holds of it already goes off
+          const float w = rw.weight[row] * rw.head->w_unscale;
+          float b = 0.f;
+          if (rw.target[row] < (uint32_t)vocab) b = expm1f(-loss) - rw.kept[row].x * ex2(rw.kept[row].y - rw.lse[row]);
+          rw.stat[row] = make_float2(w * ex2(rw.base[row] - rw.lse[row]), w * b);
+        }
+      }
+    }
   }
-  row_loss[rw.source[row]] = loss;
+  if (!acc || first) return;
+  __syncthreads();
+  for (int r = 0; r < 32; ++r) {
+    const float f = shrink[r];
+    if (f == 1.f) continue;
+    for (int sp = 0; sp < splits; ++sp)
+      for (int c = threadIdx.x; c < H; c += 32 * LOSS_WARPS) acc[sp * slab + (size_t)(blockIdx.x * 32 + r) * ld + c] *= f;
+  }
 }
 
 // Largest finite magnitude of W (first `w_blocks` blocks) and of the supervised rows (the others).
@@ -638,6 +814,49 @@ k_ce_scatter(const float* __restrict__ acc, size_t slab, int splits, int ld, Row
   }
 }
 
+// The same for E: stat holds the factors of the row's sums and of its target's column of W.
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_ce_scatter_exp(const float* __restrict__ acc, size_t slab, int splits, int ld, Rows rw, const __half* __restrict__ wy,
+                 size_t wy_plane, int wy_ld, int w_planes, int H, int rows, T* __restrict__ out) {
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const int units = ld / 4;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * units; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / units), c = (int)(i % units) * 4;
+    const int at = rw.place[r];
+    float e[4] = {0.f, 0.f, 0.f, 0.f};
+    if (at >= 0) {
+      const float2 f = rw.stat[at];
+      const float* p = acc + (size_t)at * ld + c;
+      float4 v = *(const float4*)p;
+      uint2 y[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+      // a target outside the vocabulary has no column (wy's pitch is a multiple of 8)
+      if (f.y != 0.f) {
+        y[0] = *(const uint2*)(wy + (size_t)at * wy_ld + c);
+        if (w_planes == 2) y[1] = *(const uint2*)(wy + wy_plane + (size_t)at * wy_ld + c);
+      }
+      for (int s = 1; s < splits; ++s) {
+        const float4 x = *(const float4*)(p + s * slab);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      }
+      const float2 y0 = __half22float2(*(const __half2*)&y[0].x), y1 = __half22float2(*(const __half2*)&y[0].y);
+      const float2 z0 = __half22float2(*(const __half2*)&y[1].x), z1 = __half22float2(*(const __half2*)&y[1].y);
+      e[0] = fmaf(f.x, v.x, f.y * (y0.x + z0.x));
+      e[1] = fmaf(f.x, v.y, f.y * (y0.y + z0.y));
+      e[2] = fmaf(f.x, v.z, f.y * (y1.x + z1.x));
+      e[3] = fmaf(f.x, v.w, f.y * (y1.y + z1.y));
+    }
+    T* o = out + (size_t)r * H + c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < H) {
+        if constexpr (sizeof(T) == 2) o[k] = __float2half_rn(e[k]);
+        else o[k] = e[k];
+      }
+  }
+}
+
 // ------------------------------------------------------------------------------ host side
 int make_map3(FtContext* ctx, CUtensorMap* map, const void* ptr, bool f32, uint64_t inner, uint64_t rows, uint64_t planes,
               uint64_t ld, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
@@ -661,9 +880,9 @@ int make_map3(FtContext* ctx, CUtensorMap* map, const void* ptr, bool f32, uint6
   return FT_OK;
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool SPLIT>
+template <int EPI, bool A_MN, bool B_MN, bool TWO>
 int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g) {
-  auto kernel = k_ce_gemm<EPI, A_MN, B_MN, SPLIT>;
+  auto kernel = k_ce_gemm<EPI, A_MN, B_MN, TWO>;
   static bool ready[FT_MAX_DEVICES] = {};
   static int most[FT_MAX_DEVICES] = {};
   if (!ready[ctx->device]) {
@@ -682,9 +901,10 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
     most[ctx->device] = std::max(1, std::min(n, ctx->sm_count / 2));
     ready[ctx->device] = true;
   }
-  const long long units = (long long)ft_cdiv(g.M, TILE) * ft_cdiv(g.N, TILE) * g.splits;
+  const long long units = (long long)ft_cdiv(g.M, TILE) * ft_cdiv(g.N, g.tile_n) * g.splits;
   const int pairs = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
-  const char* const names[3] = {"k_ce_gemm<statistics>", "k_ce_gemm<g>", A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>"};
+  const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
+                                A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
   cudaError_t e = ft_launch_ex(ctx, kernel, 2 * pairs, threads_of(EPI), SMEM_BYTES, a, b, o, g, ctx->status_dev);
   if (ctx->profile_all) ft_prof_end(ctx);
@@ -712,18 +932,33 @@ constexpr size_t G_PIECE_BYTES = (size_t)256 << 20;
 
 struct TcPlan {
   Rows rows;
-  __half *h, *w, *grad;
+  __half *h, *w, *grad, *wy;
   float2* part;
   float* acc;
-  int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld, parts;
-  bool w_staged;
+  int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld;
+  int stat_n, out_n;         // columns of a tile: of the statistics alone, of dh and (vocab-major) dW
+  bool w_staged, by_exp;
   size_t bytes;
 };
+
+// Columns of a tile, a multiple of 32, for n columns and `rows` tiles of rows (times parts): whole
+// waves of pairs as full as they get.  A tile costs its columns and about 24 more.
+int pick_tile_n(long long n, long long row_tiles, int pairs) {
+  int best = TILE;
+  double least = 1e30;
+  for (int t = TILE; t >= 64; t -= 32) {
+    const long long tiles = row_tiles * ft_cdiv(n, t);
+    const double cost = (double)((tiles + pairs - 1) / pairs) * (t + 24);
+    if (cost < least * 0.995) { least = cost; best = t; }
+  }
+  return best;
+}
 
 TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void* base) {
   TcPlan pl = {};
   Carver c(base);
   const bool two = ctx->gemm_mode == FT_GEMM_F16X2;
+  const int pairs = std::max(1, ctx->sm_count / 2);
   pl.rows = carve_rows(c, q.T);
   pl.Tp = (int)ft_align_up((size_t)std::max(q.T, 1), TILE);
   pl.h_ld = (int)ft_align_up((size_t)q.H, 8);
@@ -734,11 +969,13 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   pl.w_cols = q.p.weight_vocab_major ? q.H : q.V;
   pl.w_staged = q.p.weight_type == FT_TYPE_F32 || pl.w_cols % 8 != 0 || ((uintptr_t)weight & 15) != 0;
   pl.w_ld = (int)ft_align_up((size_t)pl.w_cols, 8);
+  pl.by_exp = q.grad_hidden && !q.grad_weight;
   pl.h = c.take<__half>((size_t)pl.h_planes * pl.Tp * pl.h_ld);
   pl.w = pl.w_staged ? c.take<__half>((size_t)pl.w_planes * pl.w_rows * pl.w_ld) : nullptr;
-  pl.parts = 2 * ft_cdiv(q.V, TILE);
-  const size_t part_bytes = (size_t)pl.parts * pl.Tp * sizeof(float2);
-  size_t grad_bytes = 0;
+  // few row tiles: the columns of a tile follow the number of waves (the last one may be nearly empty)
+  pl.stat_n = pl.Tp <= 2 * TILE && !pl.by_exp ? pick_tile_n(q.V, pl.Tp / TILE, pairs) : TILE;
+  pl.out_n = pick_tile_n(q.H, 1 << 20, pairs);
+  size_t part_bytes = (size_t)2 * ft_cdiv(q.V, pl.stat_n) * pl.Tp * sizeof(float2), grad_bytes = 0;
   if (q.grad_hidden || q.grad_weight) {
     const size_t column = (size_t)pl.Tp * 2 * pl.g_planes;
     size_t cols = q.p.vocab_piece ? q.p.vocab_piece : std::max<size_t>(TILE, G_PIECE_BYTES / column);
@@ -746,17 +983,23 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
     // equal pieces of whole tiles
     pl.piece = (int)ft_align_up((size_t)ft_cdiv(q.V, pieces), TILE);
     grad_bytes = column * pl.piece;
+    if (pl.by_exp) part_bytes = (size_t)2 * (pl.piece / TILE) * pl.Tp * sizeof(float2);
   }
-  // the statistics of the column tiles are done with before the first piece of g is written
-  char* shared = c.take<char>(std::max(part_bytes, grad_bytes));
-  pl.part = (float2*)shared;
-  pl.grad = (__half*)shared;
+  if (pl.by_exp) {
+    pl.part = (float2*)c.take<char>(part_bytes);
+    pl.grad = (__half*)c.take<char>(grad_bytes);
+    pl.wy = c.take<__half>((size_t)pl.w_planes * pl.Tp * pl.h_ld);
+  } else {
+    // the statistics of the column tiles are done with before the first piece of g is written
+    char* shared = c.take<char>(std::max(part_bytes, grad_bytes));
+    pl.part = (float2*)shared;
+    pl.grad = (__half*)shared;
+  }
   pl.splits = 1;
   if (q.grad_hidden) {
-    // K parts: as many as fill the pairs in whole waves, each at least 1024 deep and 64 MB of slabs
+    // K parts: as many as fill the pairs in whole waves, each at least 1024 deep, 256 MB of slabs
     pl.acc_ld = (int)ft_align_up((size_t)q.H, 4);
-    const int pairs = std::max(1, ctx->sm_count / 2);
-    const long long tiles = (long long)(pl.Tp / TILE) * ft_cdiv(q.H, TILE);
+    const long long tiles = (long long)(pl.Tp / TILE) * ft_cdiv(q.H, pl.out_n);
     double best = 1e30;
     for (int s = 1; s <= 64 && s * 1024 <= std::max(1024, pl.piece); ++s) {
       if (s > 1 && (size_t)s * pl.Tp * pl.acc_ld * 4 > ((size_t)256 << 20)) break;
@@ -798,35 +1041,105 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       FT_LAUNCH_PDL(ctx, k_ce_weight<__half>, grid, 256, 0, (const __half*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
                     pl.w_planes, pl.rows.head);
   }
-  // K-contiguous operands come in boxes of 64 x 128 rows, M/N-contiguous ones in two of 64 x 64
+  // K-contiguous operands come in boxes of 64 x 128 rows (B: half a tile's columns), M/N-contiguous ones
+  // in two of 64 x 64
+  auto k_map = [&](CUtensorMap* m, const void* p, int inner, int rows, int planes, int ld, int box) {
+    return make_map3(ctx, m, p, false, inner, rows, planes, ld, 64, box);
+  };
+  auto mn_map = [&](CUtensorMap* m, const void* p, int inner, int rows, int planes, int ld) {
+    return make_map3(ctx, m, p, false, inner, rows, planes, ld, 64, 64);
+  };
+  auto tile = [&](TcProduct& p, int tile_n, int a_rows, bool b_mn) {
+    p.tile_n = tile_n;
+    p.a_second = a_rows == 128;
+    p.stage_tx = (a_rows == 128 ? 2 : 1) * a_rows * 128 + 2 * (b_mn ? (tile_n > 128 ? 2 : 1) * 8192 : tile_n / 2 * 128);
+  };
+  // at most 128 rows: the even CTA's are all there are, and only as many are loaded
+  int a_rows = 128;
+  while (T <= 128 && a_rows > 8 && a_rows / 2 >= T) a_rows /= 2;
+  if (T > 64) a_rows = 128;
   CUtensorMap h_k, w_k, w_mn;
-  FT_TRY(make_map3(ctx, &h_k, pl.h, false, H, pl.Tp, pl.h_planes, pl.h_ld, 64, 128));
-  FT_TRY(make_map3(ctx, &w_k, w, false, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, 64, 128));
-  FT_TRY(make_map3(ctx, &w_mn, w, false, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, 64, 64));
+  FT_TRY(k_map(&h_k, pl.h, H, pl.Tp, pl.h_planes, pl.h_ld, a_rows));
+  FT_TRY(mn_map(&w_mn, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld));
 
   TcProduct z = {};
-  z.M = T; z.K = H; z.live_m = 1; z.splits = 1;
+  z.M = T; z.N = V; z.K = H; z.live_m = 1; z.splits = 1;
   z.band = 32;
   set_terms(z, pl.h_planes, pl.w_planes);
-  z.rw = pl.rows; z.part = pl.part; z.part_ld = pl.Tp; z.vocab = V; z.g_planes = pl.g_planes;
-  z.N = V;
+  z.rw = pl.rows; z.part = pl.part; z.part_ld = pl.Tp; z.vocab = V;
   z.h = pl.h; z.h_ld = pl.h_ld; z.h_plane = (long long)pl.Tp * pl.h_ld; z.h_planes = pl.h_planes;
   z.w = (const __half*)w; z.w_plane = (long long)pl.w_rows * pl.w_ld; z.w_planes = pl.w_planes;
   z.w_sk = vm ? 1 : pl.w_ld; z.w_sv = vm ? pl.w_ld : 1;
-  if (vm) FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z)));
-  else FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z)));
-  FT_LAUNCH_PDL(ctx, k_ce_loss, ft_cdiv(T, 32), 32 * LOSS_WARPS, 0, pl.part, pl.Tp, pl.parts, pl.rows, V, t.row_loss);
+  z.wy = pl.wy; z.wy_ld = pl.h_ld;
+  const size_t slab = (size_t)pl.Tp * pl.acc_ld;
+  const int join_grid = ft_cdiv(T, 32);
+  CUtensorMap acc_out;
+  if (t.grad_hidden) FT_TRY(make_map3(ctx, &acc_out, pl.acc, true, pl.acc_ld, pl.Tp, pl.splits, pl.acc_ld, 32, 32));
+  const int unpack_grid = (int)std::min<long long>(ft_cdiv((long long)T * (pl.acc_ld / 4), 256), (long long)ctx->sm_count * 16);
+  CUtensorMap g_out, g_k;
+  if (t.grad_hidden || t.grad_weight)
+    FT_TRY(make_map3(ctx, &g_out, pl.grad, false, pl.piece, pl.Tp, pl.g_planes, pl.piece, 64, 32));
+
+  // the product with W of one piece of E or g, into the slabs
+  auto dh_product = [&](int v0, int cols) {
+    TcProduct p = {};
+    p.rw = pl.rows;
+    p.M = T; p.N = H; p.K = cols; p.live_m = 1;
+    p.splits = std::min(pl.splits, ft_cdiv(cols, pl.by_exp ? TILE : BK));
+    p.n_fast = 1; p.band = 1;
+    set_terms(p, pl.g_planes, pl.w_planes);
+    p.k0 = v0; p.b_has_k0 = 1;
+    p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
+    p.part = pl.part; p.part_ld = pl.Tp;
+    tile(p, pl.out_n, 128, vm);
+    return p;
+  };
+
+  if (pl.by_exp) {
+    FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, vm ? 128 : pl.out_n / 2));
+    tile(z, TILE, a_rows, !vm);
+    for (int v0 = 0; v0 < V; v0 += pl.piece) {
+      const int cols = std::min(pl.piece, V - v0);
+      const bool first = v0 == 0, last = v0 + cols == V;
+      z.N = cols; z.v0 = v0; z.b_mn0 = v0;
+      if (vm) FT_TRY((launch_gemm<EPI_EXP, false, false>(ctx, two, h_k, w_k, g_out, z)));
+      else FT_TRY((launch_gemm<EPI_EXP, false, true>(ctx, two, h_k, w_mn, g_out, z)));
+      FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(cols, TILE), pl.rows, first ? 1 : 0,
+                    last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
+      if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, 128));
+      const TcProduct p = dh_product(v0, cols);
+      if (vm) FT_TRY((launch_gemm<EPI_FACTOR, false, true, false>(ctx, g_k, w_mn, acc_out, p)));
+      else FT_TRY((launch_gemm<EPI_FACTOR, false, false, false>(ctx, g_k, w_k, acc_out, p)));
+    }
+    if (q.p.grad_hidden_type == FT_TYPE_F16)
+      FT_LAUNCH_PDL(ctx, k_ce_scatter_exp<__half>, unpack_grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, pl.wy,
+                    (size_t)pl.Tp * pl.h_ld, pl.h_ld, pl.w_planes, H, T, (__half*)t.grad_hidden);
+    else
+      FT_LAUNCH_PDL(ctx, k_ce_scatter_exp<float>, unpack_grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, pl.wy,
+                    (size_t)pl.Tp * pl.h_ld, pl.h_ld, pl.w_planes, H, T, (float*)t.grad_hidden);
+    return FT_OK;
+  }
+
+  tile(z, pl.stat_n, a_rows, !vm);
+  if (vm) {
+    FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, pl.stat_n / 2));
+    FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z)));
+  } else {
+    FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z)));
+  }
+  FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(V, pl.stat_n), pl.rows, 1, 1, V,
+                t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
   if (!t.grad_hidden && !t.grad_weight) return FT_OK;
 
-  CUtensorMap g_out, g_k, g_mn, acc_out, h_mn, dw_out;
-  FT_TRY(make_map3(ctx, &g_out, pl.grad, false, pl.piece, pl.Tp, pl.g_planes, pl.piece, 64, 32));
-  if (t.grad_hidden) FT_TRY(make_map3(ctx, &acc_out, pl.acc, true, pl.acc_ld, pl.Tp, pl.splits, pl.acc_ld, 32, 32));
-  FT_TRY(make_map3(ctx, &h_mn, pl.h, false, H, pl.Tp, pl.h_planes, pl.h_ld, 64, 64));
+  CUtensorMap g_mn, h_mn, dw_out;
+  FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, vm ? 128 : pl.out_n / 2));
+  FT_TRY(mn_map(&h_mn, pl.h, H, pl.Tp, pl.h_planes, pl.h_ld));
   const bool dw16 = q.p.grad_weight_type == FT_TYPE_F16;
   const bool dw_tma = t.grad_weight && ((uintptr_t)t.grad_weight & 15) == 0 && pl.w_cols % (dw16 ? 8 : 4) == 0;
   if (dw_tma)
     FT_TRY(make_map3(ctx, &dw_out, t.grad_weight, !dw16, pl.w_cols, pl.w_rows, 1, pl.w_cols, 32, 32,
                      dw16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B));
+  tile(z, TILE, a_rows, !vm);
   for (int v0 = 0; v0 < V; v0 += pl.piece) {
     const int cols = std::min(pl.piece, V - v0);
     z.N = cols; z.v0 = v0; z.b_mn0 = v0;
@@ -834,18 +1147,11 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     else FT_TRY((launch_gemm<EPI_GRAD, false, true>(ctx, two, h_k, w_mn, g_out, z)));
     // as operands, the piece ends with the vocabulary: what lies behind reads as zero
     if (v0 == 0 || cols != pl.piece) {
-      FT_TRY(make_map3(ctx, &g_k, pl.grad, false, cols, pl.Tp, pl.g_planes, pl.piece, 64, 128));
-      FT_TRY(make_map3(ctx, &g_mn, pl.grad, false, cols, pl.Tp, pl.g_planes, pl.piece, 64, 64));
+      FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, 128));
+      FT_TRY(mn_map(&g_mn, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece));
     }
     if (t.grad_hidden) {
-      TcProduct p = {};
-      p.rw = pl.rows;
-      p.M = T; p.N = H; p.K = cols; p.live_m = 1;
-      p.splits = std::min(pl.splits, ft_cdiv(cols, BK));
-      p.n_fast = 1; p.band = 1;
-      set_terms(p, pl.g_planes, pl.w_planes);
-      p.k0 = v0; p.b_has_k0 = 1;
-      p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
+      const TcProduct p = dh_product(v0, cols);
       if (vm) FT_TRY((launch_gemm<EPI_STORE, false, true>(ctx, two, g_k, w_mn, acc_out, p)));
       else FT_TRY((launch_gemm<EPI_STORE, false, false>(ctx, two, g_k, w_k, acc_out, p)));
     }
@@ -863,17 +1169,16 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
         p.M = H; p.N = cols; p.out_x0 = v0;
         set_terms(p, pl.h_planes, pl.g_planes);
       }
+      tile(p, vm ? pl.out_n : TILE, 128, true);
       p.n_fast = p.M >= p.N; p.band = ft_cdiv(p.M, TILE);
       FT_TRY((launch_gemm<EPI_STORE, true, true>(ctx, two, vm ? g_mn : h_mn, vm ? h_mn : g_mn, dw_tma ? dw_out : g_mn, p)));
     }
   }
   if (t.grad_hidden) {
-    const size_t slab = (size_t)pl.Tp * pl.acc_ld;
-    const int grid = (int)std::min<long long>(ft_cdiv((long long)T * (pl.acc_ld / 4), 256), (long long)ctx->sm_count * 16);
     if (q.p.grad_hidden_type == FT_TYPE_F16)
-      FT_LAUNCH_PDL(ctx, k_ce_scatter<__half>, grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, H, T, (__half*)t.grad_hidden);
+      FT_LAUNCH_PDL(ctx, k_ce_scatter<__half>, unpack_grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, H, T, (__half*)t.grad_hidden);
     else
-      FT_LAUNCH_PDL(ctx, k_ce_scatter<float>, grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, H, T, (float*)t.grad_hidden);
+      FT_LAUNCH_PDL(ctx, k_ce_scatter<float>, unpack_grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, H, T, (float*)t.grad_hidden);
   }
   return FT_OK;
 }
