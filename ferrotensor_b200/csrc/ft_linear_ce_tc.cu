@@ -36,20 +36,26 @@ namespace {
 using namespace ft_tc;
 using namespace ft_ce;
 
-constexpr int TILE = 256;                 // rows and columns of a pair's tile
-constexpr int STAGES = 6;
+constexpr int TILE = 256;                 // rows (and most columns) of a pair's tile
 constexpr int OPERAND_BYTES = 128 * BK * 2;
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-constexpr int EPI_OFFSET = STAGES * STAGE_BYTES;      // 8 epilogue warps x 4 KiB
-constexpr int BAR_OFFSET = EPI_OFFSET + 8 * 4096;
-constexpr int BARRIERS = 2 * STAGES + 8;              // full, empty, tfull[2], tempty[2], one a quadrant
-constexpr int SMEM_BYTES = BAR_OFFSET + BARRIERS * 8 + 16 + 1024;
+constexpr int MAX_BUFFERS = 4;            // accumulators: two of 256 columns, four of 128
 
 // STATS: row statistics.  EXP: statistics and E.  GRAD: g.  STORE: the sum.  FACTOR: the sum with every
 // TILE of K scaled by its row's factor.
 enum Epi { EPI_STATS, EPI_EXP, EPI_GRAD, EPI_STORE, EPI_FACTOR };
+// Warps that drain: FACTOR's empty an accumulator for every 2048 cycles of the tensor cores, which eight
+// warps do not manage (4096 x 2048 x 24576: 345 us, 317 with sixteen, of 286 with no drain at all).
+constexpr int drain_warps(int epi) { return epi == EPI_FACTOR ? 16 : 8; }
 // The statistics' launches have two warps more, for the targets' logits.
-constexpr int threads_of(int epi) { return epi <= EPI_EXP ? GEMM_THREADS + 64 : GEMM_THREADS; }
+constexpr int threads_of(int epi) { return 64 + 32 * drain_warps(epi) + (epi <= EPI_EXP ? 64 : 0); }
+// Shared memory: the stages, 4 KiB for each draining warp, the barriers (full, empty, tfull, tempty, one a
+// quadrant), and room to align all that.
+constexpr int stages_of(int epi) { return epi == EPI_FACTOR ? 5 : 6; }
+constexpr int epi_offset(int epi) { return stages_of(epi) * STAGE_BYTES; }
+constexpr int bar_offset(int epi) { return epi_offset(epi) + drain_warps(epi) * 4096; }
+constexpr int barriers_of(int epi) { return 2 * stages_of(epi) + 2 * MAX_BUFFERS + 4; }
+constexpr int smem_bytes(int epi) { return bar_offset(epi) + barriers_of(epi) * 8 + 16 + 1024; }
 // k-blocks of 64 that are summed in tensor memory; 0: all
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
 
@@ -69,6 +75,7 @@ struct TcProduct {
   Rows rw;
   float2* part;                     // [2 * column tiles][part_ld]: {maximum in log2 units, sum}
   int part_ld;
+  int piece, pieces;                // STATS, EXP: which launch this is, of how many
   __half* wy;                       // EXP: the targets' columns of W, [planes][part_ld][wy_ld]
   int wy_ld;
   int v0, vocab;                    // first vocabulary column of the launch, columns in all
@@ -103,6 +110,11 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src,
                    (uint64_t)map),
                "r"(src), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
+}
+// Hands an accumulator back to the leader.  What has to be done before it are the warp's reads of tensor
+// memory, which tcgen05.wait::ld and the fence before have seen to; no memory is published.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // the staging tile may be written again: the copies have read it
@@ -149,50 +161,74 @@ __device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const
     *(uint4*)(st + lane * 128 + (((part * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
 }
 
-// h_row . W(:, target) on f32 FMA, one row a warp.  The tensor core's sums are cut off, not rounded (see
-// above): 4e-6 of a logit at K = 256, 4e-5 at 2048.  For most logits that is noise under the softmax,
-// but the loss of a row that is sure of its target is as exact, relative to itself, as that one
-// logit is exact in absolute terms.  [hidden, vocab] weights cost a 32-byte sector for every 2
-// bytes here; beside the products nobody waits for them.
-// KEEP: the column goes to wy as well, for the one-hot term of dh.
+// h_row . W(:, target) of the packed rows [r0, r1) on f32 FMA.  The tensor core's sums are cut off, not
+// rounded (see above): 4e-6 of a logit at K = 256, 4e-5 at 2048.  For most logits that is noise under
+// the softmax, but the loss of a row that is sure of its target is as exact, relative to itself, as
+// that one logit is exact in absolute terms.
+// A warp takes R rows with 32 / R lanes each, a lane 16 values of K at a time.  [hidden, vocab] weights
+// cost a 32-byte sector for every 2 bytes; with many rows (R = 32) all warps walk down K together,
+// so that DRAM reads a row of W once for all targets in it (with a row a warp, 4096 rows x 2048
+// read 540 MB for 100 MB of W and the products waited for them: 390 against 277 us).
+// KEEP: the columns go to wy as well, for the one-hot term of dh.
 template <bool KEEP>
-__device__ __forceinline__ float target_dot(const TcProduct& g, int row, uint32_t target, int lane) {
-  constexpr int AT_ONCE = 16;   // loads in flight before the first use (and before a store that might alias them)
-  float acc = 0.f;
-  for (int pw = 0; pw < g.w_planes; ++pw) {
-    const __half* h = g.h + (long long)row * g.h_ld;
-    const __half* w = g.w + pw * g.w_plane + (long long)target * g.w_sv;
-    __half* keep = KEEP ? g.wy + ((long long)pw * g.part_ld + row) * g.wy_ld : nullptr;
-    for (int k0 = lane; k0 < g.K; k0 += 32 * AT_ONCE) {
-      __half b[AT_ONCE];
-      float a[AT_ONCE];
+__device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, int worker, int workers, float c2, int lane) {
+  const int rows = r1 - r0;
+  int R = 1;
+  if (g.w_sk != 1)
+    while (R < 32 && rows > R * workers) R *= 2;
+  const int share = 32 / R, sub = lane % share;
+  for (int base = r0 + worker * R; base < r1; base += workers * R) {
+    const int r = base + lane / share;
+    const uint32_t y = r < r1 ? g.rw.target[r] : FT_MASKED_CE_SKIP;
+    const bool on = y < (uint32_t)g.vocab;
+    float acc = 0.f;
+    for (int pw = 0; pw < g.w_planes && on; ++pw) {
+      const __half* h = g.h + (long long)r * g.h_ld;
+      const __half* w = g.w + pw * g.w_plane + (long long)y * g.w_sv;
+      __half* keep = KEEP ? g.wy + ((long long)pw * g.part_ld + r) * g.wy_ld : nullptr;
+      // (pitches of h and wy are multiples of 8, and so is W's where K is the contiguous index)
+      for (int k0 = sub * 16; k0 < g.h_ld; k0 += share * 16) {
+        uint4 hv[2], lv[2], wv[2];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int k = k0 + 32 * j;
-        b[j] = k < g.K ? w[k * g.w_sk] : __float2half(0.f);
-        a[j] = k < g.K ? __half2float(h[k]) : 0.f;
-      }
-      if (g.h_planes == 2) {
+        for (int j = 0; j < 2; ++j) {
+          const int k = k0 + 8 * j;
+          hv[j] = lv[j] = wv[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (k >= g.h_ld) continue;
+          hv[j] = *(const uint4*)(h + k);
+          if (g.h_planes == 2) lv[j] = *(const uint4*)(h + g.h_plane + k);
+          if (g.w_sk == 1) {
+            wv[j] = *(const uint4*)(w + k);
+          } else {
+            __half e[8];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j)
-          if (k0 + 32 * j < g.K) a[j] += __half2float(h[g.h_plane + k0 + 32 * j]);
-      }
+            for (int i = 0; i < 8; ++i) e[i] = k + i < g.K ? w[(k + i) * g.w_sk] : __float2half(0.f);
+            wv[j] = *(const uint4*)e;
+          }
+        }
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        acc = fmaf(a[j], __half2float(b[j]), acc);
-        if (KEEP && k0 + 32 * j < g.K) keep[k0 + 32 * j] = b[j];
+        for (int j = 0; j < 2; ++j) {
+          const __half2 *a = (const __half2*)&hv[j], *l = (const __half2*)&lv[j], *b = (const __half2*)&wv[j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 x = __half22float2(a[i]), z = __half22float2(l[i]), f = __half22float2(b[i]);
+            acc = fmaf(x.x + z.x, f.x, acc);
+            acc = fmaf(x.y + z.y, f.y, acc);
+          }
+          if (KEEP && k0 + 8 * j < g.h_ld) *(uint4*)(keep + k0 + 8 * j) = wv[j];
+        }
       }
     }
+    for (int o = share / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (sub == 0 && on) g.rw.exact[r] = acc * c2;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  return acc;
 }
 
 template <int EPI, bool A_MN, bool B_MN, bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
+  constexpr int STAGES = stages_of(EPI), WARPS = drain_warps(EPI), EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI);
+  constexpr int CHUNKS = 32 / WARPS;        // of 32 columns, at most, a draining warp
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -200,9 +236,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const uint32_t bar_full = base + BAR_OFFSET;
   const uint32_t bar_empty = bar_full + STAGES * 8;
   const uint32_t bar_tfull = bar_empty + STAGES * 8;
-  const uint32_t bar_tempty = bar_tfull + 2 * 8;
-  const uint32_t bar_quad = bar_tempty + 2 * 8;
-  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + BARRIERS * 8);
+  const uint32_t bar_tempty = bar_tfull + MAX_BUFFERS * 8;
+  const uint32_t bar_quad = bar_tempty + MAX_BUFFERS * 8;
+  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + barriers_of(EPI) * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -214,9 +250,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       mbar_init(bar_full + s * 8, 1);
       mbar_init(bar_empty + s * 8, 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < MAX_BUFFERS; ++b) {
       mbar_init(bar_tfull + b * 8, 1);
-      mbar_init(bar_tempty + b * 8, 16);
+      mbar_init(bar_tempty + b * 8, 2 * WARPS);
     }
     for (int b = 0; b < 4; ++b) mbar_init(bar_quad + b * 8, 2);   // the two warps of a quadrant
     *abort_flag = 0;
@@ -242,6 +278,8 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const int tiles_m = g.live_m ? max(1, (live + TILE - 1) / TILE) : (g.M + TILE - 1) / TILE;
   const int tile_n = EPI == EPI_EXP || EPI == EPI_GRAD ? TILE : g.tile_n;
   const int tiles_n = (g.N + tile_n - 1) / tile_n;
+  // accumulators in tensor memory, in turn
+  const uint32_t buffers = tile_n <= 128 ? 4 : 2, buffer_cols = 512 / buffers;
   const int units = tiles_m * tiles_n * g.splits;
   const int kb_all = g.live_k ? max(1, (live + BK - 1) / BK) : (g.K + BK - 1) / BK;
   constexpr int SLICE = slice_of(EPI, TWO);
@@ -300,10 +338,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
         for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice, ++local) {
           const int todo = (min(kb1, s0 + slice) - s0) * g.terms;
-          const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+          const uint32_t buf = (uint32_t)local & (buffers - 1), acc_phase = ((uint32_t)local / buffers) & 1;
           if (!mbar_wait(bar_tempty + buf * 8, acc_phase ^ 1, abort_flag, status, 22)) break;
           tc_fence_after();
-          const uint32_t d_tmem = tmem_base + buf * TILE;
+          const uint32_t d_tmem = tmem_base + buf * buffer_cols;
           for (int i = 0; i < todo; ++i) {
             if (!mbar_wait(bar_full + stage * 8, phase, abort_flag, status, 23)) break;
             tc_fence_after();
@@ -323,24 +361,21 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
     }
     __syncwarp();
-  } else if (EPI <= EPI_EXP && warp >= GEMM_THREADS / 32) {
+  } else if (EPI <= EPI_EXP && warp >= 2 + WARPS) {
     // ------------------------------------------------------------------ the targets' logits
     const float c2 = g.rw.head->z_scale * 1.4426950408889634f;
-    for (int r = (int)blockIdx.x * 2 + warp - GEMM_THREADS / 32; r < live; r += (int)gridDim.x * 2) {
-      const uint32_t y = g.rw.target[r];
-      if (y - (uint32_t)g.v0 >= (uint32_t)g.N) continue;           // in this launch's columns?
-      const float z = target_dot<EPI == EPI_EXP>(g, r, y, lane);
-      if (lane == 0) g.rw.exact[r] = z * c2;
-    }
+    // each launch of a vocabulary in pieces takes its share of the rows
+    const int r0 = (int)((long long)live * g.piece / g.pieces), r1 = (int)((long long)live * (g.piece + 1) / g.pieces);
+    target_dots<EPI == EPI_EXP>(g, r0, r1, (int)blockIdx.x * 2 + warp - 2 - WARPS, (int)gridDim.x * 2, c2, lane);
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
-    // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the two warps of a quadrant take half of
-    // the columns each, in up to four chunks of 32.
+    // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the warps of a quadrant share the
+    // columns, in chunks of 32.
     const int quad = warp & 3, grp = (warp - 2) >> 2;
-    const int half = (tile_n / 32 + 1) / 2, mine = grp ? tile_n / 32 - half : half;
+    const int share = (tile_n / 32 + WARPS / 4 - 1) / (WARPS / 4), mine = max(0, min(share, tile_n / 32 - grp * share));
     uint8_t* st = gbase + EPI_OFFSET + (warp - 2) * 4096;
     const uint32_t st_addr = smem_u32(st);
-    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * half * 32;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * share * 32;
     const float c2 = g.rw.head->z_scale * 1.4426950408889634f;     // accumulator -> logit in log2 units
     // rows that a store may reach: all of a tile where the rows are packed ones (their buffers end with
     // a tile), else those of the output
@@ -352,7 +387,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
       const int y0 = un.mt * TILE + (int)rank * 128 + quad * 32;   // first row of this warp
       const int row = y0 + lane;
-      const int col = un.nt * tile_n + grp * half * 32;            // its first column, from the launch's first
+      const int col = un.nt * tile_n + grp * share * 32;            // its first column, from the launch's first
       uint32_t target = FT_MASKED_CE_SKIP;
       float lse2 = 0.f, wg = 0.f, alpha = 1.f, base2 = 0.f;
       if constexpr (EPI <= EPI_GRAD) {
@@ -534,33 +569,54 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       auto release = [&](uint32_t buf) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(lead_tempty + buf * 8);
+        if (lane == 0) mbar_arrive_remote(lead_tempty + buf * 8);
       };
 
       if constexpr (SLICE > 0) {
-        float acc[4][32];
+        float acc[CHUNKS][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < CHUNKS; ++i)
 #pragma unroll
           for (int k = 0; k < 32; ++k) acc[i][k] = 0.f;
+        float* factors = (float*)st;                                  // FACTOR: of the next 32 slices, [slice][row]
+        if constexpr (EPI == EPI_FACTOR) {
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+        }
         for (int s0 = kb0; s0 < kb1; s0 += slice, ++local) {
-          const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+          const uint32_t buf = (uint32_t)local & (buffers - 1), acc_phase = ((uint32_t)local / buffers) & 1;
           float f = 1.f;
           if constexpr (EPI == EPI_FACTOR) {
-            // (a difference of two infinities belongs to a row of NaN anyway)
-            if (row < live) f = ex2(finite_max(g.part[(size_t)(2 * (s0 / SLICE)) * g.part_ld + row].x) - base2);
+            const int at = ((s0 - kb0) / SLICE) & 31;
+            if (at == 0) {
+              // 32 slices' at once: a load from memory in every slice, even one asked for a slice
+              // ahead, kept each at 3900 cycles (390 us for the product above)
+#pragma unroll 4
+              for (int j = 0; j < 32 && s0 + SLICE * j < kb1; ++j) {
+                const float m = row < live ? g.part[(size_t)(2 * (s0 / SLICE + j)) * g.part_ld + row].x : 0.f;
+                // (a difference of two infinities belongs to a row of NaN anyway)
+                factors[j * 32 + lane] = ex2(finite_max(m) - base2);
+              }
+            }
+            f = factors[at * 32 + lane];
           }
           if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
           tc_fence_after();
+          // 16 columns at a time
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i >= mine) continue;
-            uint32_t r[32];
-            tc_ld32(t_lane + buf * TILE + i * 32, r);
+          for (int i = 0; i < 2 * CHUNKS; ++i) {
+            if (i >= 2 * mine) continue;
+            uint32_t r[16];
+            tc_ld16(t_lane + buf * buffer_cols + i * 16, r);
             tc_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              acc[i][k] = EPI == EPI_FACTOR ? fmaf(f, __uint_as_float(r[k]), acc[i][k]) : acc[i][k] + __uint_as_float(r[k]);
+            for (int k = 0; k < 16; k += 2) {
+              float& a0 = acc[i >> 1][(i & 1) * 16 + k];
+              float& a1 = acc[i >> 1][(i & 1) * 16 + k + 1];
+              const float x0 = __uint_as_float(r[k]), x1 = __uint_as_float(r[k + 1]);
+              if constexpr (EPI == EPI_FACTOR) ffma2(a0, a1, f, f, x0, x1, a0, a1);
+              else fadd2(a0, a1, a0, a1, x0, x1);
+            }
           }
           release(buf);
         }
@@ -568,26 +624,26 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if constexpr (EPI == EPI_EXP) {
           float m = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < CHUNKS; ++i) {
             mask_columns(col + 32 * i, acc[i]);
             m = fmaxf(m, max_of(acc[i]));
           }
           run_m = join_max(m * c2);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < CHUNKS; ++i)
           if (i < mine) finish(i, acc[i]);
       } else {
-        const uint32_t buf = local & 1, acc_phase = (local >> 1) & 1;
+        const uint32_t buf = (uint32_t)local & (buffers - 1), acc_phase = ((uint32_t)local / buffers) & 1;
         ++local;
         if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
         tc_fence_after();
         if constexpr (EPI == EPI_EXP) {
           float m = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < CHUNKS; ++i) {
             float v[32];
-            tc_ld32(t_lane + buf * TILE + i * 32, *(uint32_t(*)[32])v);
+            tc_ld32(t_lane + buf * buffer_cols + i * 32, *(uint32_t(*)[32])v);
             tc_wait_ld();
             mask_columns(col + 32 * i, v);
             m = fmaxf(m, max_of(v));
@@ -596,10 +652,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         if (mine == 0) release(buf);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < CHUNKS; ++i) {
           if (i >= mine) continue;
           float v[32];
-          tc_ld32(t_lane + buf * TILE + i * 32, *(uint32_t(*)[32])v);
+          tc_ld32(t_lane + buf * buffer_cols + i * 32, *(uint32_t(*)[32])v);
           tc_wait_ld();
           if (i == mine - 1) release(buf);                         // all chunks have been read
           finish(i, v);
@@ -886,11 +942,11 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   static bool ready[FT_MAX_DEVICES] = {};
   static int most[FT_MAX_DEVICES] = {};
   if (!ready[ctx->device]) {
-    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(EPI)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctx->sm_count & ~1));
     cfg.blockDim = dim3(threads_of(EPI));
-    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.dynamicSmemBytes = smem_bytes(EPI);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
@@ -906,7 +962,7 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
                                 A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
-  cudaError_t e = ft_launch_ex(ctx, kernel, 2 * pairs, threads_of(EPI), SMEM_BYTES, a, b, o, g, ctx->status_dev);
+  cudaError_t e = ft_launch_ex(ctx, kernel, 2 * pairs, threads_of(EPI), smem_bytes(EPI), a, b, o, g, ctx->status_dev);
   if (ctx->profile_all) ft_prof_end(ctx);
   ctx->launches++;
   if (e == cudaSuccess) e = cudaPeekAtLastError();
@@ -1071,6 +1127,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   z.w = (const __half*)w; z.w_plane = (long long)pl.w_rows * pl.w_ld; z.w_planes = pl.w_planes;
   z.w_sk = vm ? 1 : pl.w_ld; z.w_sv = vm ? pl.w_ld : 1;
   z.wy = pl.wy; z.wy_ld = pl.h_ld;
+  z.pieces = pl.by_exp ? ft_cdiv(V, pl.piece) : 1;
   const size_t slab = (size_t)pl.Tp * pl.acc_ld;
   const int join_grid = ft_cdiv(T, 32);
   CUtensorMap acc_out;
@@ -1101,7 +1158,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
       const int cols = std::min(pl.piece, V - v0);
       const bool first = v0 == 0, last = v0 + cols == V;
-      z.N = cols; z.v0 = v0; z.b_mn0 = v0;
+      z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       if (vm) FT_TRY((launch_gemm<EPI_EXP, false, false>(ctx, two, h_k, w_k, g_out, z)));
       else FT_TRY((launch_gemm<EPI_EXP, false, true>(ctx, two, h_k, w_mn, g_out, z)));
       FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(cols, TILE), pl.rows, first ? 1 : 0,
