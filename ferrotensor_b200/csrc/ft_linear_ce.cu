@@ -93,11 +93,21 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
   const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(rw.head->h_amax, OPERAND_EXP) : 1.f;
   int before = 0, all = 0;
   float big = 0.f;
-  for (int i = tid; i < rows; i += GATHER_THREADS) {
-    if (targets[i] == FT_MASKED_CE_SKIP) continue;
-    ++all;
-    if (i < r0) ++before;
-    if (weights) big = fmaxf(big, fabsf(weights[i] * grad_scale));
+  {
+    auto count = [&](int i, uint32_t y) {
+      const int one = y != FT_MASKED_CE_SKIP;
+      all += one;
+      before += i < r0 ? one : 0;
+    };
+    const int vec = (((uintptr_t)targets) & 15) == 0 ? rows / 4 : 0;
+    for (int i = tid; i < vec; i += GATHER_THREADS) {
+      const uint4 y = ((const uint4*)targets)[i];
+      count(4 * i, y.x); count(4 * i + 1, y.y); count(4 * i + 2, y.z); count(4 * i + 3, y.w);
+    }
+    for (int i = 4 * vec + tid; i < rows; i += GATHER_THREADS) count(i, targets[i]);
+    if (blockIdx.x == 0 && weights)
+      for (int i = tid; i < rows; i += GATHER_THREADS)
+        if (targets[i] != FT_MASKED_CE_SKIP) big = fmaxf(big, fabsf(weights[i] * grad_scale));
   }
   before = block_sum_int(before, red);
   all = block_sum_int(all, red);

@@ -49,12 +49,13 @@ enum Epi { EPI_STATS, EPI_EXP, EPI_GRAD, EPI_STORE, EPI_FACTOR };
 constexpr int drain_warps(int epi) { return epi == EPI_FACTOR ? 16 : 8; }
 // The statistics' launches have two warps more, for the targets' logits.
 constexpr int threads_of(int epi) { return 64 + 32 * drain_warps(epi) + (epi <= EPI_EXP ? 64 : 0); }
-// Shared memory: the stages, 4 KiB for each draining warp, the barriers (full, empty, tfull, tempty, one a
-// quadrant), and room to align all that.
-constexpr int stages_of(int epi) { return epi == EPI_FACTOR ? 5 : 6; }
-constexpr int epi_offset(int epi) { return stages_of(epi) * STAGE_BYTES; }
+// Shared memory: the stages (six, or five, of 32 KiB; more where few rows or narrow tiles make them
+// smaller), 4 KiB for each draining warp, the barriers (full, empty, tfull, tempty, one a quadrant),
+// and room to align all that.
+constexpr int MAX_STAGES = 16;
+constexpr int epi_offset(int epi) { return (epi == EPI_FACTOR ? 5 : 6) * STAGE_BYTES; }
 constexpr int bar_offset(int epi) { return epi_offset(epi) + drain_warps(epi) * 4096; }
-constexpr int barriers_of(int epi) { return 2 * stages_of(epi) + 2 * MAX_BUFFERS + 4; }
+constexpr int barriers_of(int) { return 2 * MAX_STAGES + 2 * MAX_BUFFERS + 4; }
 constexpr int smem_bytes(int epi) { return bar_offset(epi) + barriers_of(epi) * 8 + 16 + 1024; }
 // k-blocks of 64 that are summed in tensor memory; 0: all
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
@@ -62,11 +63,14 @@ constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK
 struct TcProduct {
   int M, N, K;
   int live_m, live_k;               // 1: that extent is the number of supervised rows
+  int unpacked;                     // STATS: the rows are the caller's own, all M of them (no head, no scales)
+  int carry;                        // STATS: one tile of rows; a pair joins its column tiles before it writes them
   int splits;                       // parts of K, each with a slab of its own
   int tile_n;                       // columns of a tile: a multiple of 32 up to TILE
   int n_fast, band;                 // order of the tiles
   int a_second;                     // whether the odd CTA's rows are loaded (not: at most 128 rows, nobody reads them)
-  int stage_tx;                     // bytes of a stage, both CTAs
+  int a_bytes, stage_bytes;         // of A in a stage, of a stage (multiples of 1024)
+  int stage_tx;                     // what both CTAs load into one
   int terms;                        // plane pairs, the small ones first
   int a_plane[3], b_plane[3];
   int a_mn0, b_mn0, k0;             // where M, N and K begin in the operands' tensors...
@@ -75,6 +79,7 @@ struct TcProduct {
   Rows rw;
   float2* part;                     // [2 * column tiles][part_ld]: {maximum in log2 units, sum}
   int part_ld;
+  int w_early;                      // STATS: W may be read before the launch before this one has ended
   int piece, pieces;                // STATS, EXP: which launch this is, of how many
   __half* wy;                       // EXP: the targets' columns of W, [planes][part_ld][wy_ld]
   int wy_ld;
@@ -99,6 +104,10 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
       "{%3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
+}
+__device__ __forceinline__ void l2_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"((uint64_t)map),
@@ -227,15 +236,15 @@ template <int EPI, bool A_MN, bool B_MN, bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
-  constexpr int STAGES = stages_of(EPI), WARPS = drain_warps(EPI), EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI);
+  constexpr int WARPS = drain_warps(EPI), EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI);
   constexpr int CHUNKS = 32 / WARPS;        // of 32 columns, at most, a draining warp
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   const uint32_t bar_full = base + BAR_OFFSET;
-  const uint32_t bar_empty = bar_full + STAGES * 8;
-  const uint32_t bar_tfull = bar_empty + STAGES * 8;
+  const uint32_t bar_empty = bar_full + MAX_STAGES * 8;
+  const uint32_t bar_tfull = bar_empty + MAX_STAGES * 8;
   const uint32_t bar_tempty = bar_tfull + MAX_BUFFERS * 8;
   const uint32_t bar_quad = bar_tempty + MAX_BUFFERS * 8;
   uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + barriers_of(EPI) * 8);
@@ -246,7 +255,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < MAX_STAGES; ++s) {
       mbar_init(bar_full + s * 8, 1);
       mbar_init(bar_empty + s * 8, 1);
     }
@@ -268,12 +277,23 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  const uint32_t stages = (uint32_t)min(MAX_STAGES, EPI_OFFSET / g.stage_bytes);
+  if (EPI == EPI_STATS && g.w_early && warp == 0 && elect_one()) {
+    // W is the caller's and older than the launch before this one: its first tile may be on its way
+    // into L2 while that packs the rows
+    const int first = pair / ((g.M + TILE - 1) / TILE);
+    for (int k = 0; k < g.K && first * g.tile_n < g.N; k += BK) {
+      if (B_MN) l2_prefetch_3d(&map_b, first * g.tile_n + (int)rank * (g.tile_n / 2), k, 0);
+      else l2_prefetch_3d(&map_b, k, first * g.tile_n + (int)rank * (g.tile_n / 2), 0);
+    }
+  }
   ft_pdl_wait();
   ft_pdl_launch();
 
   const uint32_t lead_full = mapa_shared(bar_full, 0);
   const uint32_t lead_tempty = mapa_shared(bar_tempty, 0);
-  const int live = g.rw.head->count;
+  const bool unpacked = EPI == EPI_STATS && g.unpacked;
+  const int live = unpacked ? g.M : g.rw.head->count;
   // no supervised row at all still makes one tile (of zeros): gradients are overwritten, not left
   const int tiles_m = g.live_m ? max(1, (live + TILE - 1) / TILE) : (g.M + TILE - 1) / TILE;
   const int tile_n = EPI == EPI_EXP || EPI == EPI_GRAD ? TILE : g.tile_n;
@@ -304,7 +324,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const int pa = g.a_plane[t], pb = g.b_plane[t];
             for (int kb = s0; kb < s1; ++kb) {
               if (!mbar_wait(bar_empty + stage * 8, phase ^ 1, abort_flag, status, 21)) break;
-              const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OPERAND_BYTES;
+              const uint32_t sa = base + stage * g.stage_bytes, sb = sa + g.a_bytes;
               const uint32_t bar = lead_full + stage * 8;
               if (rank == 0) mbar_expect_tx(bar_full + stage * 8, (uint32_t)g.stage_tx);
               if (rank != 0 && !g.a_second) {
@@ -320,7 +340,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               } else {
                 tma_load_3d_pair(sb, &map_b, bar, bk0 + kb * BK, bn, pb);
               }
-              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+              if (++stage == stages) { stage = 0; phase ^= 1; }
             }
           }
         }
@@ -345,7 +365,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           for (int i = 0; i < todo; ++i) {
             if (!mbar_wait(bar_full + stage * 8, phase, abort_flag, status, 23)) break;
             tc_fence_after();
-            const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OPERAND_BYTES;
+            const uint32_t sa = base + stage * g.stage_bytes, sb = sa + g.a_bytes;
             const uint64_t da = A_MN ? make_desc_mn_sw128(sa, 8192) : make_desc_sw128(sa);
             const uint64_t db = B_MN ? make_desc_mn_sw128(sb, 8192) : make_desc_sw128(sb);
 #pragma unroll
@@ -353,7 +373,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               tc_mma_f16_pair(d_tmem, da + (uint64_t)(k * (A_MN ? 128 : 2)), db + (uint64_t)(k * (B_MN ? 128 : 2)), idesc,
                               (i > 0 || k > 0) ? 1u : 0u);
             tc_commit_pair(bar_empty + stage * 8, 3);
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            if (++stage == stages) { stage = 0; phase ^= 1; }
           }
           if (*abort_flag) break;
           tc_commit_pair(bar_tfull + buf * 8, 3);
@@ -363,7 +383,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     __syncwarp();
   } else if (EPI <= EPI_EXP && warp >= 2 + WARPS) {
     // ------------------------------------------------------------------ the targets' logits
-    const float c2 = g.rw.head->z_scale * 1.4426950408889634f;
+    const float c2 = (unpacked ? 1.f : g.rw.head->z_scale) * 1.4426950408889634f;
     // each launch of a vocabulary in pieces takes its share of the rows
     const int r0 = (int)((long long)live * g.piece / g.pieces), r1 = (int)((long long)live * (g.piece + 1) / g.pieces);
     target_dots<EPI == EPI_EXP>(g, r0, r1, (int)blockIdx.x * 2 + warp - 2 - WARPS, (int)gridDim.x * 2, c2, lane);
@@ -376,12 +396,12 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     uint8_t* st = gbase + EPI_OFFSET + (warp - 2) * 4096;
     const uint32_t st_addr = smem_u32(st);
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * share * 32;
-    const float c2 = g.rw.head->z_scale * 1.4426950408889634f;     // accumulator -> logit in log2 units
-    // rows that a store may reach: all of a tile where the rows are packed ones (their buffers end with
-    // a tile), else those of the output
-    const int rows_end = g.live_m ? tiles_m * TILE : g.M;
+    const float c2 = (unpacked ? 1.f : g.rw.head->z_scale) * 1.4426950408889634f;   // accumulator -> logit in log2 units
+    // rows that a store may reach (packed ones: whole warps of them, their buffers end with a tile)
+    const int rows_end = g.live_m ? live : g.M;
     int local = 0;
     uint32_t quad_phase = 0;
+    float run_m = -INFINITY, run_s = 0.f;
     for (int u = pair; u < units && !*abort_flag; u += npairs) {
       const Unit un = decode_unit(u, tiles_m, tiles_n, g);
       const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
@@ -403,7 +423,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       } else {
         if (row < live) base2 = g.rw.base[row];
       }
-      float run_m = -INFINITY, run_s = 0.f;
+      // a warp without a supervised row hands the accumulators back as they come (g's rows behind the
+      // last one are zeros that dW reads)
+      const bool idle = (EPI <= EPI_EXP || EPI == EPI_FACTOR) && y0 >= live;
+      if (EPI != EPI_STATS || !g.carry || u == pair) { run_m = -INFINITY; run_s = 0.f; }
       uint32_t low[TWO && (EPI == EPI_EXP || EPI == EPI_GRAD) ? 2 : 1][16];   // the second plane, until its store
 
       auto mask_columns = [&](int c0, float (&v)[32]) {
@@ -588,7 +611,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           float f = 1.f;
           if constexpr (EPI == EPI_FACTOR) {
             const int at = ((s0 - kb0) / SLICE) & 31;
-            if (at == 0) {
+            if (at == 0 && !idle) {
               // 32 slices' at once: a load from memory in every slice, even one asked for a slice
               // ahead, kept each at 3900 cycles (390 us for the product above)
 #pragma unroll 4
@@ -602,6 +625,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
           if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
           tc_fence_after();
+          if (idle) {
+            release(buf);
+            continue;
+          }
           // 16 columns at a time
 #pragma unroll
           for (int i = 0; i < 2 * CHUNKS; ++i) {
@@ -621,6 +648,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           release(buf);
         }
         if (*abort_flag) break;
+        if (idle) continue;
         if constexpr (EPI == EPI_EXP) {
           float m = -INFINITY;
 #pragma unroll
@@ -638,6 +666,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         ++local;
         if (!mbar_wait(bar_tfull + buf * 8, acc_phase, abort_flag, status, 24)) break;
         tc_fence_after();
+        if (idle) {
+          release(buf);
+          continue;
+        }
         if constexpr (EPI == EPI_EXP) {
           float m = -INFINITY;
 #pragma unroll
@@ -661,7 +693,13 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           finish(i, v);
         }
       }
-      if constexpr (EPI <= EPI_EXP) g.part[(size_t)(un.nt * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+      if constexpr (EPI <= EPI_EXP) {
+        if (EPI != EPI_STATS || !g.carry) g.part[(size_t)(un.nt * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+      }
+    }
+    if (EPI == EPI_STATS && g.carry) {
+      const int row = (int)rank * 128 + quad * 32 + lane;
+      g.part[(size_t)(pair * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
     }
     // what was stored is complete before the launch ends
     if (lane == 0) bulk_wait_all();
@@ -682,26 +720,26 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 }
 
 // ------------------------------------------------------------------------------ around the products
-// Joins the column tiles' {maximum, sum} of 32 rows, tiles over 16 warps in a fixed order, with what
+// Joins the column tiles' {maximum, sum} of 32 rows, tiles over 32 warps in a fixed order, with what
 // the pieces before (not `first`) have left; after the last piece writes the row's log-sum-exp (in
 // log2 units, as the gradient's epilogue wants it) and its loss.
 // With `acc` (E is in use): sets the point R that the row's E W is scaled against.  It stays the maximum
 // of the first piece, and f32 carries what later pieces are above it, unless that is 2^64 or
 // more: then it moves, and the row's sums so far are scaled down.
-constexpr int LOSS_WARPS = 16;
+constexpr int LOSS_WARPS = 32;
 __global__ void __launch_bounds__(32 * LOSS_WARPS)
-k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int first, int last, int vocab,
-          float* __restrict__ row_loss, float* __restrict__ acc, size_t slab, int splits, int ld, int H) {
+k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int unpacked_rows, int first, int last,
+          int vocab, float* __restrict__ row_loss, float* __restrict__ acc, size_t slab, int splits, int ld, int H) {
   __shared__ float2 red[LOSS_WARPS][32];
   __shared__ float shrink[32];
   ft_pdl_wait();
   ft_pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
-  const int live = rw.head->count;
+  const int live = unpacked_rows ? unpacked_rows : rw.head->count;
   if ((int)blockIdx.x * 32 >= live) return;
   float m = -INFINITY, s = 0.f;
-  constexpr int AT_ONCE = 8;
+  constexpr int AT_ONCE = 16;
   for (int p0 = warp; p0 < parts; p0 += AT_ONCE * LOSS_WARPS) {
     float2 v[AT_ONCE];
 #pragma unroll
@@ -742,7 +780,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
       }
       if (last) {
         const float l2 = log2f(S);
-        rw.lse[row] = ref + l2;
+        if (!unpacked_rows) rw.lse[row] = ref + l2;
         float loss = 0.f;
         if (rw.target[row] < (uint32_t)vocab) {
           // the sum with the target's logit z replaced by its exact value z + d:
@@ -752,7 +790,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
           const float d = (rw.exact[row] - z) * 0.6931471805599453f;
           loss = above - d + log1pf(expf(-above) * expm1f(d));
         }
-        row_loss[rw.source[row]] = loss;
+        row_loss[unpacked_rows ? row : rw.source[row]] = loss;
         if (acc) {
           // the gradient at the target, p - 1, is -(1 - e^-loss), exact for a row that is sure of its
           // target; what E W holds of it already goes off
@@ -937,7 +975,8 @@ int make_map3(FtContext* ctx, CUtensorMap* map, const void* ptr, bool f32, uint6
 }
 
 template <int EPI, bool A_MN, bool B_MN, bool TWO>
-int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g) {
+int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g,
+                int* pairs_used = nullptr) {
   auto kernel = k_ce_gemm<EPI, A_MN, B_MN, TWO>;
   static bool ready[FT_MAX_DEVICES] = {};
   static int most[FT_MAX_DEVICES] = {};
@@ -959,6 +998,7 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   }
   const long long units = (long long)ft_cdiv(g.M, TILE) * ft_cdiv(g.N, g.tile_n) * g.splits;
   const int pairs = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
+  if (pairs_used) *pairs_used = pairs;
   const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
                                 A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
@@ -971,8 +1011,10 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
 }
 
 template <int EPI, bool A_MN, bool B_MN>
-int launch_gemm(FtContext* ctx, bool split, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g) {
-  return split ? launch_gemm<EPI, A_MN, B_MN, true>(ctx, a, b, o, g) : launch_gemm<EPI, A_MN, B_MN, false>(ctx, a, b, o, g);
+int launch_gemm(FtContext* ctx, bool two, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g,
+                int* pairs_used = nullptr) {
+  return two ? launch_gemm<EPI, A_MN, B_MN, true>(ctx, a, b, o, g, pairs_used)
+             : launch_gemm<EPI, A_MN, B_MN, false>(ctx, a, b, o, g, pairs_used);
 }
 
 // plane pairs of a product, the smallest first: sums grow as late as they can
@@ -1085,7 +1127,11 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     FT_LAUNCH_PDL(ctx, k_ce_amax, wb + hb, 256, 0, (const float*)t.weight, (long long)pl.w_rows * pl.w_cols, wb,
                   (const float*)t.hidden, t.targets, T, H, pl.rows.head);
   }
-  FT_TRY(launch_gather_f16(ctx, q, t, pl.rows, pl.h, pl.h_ld, pl.Tp, pl.h_planes));
+  // One tile of rows, no gradient: packing would save nothing, and a row's statistics are its own
+  // whatever the others hold.
+  const bool unpacked = T <= 128 && !t.grad_hidden && !t.grad_weight && !h32 && !w32 && H % 8 == 0 &&
+                        ((uintptr_t)t.hidden & 15) == 0;
+  if (!unpacked) FT_TRY(launch_gather_f16(ctx, q, t, pl.rows, pl.h, pl.h_ld, pl.Tp, pl.h_planes));
   const void* w = t.weight;
   if (pl.w_staged) {
     w = pl.w;
@@ -1105,25 +1151,29 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   auto mn_map = [&](CUtensorMap* m, const void* p, int inner, int rows, int planes, int ld) {
     return make_map3(ctx, m, p, false, inner, rows, planes, ld, 64, 64);
   };
-  auto tile = [&](TcProduct& p, int tile_n, int a_rows, bool b_mn) {
+  auto tile = [&](TcProduct& p, int tile_n, int a_rows, bool second, bool b_mn) {
     p.tile_n = tile_n;
-    p.a_second = a_rows == 128;
-    p.stage_tx = (a_rows == 128 ? 2 : 1) * a_rows * 128 + 2 * (b_mn ? (tile_n > 128 ? 2 : 1) * 8192 : tile_n / 2 * 128);
+    p.a_second = second;
+    p.a_bytes = a_rows * 128;
+    const int b_bytes = b_mn ? (tile_n > 128 ? 2 : 1) * 8192 : tile_n / 2 * 128;
+    p.stage_bytes = p.a_bytes + b_bytes;
+    p.stage_tx = (second ? 2 : 1) * p.a_bytes + 2 * b_bytes;
   };
   // at most 128 rows: the even CTA's are all there are, and only as many are loaded
-  int a_rows = 128;
-  while (T <= 128 && a_rows > 8 && a_rows / 2 >= T) a_rows /= 2;
-  if (T > 64) a_rows = 128;
+  const bool second = T > 128;
+  const int a_rows = second ? 128 : (int)ft_align_up((size_t)T, 8);
   CUtensorMap h_k, w_k, w_mn;
-  FT_TRY(k_map(&h_k, pl.h, H, pl.Tp, pl.h_planes, pl.h_ld, a_rows));
-  FT_TRY(mn_map(&w_mn, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld));
+  FT_TRY(k_map(&h_k, unpacked ? t.hidden : pl.h, H, unpacked ? T : pl.Tp, pl.h_planes, pl.h_ld, a_rows));
+  if (!vm || t.grad_hidden) FT_TRY(mn_map(&w_mn, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld));
 
   TcProduct z = {};
   z.M = T; z.N = V; z.K = H; z.live_m = 1; z.splits = 1;
   z.band = 32;
   set_terms(z, pl.h_planes, pl.w_planes);
   z.rw = pl.rows; z.part = pl.part; z.part_ld = pl.Tp; z.vocab = V;
-  z.h = pl.h; z.h_ld = pl.h_ld; z.h_plane = (long long)pl.Tp * pl.h_ld; z.h_planes = pl.h_planes;
+  if (unpacked) z.rw.target = const_cast<uint32_t*>(t.targets);
+  z.unpacked = unpacked ? 1 : 0;
+  z.h = unpacked ? (const __half*)t.hidden : pl.h; z.h_ld = pl.h_ld; z.h_plane = (long long)pl.Tp * pl.h_ld; z.h_planes = pl.h_planes;
   z.w = (const __half*)w; z.w_plane = (long long)pl.w_rows * pl.w_ld; z.w_planes = pl.w_planes;
   z.w_sk = vm ? 1 : pl.w_ld; z.w_sv = vm ? pl.w_ld : 1;
   z.wy = pl.wy; z.wy_ld = pl.h_ld;
@@ -1148,20 +1198,20 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.k0 = v0; p.b_has_k0 = 1;
     p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
     p.part = pl.part; p.part_ld = pl.Tp;
-    tile(p, pl.out_n, 128, vm);
+    tile(p, pl.out_n, 128, true, vm);
     return p;
   };
 
   if (pl.by_exp) {
     FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, vm ? 128 : pl.out_n / 2));
-    tile(z, TILE, a_rows, !vm);
+    tile(z, TILE, a_rows, second, !vm);
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
       const int cols = std::min(pl.piece, V - v0);
       const bool first = v0 == 0, last = v0 + cols == V;
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       if (vm) FT_TRY((launch_gemm<EPI_EXP, false, false>(ctx, two, h_k, w_k, g_out, z)));
       else FT_TRY((launch_gemm<EPI_EXP, false, true>(ctx, two, h_k, w_mn, g_out, z)));
-      FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(cols, TILE), pl.rows, first ? 1 : 0,
+      FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(cols, TILE), pl.rows, 0, first ? 1 : 0,
                     last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
       if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, 128));
       const TcProduct p = dh_product(v0, cols);
@@ -1177,15 +1227,18 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     return FT_OK;
   }
 
-  tile(z, pl.stat_n, a_rows, !vm);
+  tile(z, pl.stat_n, a_rows, second, !vm);
+  z.w_early = !pl.w_staged;
+  z.carry = T <= TILE ? 1 : 0;
+  int pairs = 0;
   if (vm) {
     FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, pl.stat_n / 2));
-    FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z)));
+    FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z, &pairs)));
   } else {
-    FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z)));
+    FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z, &pairs)));
   }
-  FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(V, pl.stat_n), pl.rows, 1, 1, V,
-                t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
+  FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * (z.carry ? pairs : ft_cdiv(V, pl.stat_n)),
+                z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
   if (!t.grad_hidden && !t.grad_weight) return FT_OK;
 
   CUtensorMap g_mn, h_mn, dw_out;
@@ -1196,7 +1249,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   if (dw_tma)
     FT_TRY(make_map3(ctx, &dw_out, t.grad_weight, !dw16, pl.w_cols, pl.w_rows, 1, pl.w_cols, 32, 32,
                      dw16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B));
-  tile(z, TILE, a_rows, !vm);
+  tile(z, TILE, a_rows, second, !vm);
   for (int v0 = 0; v0 < V; v0 += pl.piece) {
     const int cols = std::min(pl.piece, V - v0);
     z.N = cols; z.v0 = v0; z.b_mn0 = v0;
@@ -1226,7 +1279,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
         p.M = H; p.N = cols; p.out_x0 = v0;
         set_terms(p, pl.h_planes, pl.g_planes);
       }
-      tile(p, vm ? pl.out_n : TILE, 128, true);
+      tile(p, vm ? pl.out_n : TILE, 128, true, true);
       p.n_fast = p.M >= p.N; p.band = ft_cdiv(p.M, TILE);
       FT_TRY((launch_gemm<EPI_STORE, true, true>(ctx, two, vm ? g_mn : h_mn, vm ? h_mn : g_mn, dw_tma ? dw_out : g_mn, p)));
     }

@@ -56,7 +56,8 @@ class CudaContext:
         handle = C.c_void_p()
         # torch's default stream is the legacy NULL stream: hand the library cudaStreamLegacy
         # (handle value 1) so that its kernels are ordered with torch's copies and NCCL calls
-        raw = self.stream.cuda_stream or 1
+        self._raw_stream = self.stream.cuda_stream
+        raw = self._raw_stream or 1
         call("ft_ctx_create", device, C.c_void_p(raw), C.byref(handle))
         self.handle = handle
         self.gemm_mode = GemmMode.F32
@@ -115,7 +116,7 @@ class CudaContext:
     def temporary(self, nbytes: int) -> torch.Tensor:
         """Device memory for one call: allocated on the context's stream, so that it may be released
         as soon as the call has been made, whatever stream is current."""
-        if torch.cuda.current_stream(self.device) == self.stream:
+        if torch._C._cuda_getCurrentRawStream(self.device.index) == self._raw_stream:
             return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         with torch.cuda.stream(self.stream):
             return torch.empty(nbytes, dtype=torch.uint8, device=self.device)

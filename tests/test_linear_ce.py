@@ -494,3 +494,19 @@ def test_logits_that_jump_between_pieces(cuda_ctx, eng, mode, order):
     for want in ("hidden", "both"):
         got = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, True, (F32, F32), want, piece)
         _check(got, q, _bounds(q, mode, (F16, F16), (F32, F32)), True, want)
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("vocab_major", [False, True])
+def test_losses_alone(cuda_ctx, eng, mode, vocab_major):
+    """No gradient: from one row to more than two tiles of rows, with everything skipped, odd widths, and a
+    vocabulary that ends inside a tile of any width."""
+    for i, (t, h, v) in enumerate([(1, 8, 9), (1, 576, 6001), (2, 40, 33), (31, 64, 20000), (64, 136, 3000), (65, 72, 777), (128, 64, 1024),
+                                   (129, 64, 1025), (256, 31, 4096), (257, 48, 900), (520, 24, 1500)]):
+        for types in ((F16, F16), (F32, F16), (F16, F32)):
+            x, w, y, a = _make(t, h, v, types, vocab_major, ("none", "beyond", "half", "all")[i % 4], 500 + i)
+            x[y == SKIP] = float("inf")
+            q = _truth(x, w, y, a, 1.0, vocab_major)
+            got = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, vocab_major, want="none")
+            _check(got, q, _bounds(q, mode, types, (F32, F32)), vocab_major, f"{(t, h, v)}")
