@@ -68,9 +68,8 @@ struct TcProduct {
   int splits;                       // parts of K, each with a slab of its own
   int tile_n;                       // columns of a tile: a multiple of 32 up to TILE
   int n_fast, band;                 // order of the tiles
-  int a_second;                     // whether the odd CTA's rows are loaded (not: at most 128 rows, nobody reads them)
   int a_bytes, stage_bytes;         // of A in a stage, of a stage (multiples of 1024)
-  int stage_tx;                     // what both CTAs load into one
+  int stage_tx;                     // what the tile's CTAs load into one
   int terms;                        // plane pairs, the small ones first
   int a_plane[3], b_plane[3];
   int a_mn0, b_mn0, k0;             // where M, N and K begin in the operands' tensors...
@@ -98,12 +97,18 @@ struct TcProduct {
   long long direct_ld;
 };
 
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t leader_bar, int c0,
-                                                 int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-      "{%3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, uint32_t leader_bar, int c0, int c1, int c2) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
 __device__ __forceinline__ void l2_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2)
@@ -133,6 +138,13 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// an arrival in every CTA of the tile once the products issued so far are complete
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (PAIR) tc_commit_pair(bar, 3);
+  else tc_commit(bar);
 }
 
 struct Unit { int mt, nt, sp; };
@@ -232,8 +244,8 @@ __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, 
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool TWO>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI), 1)
+template <bool PAIR, int EPI, bool A_MN, bool B_MN, bool TWO>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(threads_of(EPI), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
   constexpr int WARPS = drain_warps(EPI), EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI);
@@ -251,8 +263,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  constexpr int TM = PAIR ? 256 : 128;       // rows of a tile
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const int pair = PAIR ? blockIdx.x >> 1 : blockIdx.x, npairs = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < MAX_STAGES; ++s) {
@@ -261,41 +274,48 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
     for (int b = 0; b < MAX_BUFFERS; ++b) {
       mbar_init(bar_tfull + b * 8, 1);
-      mbar_init(bar_tempty + b * 8, 2 * WARPS);
+      mbar_init(bar_tempty + b * 8, (PAIR ? 2 : 1) * WARPS);
     }
     for (int b = 0; b < 4; ++b) mbar_init(bar_quad + b * 8, 2);   // the two warps of a quadrant
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if constexpr (PAIR) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t stages = (uint32_t)min(MAX_STAGES, EPI_OFFSET / g.stage_bytes);
   if (EPI == EPI_STATS && g.w_early && warp == 0 && elect_one()) {
     // W is the caller's and older than the launch before this one: its first tile may be on its way
     // into L2 while that packs the rows
-    const int first = pair / ((g.M + TILE - 1) / TILE);
-    for (int k = 0; k < g.K && first * g.tile_n < g.N; k += BK) {
-      if (B_MN) l2_prefetch_3d(&map_b, first * g.tile_n + (int)rank * (g.tile_n / 2), k, 0);
-      else l2_prefetch_3d(&map_b, k, first * g.tile_n + (int)rank * (g.tile_n / 2), 0);
+    const int first = pair / ((g.M + TM - 1) / TM);
+    const int bn = first * g.tile_n + (PAIR ? (int)rank * (g.tile_n / 2) : 0);
+    for (int k = 0; k < g.K && bn < g.N; k += BK) {
+      if (B_MN) l2_prefetch_3d(&map_b, bn, k, 0);
+      else l2_prefetch_3d(&map_b, k, bn, 0);
     }
   }
   ft_pdl_wait();
   ft_pdl_launch();
 
-  const uint32_t lead_full = mapa_shared(bar_full, 0);
-  const uint32_t lead_tempty = mapa_shared(bar_tempty, 0);
+  const uint32_t lead_full = PAIR ? mapa_shared(bar_full, 0) : bar_full;
+  const uint32_t lead_tempty = PAIR ? mapa_shared(bar_tempty, 0) : bar_tempty;
   const bool unpacked = EPI == EPI_STATS && g.unpacked;
   const int live = unpacked ? g.M : g.rw.head->count;
   // no supervised row at all still makes one tile (of zeros): gradients are overwritten, not left
-  const int tiles_m = g.live_m ? max(1, (live + TILE - 1) / TILE) : (g.M + TILE - 1) / TILE;
+  const int tiles_m = g.live_m ? max(1, (live + TM - 1) / TM) : (g.M + TM - 1) / TM;
   const int tile_n = EPI == EPI_EXP || EPI == EPI_GRAD ? TILE : g.tile_n;
   const int tiles_n = (g.N + tile_n - 1) / tile_n;
   // accumulators in tensor memory, in turn
@@ -317,7 +337,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       for (int u = pair; u < units && !*abort_flag; u += npairs) {
         const Unit un = decode_unit(u, tiles_m, tiles_n, g);
         const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
-        const int am = g.a_mn0 + un.mt * TILE + (int)rank * 128, bn = g.b_mn0 + un.nt * tile_n + (int)rank * (tile_n / 2);
+        const int am = g.a_mn0 + un.mt * TM + (int)rank * 128;
+        const int bn = g.b_mn0 + un.nt * tile_n + (PAIR ? (int)rank * (tile_n / 2) : 0);
+        const int b_cols = PAIR ? tile_n / 2 : tile_n;
         for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice) {
           const int s1 = min(kb1, s0 + slice);
           for (int t = 0; t < g.terms; ++t) {
@@ -327,18 +349,16 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               const uint32_t sa = base + stage * g.stage_bytes, sb = sa + g.a_bytes;
               const uint32_t bar = lead_full + stage * 8;
               if (rank == 0) mbar_expect_tx(bar_full + stage * 8, (uint32_t)g.stage_tx);
-              if (rank != 0 && !g.a_second) {
-              } else if constexpr (A_MN) {
-                tma_load_3d_pair(sa, &map_a, bar, am, ak0 + kb * BK, pa);
-                tma_load_3d_pair(sa + 8192, &map_a, bar, am + 64, ak0 + kb * BK, pa);
+              if constexpr (A_MN) {
+                load_3d<PAIR>(sa, &map_a, bar, am, ak0 + kb * BK, pa);
+                load_3d<PAIR>(sa + 8192, &map_a, bar, am + 64, ak0 + kb * BK, pa);
               } else {
-                tma_load_3d_pair(sa, &map_a, bar, ak0 + kb * BK, am, pa);
+                load_3d<PAIR>(sa, &map_a, bar, ak0 + kb * BK, am, pa);
               }
               if constexpr (B_MN) {
-                tma_load_3d_pair(sb, &map_b, bar, bn, bk0 + kb * BK, pb);
-                if (tile_n > 128) tma_load_3d_pair(sb + 8192, &map_b, bar, bn + 64, bk0 + kb * BK, pb);
+                for (int c = 0; c < b_cols; c += 64) load_3d<PAIR>(sb + c * 128, &map_b, bar, bn + c, bk0 + kb * BK, pb);
               } else {
-                tma_load_3d_pair(sb, &map_b, bar, bk0 + kb * BK, bn, pb);
+                load_3d<PAIR>(sb, &map_b, bar, bk0 + kb * BK, bn, pb);
               }
               if (++stage == stages) { stage = 0; phase ^= 1; }
             }
@@ -350,7 +370,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (leader only)
     if (rank == 0 && elect_one()) {
-      const uint32_t idesc = make_idesc(256, tile_n, 0, 0) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16);
+      const uint32_t idesc = make_idesc(TM, tile_n, 0, 0) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16);
       uint32_t stage = 0, phase = 0;
       int local = 0;
       for (int u = pair; u < units && !*abort_flag; u += npairs) {
@@ -369,14 +389,16 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const uint64_t da = A_MN ? make_desc_mn_sw128(sa, 8192) : make_desc_sw128(sa);
             const uint64_t db = B_MN ? make_desc_mn_sw128(sb, 8192) : make_desc_sw128(sb);
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k)
-              tc_mma_f16_pair(d_tmem, da + (uint64_t)(k * (A_MN ? 128 : 2)), db + (uint64_t)(k * (B_MN ? 128 : 2)), idesc,
-                              (i > 0 || k > 0) ? 1u : 0u);
-            tc_commit_pair(bar_empty + stage * 8, 3);
+            for (int k = 0; k < BK / UMMA_K; ++k) {
+              const uint64_t ka = da + (uint64_t)(k * (A_MN ? 128 : 2)), kb = db + (uint64_t)(k * (B_MN ? 128 : 2));
+              if constexpr (PAIR) tc_mma_f16_pair(d_tmem, ka, kb, idesc, (i > 0 || k > 0) ? 1u : 0u);
+              else tc_mma_f16(d_tmem, ka, kb, idesc, (i > 0 || k > 0) ? 1u : 0u);
+            }
+            commit<PAIR>(bar_empty + stage * 8);
             if (++stage == stages) { stage = 0; phase ^= 1; }
           }
           if (*abort_flag) break;
-          tc_commit_pair(bar_tfull + buf * 8, 3);
+          commit<PAIR>(bar_tfull + buf * 8);
         }
       }
     }
@@ -405,7 +427,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     for (int u = pair; u < units && !*abort_flag; u += npairs) {
       const Unit un = decode_unit(u, tiles_m, tiles_n, g);
       const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
-      const int y0 = un.mt * TILE + (int)rank * 128 + quad * 32;   // first row of this warp
+      const int y0 = un.mt * TM + (int)rank * 128 + quad * 32;   // first row of this warp
       const int row = y0 + lane;
       const int col = un.nt * tile_n + grp * share * 32;            // its first column, from the launch's first
       uint32_t target = FT_MASKED_CE_SKIP;
@@ -592,7 +614,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       auto release = [&](uint32_t buf) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(lead_tempty + buf * 8);
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_remote(lead_tempty + buf * 8);
+          else mbar_arrive(lead_tempty + buf * 8);
+        }
       };
 
       if constexpr (SLICE > 0) {
@@ -712,10 +737,11 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
     __syncthreads();
   }
-  cluster_sync_all();
+  if constexpr (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
   }
 }
 
@@ -974,35 +1000,36 @@ int make_map3(FtContext* ctx, CUtensorMap* map, const void* ptr, bool f32, uint6
   return FT_OK;
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool TWO>
+template <bool PAIR, int EPI, bool A_MN, bool B_MN, bool TWO>
 int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g,
-                int* pairs_used = nullptr) {
-  auto kernel = k_ce_gemm<EPI, A_MN, B_MN, TWO>;
+                int* workers_used) {
+  auto kernel = k_ce_gemm<PAIR, EPI, A_MN, B_MN, TWO>;
+  constexpr int CTAS = PAIR ? 2 : 1;
   static bool ready[FT_MAX_DEVICES] = {};
   static int most[FT_MAX_DEVICES] = {};
   if (!ready[ctx->device]) {
     FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(EPI)));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ctx->sm_count & ~1));
+    cfg.gridDim = dim3((unsigned)(ctx->sm_count / CTAS * CTAS));
     cfg.blockDim = dim3(threads_of(EPI));
     cfg.dynamicSmemBytes = smem_bytes(EPI);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.x = CTAS; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
     int n = 0;
     FT_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-    most[ctx->device] = std::max(1, std::min(n, ctx->sm_count / 2));
+    most[ctx->device] = std::max(1, std::min(n, ctx->sm_count / CTAS));
     ready[ctx->device] = true;
   }
-  const long long units = (long long)ft_cdiv(g.M, TILE) * ft_cdiv(g.N, g.tile_n) * g.splits;
-  const int pairs = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
-  if (pairs_used) *pairs_used = pairs;
+  const long long units = (long long)ft_cdiv(g.M, CTAS * 128) * ft_cdiv(g.N, g.tile_n) * g.splits;
+  const int workers = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
+  if (workers_used) *workers_used = workers;
   const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
                                 A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
-  cudaError_t e = ft_launch_ex(ctx, kernel, 2 * pairs, threads_of(EPI), smem_bytes(EPI), a, b, o, g, ctx->status_dev);
+  cudaError_t e = ft_launch_ex(ctx, kernel, CTAS * workers, threads_of(EPI), smem_bytes(EPI), a, b, o, g, ctx->status_dev);
   if (ctx->profile_all) ft_prof_end(ctx);
   ctx->launches++;
   if (e == cudaSuccess) e = cudaPeekAtLastError();
@@ -1010,11 +1037,22 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   return FT_OK;
 }
 
-template <int EPI, bool A_MN, bool B_MN>
-int launch_gemm(FtContext* ctx, bool two, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const TcProduct& g,
-                int* pairs_used = nullptr) {
-  return two ? launch_gemm<EPI, A_MN, B_MN, true>(ctx, a, b, o, g, pairs_used)
-             : launch_gemm<EPI, A_MN, B_MN, false>(ctx, a, b, o, g, pairs_used);
+// One CTA a tile (128 rows) where there are no more rows than that, else pairs (256).  `b_mn`: W's layout
+// makes B M/N-contiguous.
+template <int EPI>
+int launch_rows(FtContext* ctx, bool pair, bool b_mn, bool two, const CUtensorMap& a, const CUtensorMap& b,
+                const CUtensorMap& o, const TcProduct& g, int* workers_used = nullptr) {
+  constexpr bool F = EPI == EPI_FACTOR;   // planes make no difference there
+  if (pair) {
+    if (b_mn) return two && !F ? launch_gemm<true, EPI, false, true, !F>(ctx, a, b, o, g, workers_used)
+                               : launch_gemm<true, EPI, false, true, false>(ctx, a, b, o, g, workers_used);
+    return two && !F ? launch_gemm<true, EPI, false, false, !F>(ctx, a, b, o, g, workers_used)
+                     : launch_gemm<true, EPI, false, false, false>(ctx, a, b, o, g, workers_used);
+  }
+  if (b_mn) return two && !F ? launch_gemm<false, EPI, false, true, !F>(ctx, a, b, o, g, workers_used)
+                             : launch_gemm<false, EPI, false, true, false>(ctx, a, b, o, g, workers_used);
+  return two && !F ? launch_gemm<false, EPI, false, false, !F>(ctx, a, b, o, g, workers_used)
+                   : launch_gemm<false, EPI, false, false, false>(ctx, a, b, o, g, workers_used);
 }
 
 // plane pairs of a product, the smallest first: sums grow as late as they can
@@ -1035,18 +1073,19 @@ struct TcPlan {
   float* acc;
   int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld;
   int stat_n, out_n;         // columns of a tile: of the statistics alone, of dh and (vocab-major) dW
-  bool w_staged, by_exp;
+  int tile_m;                // rows of a tile of the products whose rows are the packed ones
+  bool pair, w_staged, by_exp;
   size_t bytes;
 };
 
 // Columns of a tile, a multiple of 32, for n columns and `rows` tiles of rows (times parts): whole
-// waves of pairs as full as they get.  A tile costs its columns and about 24 more.
-int pick_tile_n(long long n, long long row_tiles, int pairs) {
+// waves of tiles as full as they get.  A tile costs its columns and about 24 more.
+int pick_tile_n(long long n, long long row_tiles, int workers) {
   int best = TILE;
   double least = 1e30;
   for (int t = TILE; t >= 64; t -= 32) {
     const long long tiles = row_tiles * ft_cdiv(n, t);
-    const double cost = (double)((tiles + pairs - 1) / pairs) * (t + 24);
+    const double cost = (double)((tiles + workers - 1) / workers) * (t + 24);
     if (cost < least * 0.995) { least = cost; best = t; }
   }
   return best;
@@ -1056,7 +1095,9 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   TcPlan pl = {};
   Carver c(base);
   const bool two = ctx->gemm_mode == FT_GEMM_F16X2;
-  const int pairs = std::max(1, ctx->sm_count / 2);
+  pl.pair = q.T > 128;
+  pl.tile_m = pl.pair ? 256 : 128;
+  const int workers = std::max(1, pl.pair ? ctx->sm_count / 2 : ctx->sm_count);
   pl.rows = carve_rows(c, q.T);
   pl.Tp = (int)ft_align_up((size_t)std::max(q.T, 1), TILE);
   pl.h_ld = (int)ft_align_up((size_t)q.H, 8);
@@ -1071,8 +1112,8 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   pl.h = c.take<__half>((size_t)pl.h_planes * pl.Tp * pl.h_ld);
   pl.w = pl.w_staged ? c.take<__half>((size_t)pl.w_planes * pl.w_rows * pl.w_ld) : nullptr;
   // few row tiles: the columns of a tile follow the number of waves (the last one may be nearly empty)
-  pl.stat_n = pl.Tp <= 2 * TILE && !pl.by_exp ? pick_tile_n(q.V, pl.Tp / TILE, pairs) : TILE;
-  pl.out_n = pick_tile_n(q.H, 1 << 20, pairs);
+  pl.stat_n = q.T <= 2 * TILE && !pl.by_exp ? pick_tile_n(q.V, ft_cdiv(q.T, pl.tile_m), workers) : TILE;
+  pl.out_n = pick_tile_n(q.H, 1 << 20, workers);
   size_t part_bytes = (size_t)2 * ft_cdiv(q.V, pl.stat_n) * pl.Tp * sizeof(float2), grad_bytes = 0;
   if (q.grad_hidden || q.grad_weight) {
     const size_t column = (size_t)pl.Tp * 2 * pl.g_planes;
@@ -1097,11 +1138,11 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   if (q.grad_hidden) {
     // K parts: as many as fill the pairs in whole waves, each at least 1024 deep, 256 MB of slabs
     pl.acc_ld = (int)ft_align_up((size_t)q.H, 4);
-    const long long tiles = (long long)(pl.Tp / TILE) * ft_cdiv(q.H, pl.out_n);
+    const long long tiles = (long long)ft_cdiv(q.T, pl.tile_m) * ft_cdiv(q.H, pl.out_n);
     double best = 1e30;
     for (int s = 1; s <= 64 && s * 1024 <= std::max(1024, pl.piece); ++s) {
       if (s > 1 && (size_t)s * pl.Tp * pl.acc_ld * 4 > ((size_t)256 << 20)) break;
-      const double waves = (double)((tiles * s + pairs - 1) / pairs) / s;
+      const double waves = (double)((tiles * s + workers - 1) / workers) / s;
       if (waves < best * 0.97) { best = waves; pl.splits = s; }
     }
     pl.acc = c.take<float>((size_t)pl.splits * pl.Tp * pl.acc_ld);
@@ -1151,17 +1192,17 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   auto mn_map = [&](CUtensorMap* m, const void* p, int inner, int rows, int planes, int ld) {
     return make_map3(ctx, m, p, false, inner, rows, planes, ld, 64, 64);
   };
-  auto tile = [&](TcProduct& p, int tile_n, int a_rows, bool second, bool b_mn) {
+  auto tile = [&](TcProduct& p, bool pair, int tile_n, int a_rows, bool b_mn) {
     p.tile_n = tile_n;
-    p.a_second = second;
     p.a_bytes = a_rows * 128;
-    const int b_bytes = b_mn ? (tile_n > 128 ? 2 : 1) * 8192 : tile_n / 2 * 128;
-    p.stage_bytes = p.a_bytes + b_bytes;
-    p.stage_tx = (second ? 2 : 1) * p.a_bytes + 2 * b_bytes;
+    const int b_cols = pair ? tile_n / 2 : tile_n, b_bytes = (b_mn ? (int)ft_align_up((size_t)b_cols, 64) : b_cols) * 128;
+    p.stage_bytes = (int)ft_align_up((size_t)(p.a_bytes + b_bytes), 1024);
+    p.stage_tx = (pair ? 2 : 1) * (p.a_bytes + b_bytes);
   };
-  // at most 128 rows: the even CTA's are all there are, and only as many are loaded
-  const bool second = T > 128;
-  const int a_rows = second ? 128 : (int)ft_align_up((size_t)T, 8);
+  // columns of a K-contiguous B that a CTA loads
+  auto b_box = [&](int tile_n) { return pl.pair ? tile_n / 2 : tile_n; };
+  // at most 128 rows: only as many are loaded
+  const int a_rows = pl.pair ? 128 : (int)ft_align_up((size_t)T, 8);
   CUtensorMap h_k, w_k, w_mn;
   FT_TRY(k_map(&h_k, unpacked ? t.hidden : pl.h, H, unpacked ? T : pl.Tp, pl.h_planes, pl.h_ld, a_rows));
   if (!vm || t.grad_hidden) FT_TRY(mn_map(&w_mn, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld));
@@ -1198,25 +1239,23 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.k0 = v0; p.b_has_k0 = 1;
     p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
     p.part = pl.part; p.part_ld = pl.Tp;
-    tile(p, pl.out_n, 128, true, vm);
+    tile(p, pl.pair, pl.out_n, a_rows, vm);
     return p;
   };
 
   if (pl.by_exp) {
-    FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, vm ? 128 : pl.out_n / 2));
-    tile(z, TILE, a_rows, second, !vm);
+    FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(vm ? TILE : pl.out_n)));
+    tile(z, pl.pair, TILE, a_rows, !vm);
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
       const int cols = std::min(pl.piece, V - v0);
       const bool first = v0 == 0, last = v0 + cols == V;
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
-      if (vm) FT_TRY((launch_gemm<EPI_EXP, false, false>(ctx, two, h_k, w_k, g_out, z)));
-      else FT_TRY((launch_gemm<EPI_EXP, false, true>(ctx, two, h_k, w_mn, g_out, z)));
+      FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
       FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(cols, TILE), pl.rows, 0, first ? 1 : 0,
                     last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
-      if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, 128));
+      if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       const TcProduct p = dh_product(v0, cols);
-      if (vm) FT_TRY((launch_gemm<EPI_FACTOR, false, true, false>(ctx, g_k, w_mn, acc_out, p)));
-      else FT_TRY((launch_gemm<EPI_FACTOR, false, false, false>(ctx, g_k, w_k, acc_out, p)));
+      FT_TRY(launch_rows<EPI_FACTOR>(ctx, pl.pair, vm, two, g_k, vm ? w_mn : w_k, acc_out, p));
     }
     if (q.p.grad_hidden_type == FT_TYPE_F16)
       FT_LAUNCH_PDL(ctx, k_ce_scatter_exp<__half>, unpack_grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, pl.wy,
@@ -1227,43 +1266,37 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     return FT_OK;
   }
 
-  tile(z, pl.stat_n, a_rows, second, !vm);
+  tile(z, pl.pair, pl.stat_n, a_rows, !vm);
   z.w_early = !pl.w_staged;
-  z.carry = T <= TILE ? 1 : 0;
-  int pairs = 0;
-  if (vm) {
-    FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, pl.stat_n / 2));
-    FT_TRY((launch_gemm<EPI_STATS, false, false>(ctx, two, h_k, w_k, h_k, z, &pairs)));
-  } else {
-    FT_TRY((launch_gemm<EPI_STATS, false, true>(ctx, two, h_k, w_mn, h_k, z, &pairs)));
-  }
-  FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * (z.carry ? pairs : ft_cdiv(V, pl.stat_n)),
+  z.carry = T <= pl.tile_m ? 1 : 0;
+  int workers = 0;
+  if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(pl.stat_n)));
+  FT_TRY(launch_rows<EPI_STATS>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, h_k, z, &workers));
+  FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * (z.carry ? workers : ft_cdiv(V, pl.stat_n)),
                 z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
   if (!t.grad_hidden && !t.grad_weight) return FT_OK;
 
   CUtensorMap g_mn, h_mn, dw_out;
-  FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, vm ? 128 : pl.out_n / 2));
+  FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(vm ? TILE : pl.out_n)));
   FT_TRY(mn_map(&h_mn, pl.h, H, pl.Tp, pl.h_planes, pl.h_ld));
   const bool dw16 = q.p.grad_weight_type == FT_TYPE_F16;
   const bool dw_tma = t.grad_weight && ((uintptr_t)t.grad_weight & 15) == 0 && pl.w_cols % (dw16 ? 8 : 4) == 0;
   if (dw_tma)
     FT_TRY(make_map3(ctx, &dw_out, t.grad_weight, !dw16, pl.w_cols, pl.w_rows, 1, pl.w_cols, 32, 32,
                      dw16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B));
-  tile(z, TILE, a_rows, second, !vm);
+  tile(z, pl.pair, TILE, a_rows, !vm);
   for (int v0 = 0; v0 < V; v0 += pl.piece) {
     const int cols = std::min(pl.piece, V - v0);
     z.N = cols; z.v0 = v0; z.b_mn0 = v0;
-    if (vm) FT_TRY((launch_gemm<EPI_GRAD, false, false>(ctx, two, h_k, w_k, g_out, z)));
-    else FT_TRY((launch_gemm<EPI_GRAD, false, true>(ctx, two, h_k, w_mn, g_out, z)));
+    FT_TRY(launch_rows<EPI_GRAD>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
     // as operands, the piece ends with the vocabulary: what lies behind reads as zero
     if (v0 == 0 || cols != pl.piece) {
-      FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, 128));
+      FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       FT_TRY(mn_map(&g_mn, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece));
     }
     if (t.grad_hidden) {
       const TcProduct p = dh_product(v0, cols);
-      if (vm) FT_TRY((launch_gemm<EPI_STORE, false, true>(ctx, two, g_k, w_mn, acc_out, p)));
-      else FT_TRY((launch_gemm<EPI_STORE, false, false>(ctx, two, g_k, w_k, acc_out, p)));
+      FT_TRY(launch_rows<EPI_STORE>(ctx, pl.pair, vm, two, g_k, vm ? w_mn : w_k, acc_out, p));
     }
     if (t.grad_weight) {
       TcProduct p = {};
@@ -1279,9 +1312,11 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
         p.M = H; p.N = cols; p.out_x0 = v0;
         set_terms(p, pl.h_planes, pl.g_planes);
       }
-      tile(p, vm ? pl.out_n : TILE, 128, true, true);
+      tile(p, true, vm ? pl.out_n : TILE, 128, true);
       p.n_fast = p.M >= p.N; p.band = ft_cdiv(p.M, TILE);
-      FT_TRY((launch_gemm<EPI_STORE, true, true>(ctx, two, vm ? g_mn : h_mn, vm ? h_mn : g_mn, dw_tma ? dw_out : g_mn, p)));
+      const CUtensorMap &pa = vm ? g_mn : h_mn, &pb = vm ? h_mn : g_mn, &po = dw_tma ? dw_out : g_mn;
+      if (two) FT_TRY((launch_gemm<true, EPI_STORE, true, true, true>(ctx, pa, pb, po, p, nullptr)));
+      else FT_TRY((launch_gemm<true, EPI_STORE, true, true, false>(ctx, pa, pb, po, p, nullptr)));
     }
   }
   if (t.grad_hidden) {
