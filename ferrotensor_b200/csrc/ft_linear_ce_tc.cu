@@ -5,10 +5,11 @@
 // operand is ever transposed:
 //   logits   A = packed rows,    B = W            K = hidden    epilogue: row statistics, E, or g
 //   dh       A = E or g,         B = W            K = a vocabulary piece (in `splits` parts)
-//   dW       A = g, B = rows (W is [vocab, hidden]) or A = rows, B = g ([hidden, vocab])   K = rows
+//   dW       A = g,              B = packed rows  K = rows (turned over for [hidden, vocab] weights)
 //
 // dW's K runs over rows, so its operand g must be normalised, which needs every row's log-sum-exp
-// first: the logits are computed twice.  dh alone does not need that.  The pass that finds the
+// first: the logits are computed twice (or, in the split mode when the vocabulary is one piece, g is made
+// of E in place).  dh alone does not need that.  The pass that finds the
 // statistics writes E = 2^(z2 - ref) for each column tile (z2 in log2 units, ref the row's maximum in
 // that tile: E has f16's full precision whatever the row's normaliser turns out to be), and the
 // product E W is drained from tensor memory once a tile of K and scaled there, in f32, by the
@@ -44,19 +45,25 @@ constexpr int MAX_BUFFERS = 4;            // accumulators: two of 256 columns, f
 // STATS: row statistics.  EXP: statistics and E.  GRAD: g.  STORE: the sum.  FACTOR: the sum with every
 // TILE of K scaled by its row's factor.
 enum Epi { EPI_STATS, EPI_EXP, EPI_GRAD, EPI_STORE, EPI_FACTOR };
-// Warps that drain: FACTOR's empty an accumulator for every 2048 cycles of the tensor cores, which eight
+// Warps that drain.  FACTOR's empty an accumulator for every 2048 cycles of the tensor cores, which eight
 // warps do not manage (4096 x 2048 x 24576: 345 us, 317 with sixteen, of 286 with no drain at all).
-constexpr int drain_warps(int epi) { return epi == EPI_FACTOR ? 16 : 8; }
+// The statistics bound small K (a tile takes eight warps 6100 cycles, sixteen 4400, the products 512
+// for each 64 of K).  Where results are staged or slices summed, sixteen cost a stage or spills:
+// eight there (8 x 4 KiB beside six stages; g at K = 2048 takes 412 thousand cycles, with sixteen and
+// five stages 419).
+constexpr int drain_warps(int epi, bool two) { return epi == EPI_FACTOR || (epi == EPI_STATS && !two) ? 16 : 8; }
+// Statistics of a row that a tile leaves: one a warp of its quadrant.
+constexpr int parts_of(int epi, bool two) { return drain_warps(epi, two) / 4; }
 // The statistics' launches have two warps more, for the targets' logits.
-constexpr int threads_of(int epi) { return 64 + 32 * drain_warps(epi) + (epi <= EPI_EXP ? 64 : 0); }
+constexpr int threads_of(int epi, bool two) { return 64 + 32 * drain_warps(epi, two) + (epi <= EPI_EXP ? 64 : 0); }
 // Shared memory: the stages (six, or five, of 32 KiB; more where few rows or narrow tiles make them
-// smaller), 4 KiB for each draining warp, the barriers (full, empty, tfull, tempty, one a quadrant),
-// and room to align all that.
+// smaller), 4 KiB for each draining warp that stages results, the barriers (full, empty, tfull, tempty,
+// one a quadrant), and room to align all that.
 constexpr int MAX_STAGES = 16;
 constexpr int epi_offset(int epi) { return (epi == EPI_FACTOR ? 5 : 6) * STAGE_BYTES; }
-constexpr int bar_offset(int epi) { return epi_offset(epi) + drain_warps(epi) * 4096; }
-constexpr int barriers_of(int) { return 2 * MAX_STAGES + 2 * MAX_BUFFERS + 4; }
-constexpr int smem_bytes(int epi) { return bar_offset(epi) + barriers_of(epi) * 8 + 16 + 1024; }
+constexpr int bar_offset(int epi, bool two) { return epi_offset(epi) + (epi == EPI_STATS ? 16384 : drain_warps(epi, two) * 4096); }
+constexpr int BARRIERS = 2 * MAX_STAGES + 2 * MAX_BUFFERS + 4;
+constexpr int smem_bytes(int epi, bool two) { return bar_offset(epi, two) + BARRIERS * 8 + 16 + 1024; }
 // k-blocks of 64 that are summed in tensor memory; 0: all
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
 
@@ -76,7 +83,7 @@ struct TcProduct {
   int a_has_k0, b_has_k0;           // ... and which of them k0 applies to
   // EPI_STATS, EPI_GRAD
   Rows rw;
-  float2* part;                     // [2 * column tiles][part_ld]: {maximum in log2 units, sum}
+  float2* part;                     // [parts of a tile * column tiles][part_ld]: {maximum in log2 units, sum}
   int part_ld;
   int w_early;                      // STATS: W may be read before the launch before this one has ended
   int piece, pieces;                // STATS, EXP: which launch this is, of how many
@@ -92,6 +99,7 @@ struct TcProduct {
   int out_type;                     // FT_TYPE_*
   int accumulate;
   int unscale;                      // multiply by the scales of g and of the rows
+  int transposed;                   // the output is [N, M]
   int out_x0, out_y0;
   void* direct;                     // when the output breaks a TMA rule: plain stores
   long long direct_ld;
@@ -190,8 +198,7 @@ __device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const
 // cost a 32-byte sector for every 2 bytes; with many rows (R = 32) all warps walk down K together,
 // so that DRAM reads a row of W once for all targets in it (with a row a warp, 4096 rows x 2048
 // read 540 MB for 100 MB of W and the products waited for them: 390 against 277 us).
-// KEEP: the columns go to wy as well, for the one-hot term of dh.
-template <bool KEEP>
+// With g.wy the columns are kept, for the one-hot term of dh.
 __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, int worker, int workers, float c2, int lane) {
   const int rows = r1 - r0;
   int R = 1;
@@ -206,7 +213,7 @@ __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, 
     for (int pw = 0; pw < g.w_planes && on; ++pw) {
       const __half* h = g.h + (long long)r * g.h_ld;
       const __half* w = g.w + pw * g.w_plane + (long long)y * g.w_sv;
-      __half* keep = KEEP ? g.wy + ((long long)pw * g.part_ld + r) * g.wy_ld : nullptr;
+      __half* keep = g.wy ? g.wy + ((long long)pw * g.part_ld + r) * g.wy_ld : nullptr;
       // (pitches of h and wy are multiples of 8, and so is W's where K is the contiguous index)
       for (int k0 = sub * 16; k0 < g.h_ld; k0 += share * 16) {
         uint4 hv[2], lv[2], wv[2];
@@ -235,7 +242,7 @@ __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, 
             acc = fmaf(x.x + z.x, f.x, acc);
             acc = fmaf(x.y + z.y, f.y, acc);
           }
-          if (KEEP && k0 + 8 * j < g.h_ld) *(uint4*)(keep + k0 + 8 * j) = wv[j];
+          if (keep && k0 + 8 * j < g.h_ld) *(uint4*)(keep + k0 + 8 * j) = wv[j];
         }
       }
     }
@@ -245,10 +252,11 @@ __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, 
 }
 
 template <bool PAIR, int EPI, bool A_MN, bool B_MN, bool TWO>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(threads_of(EPI), 1)
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(threads_of(EPI, TWO), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
-  constexpr int WARPS = drain_warps(EPI), EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI);
+  constexpr int WARPS = drain_warps(EPI, TWO), PARTS = parts_of(EPI, TWO);
+  constexpr int EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI, TWO);
   constexpr int CHUNKS = 32 / WARPS;        // of 32 columns, at most, a draining warp
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -259,7 +267,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const uint32_t bar_tfull = bar_empty + MAX_STAGES * 8;
   const uint32_t bar_tempty = bar_tfull + MAX_BUFFERS * 8;
   const uint32_t bar_quad = bar_tempty + MAX_BUFFERS * 8;
-  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + barriers_of(EPI) * 8);
+  uint32_t* tmem_slot = (uint32_t*)(gbase + BAR_OFFSET + BARRIERS * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -276,7 +284,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       mbar_init(bar_tfull + b * 8, 1);
       mbar_init(bar_tempty + b * 8, (PAIR ? 2 : 1) * WARPS);
     }
-    for (int b = 0; b < 4; ++b) mbar_init(bar_quad + b * 8, 2);   // the two warps of a quadrant
+    for (int b = 0; b < 4; ++b) mbar_init(bar_quad + b * 8, WARPS / 4);   // the warps of a quadrant
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -408,7 +416,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const float c2 = (unpacked ? 1.f : g.rw.head->z_scale) * 1.4426950408889634f;
     // each launch of a vocabulary in pieces takes its share of the rows
     const int r0 = (int)((long long)live * g.piece / g.pieces), r1 = (int)((long long)live * (g.piece + 1) / g.pieces);
-    target_dots<EPI == EPI_EXP>(g, r0, r1, (int)blockIdx.x * 2 + warp - 2 - WARPS, (int)gridDim.x * 2, c2, lane);
+    target_dots(g, r0, r1, (int)blockIdx.x * 2 + warp - 2 - WARPS, (int)gridDim.x * 2, c2, lane);
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
     // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the warps of a quadrant share the
@@ -557,9 +565,29 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (c0 >= g.N || y0 >= rows_end) return;                 // the whole block lies outside
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] *= alpha;
+          if (g.direct != nullptr && g.transposed) {
+            // a lane is a column of the output: 32 consecutive ones a store
+            if (row < rows_end) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const long long at = (long long)(c0 + k) * g.direct_ld + g.out_x0 + row;
+                if (c0 + k >= g.N) break;
+                if (g.out_type == FT_TYPE_F16) ((__half*)g.direct)[at] = __float2half_rn(v[k]);
+                else ((float*)g.direct)[at] = v[k];
+              }
+            }
+            return;
+          }
           if (lane == 0) bulk_wait_read();
           __syncwarp();
-          if (g.direct == nullptr && g.out_type == FT_TYPE_F16) {
+          if (g.transposed) {
+            // the block turned over: output row k in staging row k, this lane's value in column `lane`
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              if (g.out_type == FT_TYPE_F16) *(__half*)(st + k * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __float2half_rn(v[k]);
+              else *(float*)(st + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4) = v[k];
+            }
+          } else if (g.direct == nullptr && g.out_type == FT_TYPE_F16) {
             uint32_t h[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) h[k >> 1] = pack_h2(v[k], v[k + 1]);
@@ -574,8 +602,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-              if (g.accumulate) tma_add_3d(&map_o, st_addr, g.out_x0 + c0, g.out_y0 + y0, un.sp);
-              else tma_store_3d(&map_o, st_addr, g.out_x0 + c0, g.out_y0 + y0, un.sp);
+              const int x = g.out_x0 + (g.transposed ? y0 : c0), y = g.out_y0 + (g.transposed ? c0 : y0);
+              if (g.accumulate) tma_add_3d(&map_o, st_addr, x, y, un.sp);
+              else tma_store_3d(&map_o, st_addr, x, y, un.sp);
               bulk_commit();
             }
           } else {
@@ -607,9 +636,11 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         __syncwarp();
         slot[lane] = m;
         if (!meet()) return m;
-        const float other = ((const float*)(gbase + EPI_OFFSET))[((warp - 2) ^ 4) * 1024 + lane];
+#pragma unroll
+        for (int j = 1; j < WARPS / 4; ++j)
+          m = fmaxf(m, ((const float*)(gbase + EPI_OFFSET))[((warp - 2 + 4 * j) % WARPS) * 1024 + lane]);
         meet();
-        return fmaxf(m, other);
+        return m;
       };
       auto release = [&](uint32_t buf) {
         tc_fence_before();
@@ -641,7 +672,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               // ahead, kept each at 3900 cycles (390 us for the product above)
 #pragma unroll 4
               for (int j = 0; j < 32 && s0 + SLICE * j < kb1; ++j) {
-                const float m = row < live ? g.part[(size_t)(2 * (s0 / SLICE + j)) * g.part_ld + row].x : 0.f;
+                const float m = row < live ? g.part[(size_t)(parts_of(EPI_EXP, true) * (s0 / SLICE + j)) * g.part_ld + row].x : 0.f;
                 // (a difference of two infinities belongs to a row of NaN anyway)
                 factors[j * 32 + lane] = ex2(finite_max(m) - base2);
               }
@@ -719,12 +750,12 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
       }
       if constexpr (EPI <= EPI_EXP) {
-        if (EPI != EPI_STATS || !g.carry) g.part[(size_t)(un.nt * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+        if (EPI != EPI_STATS || !g.carry) g.part[(size_t)(un.nt * PARTS + grp) * g.part_ld + row] = make_float2(run_m, run_s);
       }
     }
     if (EPI == EPI_STATS && g.carry) {
       const int row = (int)rank * 128 + quad * 32 + lane;
-      g.part[(size_t)(pair * 2 + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+      g.part[(size_t)(pair * PARTS + grp) * g.part_ld + row] = make_float2(run_m, run_s);
     }
     // what was stored is complete before the launch ends
     if (lane == 0) bulk_wait_all();
@@ -746,31 +777,31 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 }
 
 // ------------------------------------------------------------------------------ around the products
-// Joins the column tiles' {maximum, sum} of 32 rows, tiles over 32 warps in a fixed order, with what
+// Joins the column tiles' {maximum, sum} of 32 rows, tiles over the warps in a fixed order, with what
 // the pieces before (not `first`) have left; after the last piece writes the row's log-sum-exp (in
 // log2 units, as the gradient's epilogue wants it) and its loss.
 // With `acc` (E is in use): sets the point R that the row's E W is scaled against.  It stays the maximum
 // of the first piece, and f32 carries what later pieces are above it, unless that is 2^64 or
 // more: then it moves, and the row's sums so far are scaled down.
-constexpr int LOSS_WARPS = 32;
-__global__ void __launch_bounds__(32 * LOSS_WARPS)
+constexpr int JOIN_WARPS = 32;            // at most; few parts of many rows take eight
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
 k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int unpacked_rows, int first, int last,
           int vocab, float* __restrict__ row_loss, float* __restrict__ acc, size_t slab, int splits, int ld, int H) {
-  __shared__ float2 red[LOSS_WARPS][32];
+  __shared__ float2 red[JOIN_WARPS][32];
   __shared__ float shrink[32];
   ft_pdl_wait();
   ft_pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   const int live = unpacked_rows ? unpacked_rows : rw.head->count;
   if ((int)blockIdx.x * 32 >= live) return;
   float m = -INFINITY, s = 0.f;
   constexpr int AT_ONCE = 16;
-  for (int p0 = warp; p0 < parts; p0 += AT_ONCE * LOSS_WARPS) {
+  for (int p0 = warp; p0 < parts; p0 += AT_ONCE * warps) {
     float2 v[AT_ONCE];
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
-      const int p = p0 + j * LOSS_WARPS;
+      const int p = p0 + j * warps;
       v[j] = p < parts ? part[(size_t)p * part_ld + row] : make_float2(-INFINITY, 0.f);
     }
     float mn = m;
@@ -789,12 +820,10 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
     if (row < live) {
       const float2 old = first ? make_float2(-INFINITY, 0.f) : rw.stat[row];
       float M = old.x;
-#pragma unroll
-      for (int w = 0; w < LOSS_WARPS; ++w) M = fmaxf(M, red[w][lane].x);
+      for (int w = 0; w < warps; ++w) M = fmaxf(M, red[w][lane].x);
       const float ref = finite_max(M);
       float S = old.y * ex2(old.x - ref);
-#pragma unroll
-      for (int w = 0; w < LOSS_WARPS; ++w) S += red[w][lane].y * ex2(red[w][lane].x - ref);
+      for (int w = 0; w < warps; ++w) S += red[w][lane].y * ex2(red[w][lane].x - ref);
       if (!last) rw.stat[row] = make_float2(M, S);
       if (acc) {
         if (first) {
@@ -834,7 +863,52 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
     const float f = shrink[r];
     if (f == 1.f) continue;
     for (int sp = 0; sp < splits; ++sp)
-      for (int c = threadIdx.x; c < H; c += 32 * LOSS_WARPS) acc[sp * slab + (size_t)(blockIdx.x * 32 + r) * ld + c] *= f;
+      for (int c = threadIdx.x; c < H; c += blockDim.x) acc[sp * slab + (size_t)(blockIdx.x * 32 + r) * ld + c] *= f;
+  }
+}
+
+// E -> g in place, both planes, for a vocabulary that is one piece: g = w (2^(ref - lse) E - onehot), with the
+// gradient at the target from the row's loss (as k_ce_join has it), and zero rows up to a K block of dW.
+// One read and one write of E against a second product for the logits: from hidden = 300 or so on
+// the cheaper way.  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
+__global__ void __launch_bounds__(256)
+k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __restrict__ part, int part_ld, Rows rw, int cols,
+               const float* __restrict__ row_loss) {
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const int live = rw.head->count, end = max(64, (live + 63) / 64 * 64);
+  for (int r = blockIdx.y; r < end; r += gridDim.y) {
+    float lse2 = 0.f, w = 0.f, at_target = 0.f;
+    uint32_t y = FT_MASKED_CE_SKIP;
+    if (r < live) {
+      lse2 = rw.lse[r];
+      w = rw.weight[r] * rw.head->g_scale;
+      y = rw.target[r];
+      at_target = w * expm1f(-row_loss[rw.source[r]]);
+    }
+    for (int c = (blockIdx.x * 256 + threadIdx.x) * 8; c < cols; c += gridDim.x * 2048) {
+      __half* p = e + (size_t)r * ld + c;
+      uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
+      if (r < live) {
+        const float f = w * ex2(finite_max(part[(size_t)(parts_of(EPI_EXP, true) * (c / TILE)) * part_ld + r].x) - lse2);
+        hi = *(const uint4*)p;
+        lo = *(const uint4*)(p + plane);
+        uint32_t* a = (uint32_t*)&hi;
+        uint32_t* b = (uint32_t*)&lo;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = __half22float2(*(const __half2*)&a[k]), z = __half22float2(*(const __half2*)&b[k]);
+          float g0 = f * (x.x + z.x), g1 = f * (x.y + z.y);
+          if (y == (uint32_t)(c + 2 * k)) g0 = at_target;
+          if (y == (uint32_t)(c + 2 * k + 1)) g1 = at_target;
+          a[k] = pack_h2(g0, g1);
+          const float2 q = __half22float2(*(const __half2*)&a[k]);
+          b[k] = pack_h2(g0 - q.x, g1 - q.y);
+        }
+      }
+      *(uint4*)p = hi;
+      *(uint4*)(p + plane) = lo;
+    }
   }
 }
 
@@ -848,20 +922,23 @@ k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* _
   if ((int)blockIdx.x < w_blocks) {
     const long long step = (long long)w_blocks * 256;
     long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    auto see = [&](float x) {
+      const float a = fabsf(x);
+      if (a < INFINITY) m = fmaxf(m, a);
+    };
     if (((uintptr_t)w & 15) == 0) {
-      for (; i < n / 4; i += step) {
-        const float4 v = ((const float4*)w)[i];
-        const float a = fmaxf(fabsf(v.x), fabsf(v.y)), b = fmaxf(fabsf(v.z), fabsf(v.w));
-        if (fmaxf(a, b) < INFINITY && a + b == a + b) m = fmaxf(m, fmaxf(a, b));
-        else {
-          const float e[4] = {v.x, v.y, v.z, v.w};
-          for (float x : e) if (fabsf(x) < INFINITY) m = fmaxf(m, fabsf(x));
-        }
+      constexpr int AT_ONCE = 4;
+      const float4* w4 = (const float4*)w;
+      for (; i < n / 4; i += AT_ONCE * step) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) v[j] = i + j * step < n / 4 ? w4[i + j * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) { see(v[j].x); see(v[j].y); see(v[j].z); see(v[j].w); }
       }
       i = n / 4 * 4 + (long long)blockIdx.x * 256 + threadIdx.x;
     }
-    for (; i < n; i += step)
-      if (fabsf(w[i]) < INFINITY) m = fmaxf(m, fabsf(w[i]));
+    for (; i < n; i += step) see(w[i]);
   } else {
     for (int r = blockIdx.x - w_blocks; r < rows; r += gridDim.x - w_blocks) {
       if (targets[r] == FT_MASKED_CE_SKIP) continue;
@@ -886,9 +963,10 @@ k_ce_weight(const T* __restrict__ w, int rows, int cols, __half* __restrict__ ou
   ft_pdl_launch();
   const float S = sizeof(T) == 4 ? power_for(head->w_amax, OPERAND_EXP) : 1.f;
   const size_t plane = (size_t)rows * ld;
-  const int units = ld / 8;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * units; i += (long long)gridDim.x * 256) {
-    const int r = (int)(i / units), c = (int)(i % units) * 8;
+  // a warp takes 1024 columns of a row
+  const int c_end = min(ld, ((int)blockIdx.y + 1) * 1024);
+  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
+  for (int c = blockIdx.y * 1024 + (threadIdx.x % 32) * 8; c < c_end; c += 256) {
     const T* p = w + (size_t)r * cols + c;
     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -910,9 +988,11 @@ k_ce_scatter(const float* __restrict__ acc, size_t slab, int splits, int ld, Row
   ft_pdl_wait();
   ft_pdl_launch();
   const float alpha = rw.head->g_unscale * rw.head->w_unscale;
-  const int units = ld / 4;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * units; i += (long long)gridDim.x * 256) {
-    const int r = (int)(i / units), c = (int)(i % units) * 4;
+  // a warp takes 256 columns of a row
+  const int c_end = min(ld, ((int)blockIdx.y + 1) * 256);
+  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
+#pragma unroll
+  for (int c = blockIdx.y * 256 + (threadIdx.x % 32) * 4; c < c_end; c += 128) {
     const int at = rw.place[r];
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (at >= 0) {
@@ -941,9 +1021,11 @@ k_ce_scatter_exp(const float* __restrict__ acc, size_t slab, int splits, int ld,
                  size_t wy_plane, int wy_ld, int w_planes, int H, int rows, T* __restrict__ out) {
   ft_pdl_wait();
   ft_pdl_launch();
-  const int units = ld / 4;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * units; i += (long long)gridDim.x * 256) {
-    const int r = (int)(i / units), c = (int)(i % units) * 4;
+  // a warp takes 256 columns of a row
+  const int c_end = min(ld, ((int)blockIdx.y + 1) * 256);
+  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
+#pragma unroll
+  for (int c = blockIdx.y * 256 + (threadIdx.x % 32) * 4; c < c_end; c += 128) {
     const int at = rw.place[r];
     float e[4] = {0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
@@ -1008,11 +1090,11 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   static bool ready[FT_MAX_DEVICES] = {};
   static int most[FT_MAX_DEVICES] = {};
   if (!ready[ctx->device]) {
-    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(EPI)));
+    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(EPI, TWO)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctx->sm_count / CTAS * CTAS));
-    cfg.blockDim = dim3(threads_of(EPI));
-    cfg.dynamicSmemBytes = smem_bytes(EPI);
+    cfg.blockDim = dim3(threads_of(EPI, TWO));
+    cfg.dynamicSmemBytes = smem_bytes(EPI, TWO);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = CTAS; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
@@ -1029,7 +1111,7 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
                                 A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
-  cudaError_t e = ft_launch_ex(ctx, kernel, CTAS * workers, threads_of(EPI), smem_bytes(EPI), a, b, o, g, ctx->status_dev);
+  cudaError_t e = ft_launch_ex(ctx, kernel, CTAS * workers, threads_of(EPI, TWO), smem_bytes(EPI, TWO), a, b, o, g, ctx->status_dev);
   if (ctx->profile_all) ft_prof_end(ctx);
   ctx->launches++;
   if (e == cudaSuccess) e = cudaPeekAtLastError();
@@ -1064,7 +1146,10 @@ void set_terms(TcProduct& g, int pa, int pb) {
   add(0, 0);
 }
 
-constexpr size_t G_PIECE_BYTES = (size_t)256 << 20;
+// Bytes of E or g at a time, when the caller leaves the choice.  A piece costs launches whose last wave is
+// not full: 8192 x 2048 x 49152 takes 3.27 ms in pieces of 128 MB, 3.09 of 256, 3.03 of 512, 2.95 in one
+// piece (805 MB: half of the logits in f32), 2048 x 896 x 151936 2.34, 2.17, 2.10 and 2.05.
+constexpr size_t G_PIECE_BYTES = (size_t)512 << 20;
 
 struct TcPlan {
   Rows rows;
@@ -1074,7 +1159,7 @@ struct TcPlan {
   int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld;
   int stat_n, out_n;         // columns of a tile: of the statistics alone, of dh and (vocab-major) dW
   int tile_m;                // rows of a tile of the products whose rows are the packed ones
-  bool pair, w_staged, by_exp;
+  bool pair, w_staged, by_exp, in_place;   // in_place: g is made of E, see k_ce_normalise
   size_t bytes;
 };
 
@@ -1114,7 +1199,7 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   // few row tiles: the columns of a tile follow the number of waves (the last one may be nearly empty)
   pl.stat_n = q.T <= 2 * TILE && !pl.by_exp ? pick_tile_n(q.V, ft_cdiv(q.T, pl.tile_m), workers) : TILE;
   pl.out_n = pick_tile_n(q.H, 1 << 20, workers);
-  size_t part_bytes = (size_t)2 * ft_cdiv(q.V, pl.stat_n) * pl.Tp * sizeof(float2), grad_bytes = 0;
+  size_t part_bytes = (size_t)parts_of(EPI_STATS, two) * ft_cdiv(q.V, pl.stat_n) * pl.Tp * sizeof(float2), grad_bytes = 0;
   if (q.grad_hidden || q.grad_weight) {
     const size_t column = (size_t)pl.Tp * 2 * pl.g_planes;
     size_t cols = q.p.vocab_piece ? q.p.vocab_piece : std::max<size_t>(TILE, G_PIECE_BYTES / column);
@@ -1122,12 +1207,13 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
     // equal pieces of whole tiles
     pl.piece = (int)ft_align_up((size_t)ft_cdiv(q.V, pieces), TILE);
     grad_bytes = column * pl.piece;
-    if (pl.by_exp) part_bytes = (size_t)2 * (pl.piece / TILE) * pl.Tp * sizeof(float2);
+    pl.in_place = two && q.grad_weight && pieces == 1;
+    if (pl.by_exp || pl.in_place) part_bytes = (size_t)parts_of(EPI_EXP, two) * (pl.piece / TILE) * pl.Tp * sizeof(float2);
   }
-  if (pl.by_exp) {
+  if (pl.by_exp || pl.in_place) {
     pl.part = (float2*)c.take<char>(part_bytes);
     pl.grad = (__half*)c.take<char>(grad_bytes);
-    pl.wy = c.take<__half>((size_t)pl.w_planes * pl.Tp * pl.h_ld);
+    if (pl.by_exp) pl.wy = c.take<__half>((size_t)pl.w_planes * pl.Tp * pl.h_ld);
   } else {
     // the statistics of the column tiles are done with before the first piece of g is written
     char* shared = c.take<char>(std::max(part_bytes, grad_bytes));
@@ -1176,7 +1262,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   const void* w = t.weight;
   if (pl.w_staged) {
     w = pl.w;
-    const int grid = (int)std::min<long long>(ft_cdiv((long long)pl.w_rows * (pl.w_ld / 8), 256), (long long)ctx->sm_count * 16);
+    const dim3 grid((unsigned)std::min(ft_cdiv(pl.w_rows, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(pl.w_ld, 1024));
     if (w32)
       FT_LAUNCH_PDL(ctx, k_ce_weight<float>, grid, 256, 0, (const float*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
                     pl.w_planes, pl.rows.head);
@@ -1220,10 +1306,10 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   z.wy = pl.wy; z.wy_ld = pl.h_ld;
   z.pieces = pl.by_exp ? ft_cdiv(V, pl.piece) : 1;
   const size_t slab = (size_t)pl.Tp * pl.acc_ld;
-  const int join_grid = ft_cdiv(T, 32);
+  const int join_grid = ft_cdiv(T, 32), join_threads = T <= 1024 ? 32 * JOIN_WARPS : 256;
   CUtensorMap acc_out;
   if (t.grad_hidden) FT_TRY(make_map3(ctx, &acc_out, pl.acc, true, pl.acc_ld, pl.Tp, pl.splits, pl.acc_ld, 32, 32));
-  const int unpack_grid = (int)std::min<long long>(ft_cdiv((long long)T * (pl.acc_ld / 4), 256), (long long)ctx->sm_count * 16);
+  const dim3 unpack_grid((unsigned)std::min(ft_cdiv(T, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(std::max(pl.acc_ld, 1), 256));
   CUtensorMap g_out, g_k;
   if (t.grad_hidden || t.grad_weight)
     FT_TRY(make_map3(ctx, &g_out, pl.grad, false, pl.piece, pl.Tp, pl.g_planes, pl.piece, 64, 32));
@@ -1251,7 +1337,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       const bool first = v0 == 0, last = v0 + cols == V;
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
-      FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * ft_cdiv(cols, TILE), pl.rows, 0, first ? 1 : 0,
+      FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two) * ft_cdiv(cols, TILE), pl.rows, 0, first ? 1 : 0,
                     last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
       if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       const TcProduct p = dh_product(v0, cols);
@@ -1266,14 +1352,26 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     return FT_OK;
   }
 
-  tile(z, pl.pair, pl.stat_n, a_rows, !vm);
-  z.w_early = !pl.w_staged;
-  z.carry = T <= pl.tile_m ? 1 : 0;
-  int workers = 0;
-  if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(pl.stat_n)));
-  FT_TRY(launch_rows<EPI_STATS>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, h_k, z, &workers));
-  FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, 32 * LOSS_WARPS, 0, pl.part, pl.Tp, 2 * (z.carry ? workers : ft_cdiv(V, pl.stat_n)),
-                z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
+  if (pl.in_place) {
+    tile(z, pl.pair, TILE, a_rows, !vm);
+    if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(TILE)));
+    FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
+    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two) * ft_cdiv(V, TILE), pl.rows,
+                  0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
+    const dim3 grid(ft_cdiv(V, 2048), std::max(1, std::min(pl.Tp, ctx->sm_count * 32 / ft_cdiv(V, 2048))));
+    FT_LAUNCH_PDL(ctx, k_ce_normalise, grid, 256, 0, pl.grad, (size_t)pl.Tp * pl.piece, pl.piece, pl.part, pl.Tp, pl.rows, pl.piece,
+                  t.row_loss);
+  } else {
+    tile(z, pl.pair, pl.stat_n, a_rows, !vm);
+    z.w_early = !pl.w_staged;
+    z.carry = T <= pl.tile_m ? 1 : 0;
+    int workers = 0;
+    if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(pl.stat_n)));
+    FT_TRY(launch_rows<EPI_STATS>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, h_k, z, &workers));
+    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp,
+                  parts_of(EPI_STATS, two) * (z.carry ? workers : ft_cdiv(V, pl.stat_n)), z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss,
+                  (float*)nullptr, (size_t)0, 0, 0, 0);
+  }
   if (!t.grad_hidden && !t.grad_weight) return FT_OK;
 
   CUtensorMap g_mn, h_mn, dw_out;
@@ -1288,7 +1386,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   for (int v0 = 0; v0 < V; v0 += pl.piece) {
     const int cols = std::min(pl.piece, V - v0);
     z.N = cols; z.v0 = v0; z.b_mn0 = v0;
-    FT_TRY(launch_rows<EPI_GRAD>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
+    if (!pl.in_place) FT_TRY(launch_rows<EPI_GRAD>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
     // as operands, the piece ends with the vocabulary: what lies behind reads as zero
     if (v0 == 0 || cols != pl.piece) {
       FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
@@ -1305,18 +1403,17 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       p.unscale = 1;
       p.out_type = (int)q.p.grad_weight_type;
       if (!dw_tma) { p.direct = t.grad_weight; p.direct_ld = pl.w_cols; }
-      if (vm) {
-        p.M = cols; p.N = H; p.out_y0 = v0;
-        set_terms(p, pl.g_planes, pl.h_planes);
-      } else {
-        p.M = H; p.N = cols; p.out_x0 = v0;
-        set_terms(p, pl.h_planes, pl.g_planes);
-      }
-      tile(p, true, vm ? pl.out_n : TILE, 128, true);
+      // rows of a tile are vocabulary either way: their number is a multiple of the tile, hidden's is not
+      p.M = cols; p.N = H;
+      p.transposed = vm ? 0 : 1;
+      if (vm) p.out_y0 = v0;
+      else p.out_x0 = v0;
+      set_terms(p, pl.g_planes, pl.h_planes);
+      tile(p, true, pl.out_n, 128, true);
       p.n_fast = p.M >= p.N; p.band = ft_cdiv(p.M, TILE);
-      const CUtensorMap &pa = vm ? g_mn : h_mn, &pb = vm ? h_mn : g_mn, &po = dw_tma ? dw_out : g_mn;
-      if (two) FT_TRY((launch_gemm<true, EPI_STORE, true, true, true>(ctx, pa, pb, po, p, nullptr)));
-      else FT_TRY((launch_gemm<true, EPI_STORE, true, true, false>(ctx, pa, pb, po, p, nullptr)));
+      const CUtensorMap& po = dw_tma ? dw_out : g_mn;
+      if (two) FT_TRY((launch_gemm<true, EPI_STORE, true, true, true>(ctx, g_mn, h_mn, po, p, nullptr)));
+      else FT_TRY((launch_gemm<true, EPI_STORE, true, true, false>(ctx, g_mn, h_mn, po, p, nullptr)));
     }
   }
   if (t.grad_hidden) {
