@@ -90,7 +90,7 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
   ft_pdl_launch();
   const int r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(rw.head->h_amax, OPERAND_EXP) : 1.f;
+  const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(block_max_of(rw.h_max, AMAX_BLOCKS, redf), OPERAND_EXP) : 1.f;
   int before = 0, all = 0;
   float big = 0.f;
   {
@@ -112,18 +112,19 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
   before = block_sum_int(before, red);
   all = block_sum_int(all, red);
   if (blockIdx.x == 0) {
+    const float wu = sizeof(TO) == 2 && w_scaled ? 1.0f / power_for(block_max_of(rw.w_max, AMAX_BLOCKS, redf), OPERAND_EXP) : 1.0f;
+    __syncthreads();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
     if (lane == 0) redf[warp] = big;
     __syncthreads();
     if (tid == 0) {
       for (int w = 1; w < GATHER_THREADS / 32; ++w) big = fmaxf(big, redf[w]);
-      const float S = power_for(__float_as_int(big), G_EXP);
+      const float S = power_for(big, G_EXP);
       rw.head->count = all;
       rw.head->g_scale = S;
       rw.head->g_unscale = 1.0f / S;
       if constexpr (sizeof(TO) == 2) {
-        const float wu = w_scaled ? 1.0f / power_for(rw.head->w_amax, OPERAND_EXP) : 1.0f;
         rw.head->h_unscale = 1.0f / h_scale;
         rw.head->w_unscale = wu;
         rw.head->z_scale = wu / h_scale;

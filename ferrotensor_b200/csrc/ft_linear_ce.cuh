@@ -14,9 +14,8 @@ constexpr int G_EXP = 14;
 // an f32 operand is brought to the same range before it is split into f16 planes
 constexpr int OPERAND_EXP = 14;
 
-// The power of two that brings the magnitude with these bits into [2^(exp-1), 2^exp).
-__device__ __forceinline__ float power_for(int bits, int exp) {
-  const float amax = __int_as_float(bits);
+// The power of two that brings this magnitude into [2^(exp-1), 2^exp).
+__device__ __forceinline__ float power_for(float amax, int exp) {
   if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
   int e;
   frexpf(amax, &e);
@@ -30,12 +29,29 @@ struct Head {
   float g_unscale;
   float h_scale, h_unscale, w_unscale;   // of the f16 planes of f32 operands, else 1
   float z_scale;      // h_unscale * w_unscale
-  int h_amax, w_amax; // bits of the f32 operands' largest finite magnitudes
 };
+
+// Blocks of k_ce_amax for each operand, and the values that it leaves.
+constexpr int AMAX_BLOCKS = 512;
+
+// The largest of n values, in every thread of a block of 256; `red` holds 8.
+__device__ __forceinline__ float block_max_of(const float* __restrict__ v, int n, float* red) {
+  float m = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, v[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+  return m;
+}
 
 // Per packed row, except where noted.
 struct Rows {
   Head* head;
+  float *h_max, *w_max;   // [AMAX_BLOCKS] largest finite magnitudes of parts of the f32 operands
   int* place;         // [source row] its packed row, -1 for a skipped one
   int* source;        // its row in the caller's tensors
   uint32_t* target;
@@ -82,6 +98,8 @@ class Carver {
 inline Rows carve_rows(Carver& c, int T) {
   Rows r;
   r.head = c.take<Head>(1);
+  r.h_max = c.take<float>(AMAX_BLOCKS);
+  r.w_max = c.take<float>(AMAX_BLOCKS);
   r.place = c.take<int>(T);
   r.source = c.take<int>(T);
   r.target = c.take<uint32_t>(T);

@@ -70,7 +70,7 @@ constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK
 struct TcProduct {
   int M, N, K;
   int live_m, live_k;               // 1: that extent is the number of supervised rows
-  int unpacked;                     // STATS: the rows are the caller's own, all M of them (no head, no scales)
+  int unpacked;                     // STATS, EXP, FACTOR: the rows are the caller's own, all M of them (no head, no scales)
   int carry;                        // STATS: one tile of rows; a pair joins its column tiles before it writes them
   int splits;                       // parts of K, each with a slab of its own
   int tile_n;                       // columns of a tile: a multiple of 32 up to TILE
@@ -87,6 +87,7 @@ struct TcProduct {
   int part_ld;
   int w_early;                      // STATS: W may be read before the launch before this one has ended
   int piece, pieces;                // STATS, EXP: which launch this is, of how many
+  float* base_out;                  // FACTOR: a part of K chooses its own point of reference, [splits][part_ld]
   __half* wy;                       // EXP: the targets' columns of W, [planes][part_ld][wy_ld]
   int wy_ld;
   int v0, vocab;                    // first vocabulary column of the launch, columns in all
@@ -320,7 +321,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
   const uint32_t lead_full = PAIR ? mapa_shared(bar_full, 0) : bar_full;
   const uint32_t lead_tempty = PAIR ? mapa_shared(bar_tempty, 0) : bar_tempty;
-  const bool unpacked = EPI == EPI_STATS && g.unpacked;
+  const bool unpacked = (EPI <= EPI_EXP || EPI == EPI_FACTOR) && g.unpacked;
   const int live = unpacked ? g.M : g.rw.head->count;
   // no supervised row at all still makes one tile (of zeros): gradients are overwritten, not left
   const int tiles_m = g.live_m ? max(1, (live + TM - 1) / TM) : (g.M + TM - 1) / TM;
@@ -450,6 +451,15 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
       } else if constexpr (EPI == EPI_STORE) {
         if (g.unscale) alpha = g.rw.head->g_unscale * g.rw.head->h_unscale;
+      } else if (g.base_out) {
+        float m = -INFINITY;
+        if (row < live) {
+#pragma unroll 8
+          for (int s0 = kb0; s0 < kb1; s0 += SLICE)
+            m = fmaxf(m, g.part[(size_t)(parts_of(EPI_EXP, true) * (s0 / SLICE)) * g.part_ld + row].x);
+          base2 = finite_max(m);
+          if (un.nt == 0 && grp == 0) g.base_out[(size_t)un.sp * g.part_ld + row] = base2;
+        }
       } else {
         if (row < live) base2 = g.rw.base[row];
       }
@@ -777,6 +787,16 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 }
 
 // ------------------------------------------------------------------------------ around the products
+// The loss of a row from its log-sum-exp ref + l2 and its target's logit, as the tensor cores summed it (z)
+// and exactly (z + d), all in log2 units: the sum with that logit replaced,
+//   log(e^(lse - z) + e^d - 1) - d = (lse - z) - d + log(1 + p (e^d - 1)),  p = e^(z - lse)
+// (ref - z) first: a row that is sure of its target loses nothing to the size of its logits.
+__device__ __forceinline__ float loss_of(float ref, float l2, float z, float exact) {
+  const float above = ((ref - z) + l2) * 0.6931471805599453f;
+  const float d = (exact - z) * 0.6931471805599453f;
+  return above - d + log1pf(expf(-above) * expm1f(d));
+}
+
 // Joins the column tiles' {maximum, sum} of 32 rows, tiles over the warps in a fixed order, with what
 // the pieces before (not `first`) have left; after the last piece writes the row's log-sum-exp (in
 // log2 units, as the gradient's epilogue wants it) and its loss.
@@ -838,12 +858,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
         if (!unpacked_rows) rw.lse[row] = ref + l2;
         float loss = 0.f;
         if (rw.target[row] < (uint32_t)vocab) {
-          // the sum with the target's logit z replaced by its exact value z + d:
-          //   loss = log(e^(lse - z) + e^d - 1) - d = (lse - z) - d + log(1 + p (e^d - 1)),  p = e^(z - lse)
-          // (ref - z) first: a row that is sure of its target loses nothing to the size of its logits
-          const float z = rw.picked[row], above = ((ref - z) + l2) * 0.6931471805599453f;
-          const float d = (rw.exact[row] - z) * 0.6931471805599453f;
-          loss = above - d + log1pf(expf(-above) * expm1f(d));
+          loss = loss_of(ref, l2, rw.picked[row], rw.exact[row]);
         }
         row_loss[unpacked_rows ? row : rw.source[row]] = loss;
         if (acc) {
@@ -912,10 +927,12 @@ k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __res
   }
 }
 
-// Largest finite magnitude of W (first `w_blocks` blocks) and of the supervised rows (the others).
+// Largest finite magnitudes of W (first `w_blocks` blocks, AMAX_BLOCKS or none) and of the supervised rows
+// (the others), one value a block.
 __global__ void __launch_bounds__(256)
 k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* __restrict__ hidden,
-          const uint32_t* __restrict__ targets, int rows, int H, Head* __restrict__ head) {
+          const uint32_t* __restrict__ targets, int rows, int H, Rows rw) {
+  __shared__ float red[8];
   ft_pdl_wait();
   ft_pdl_launch();
   float m = 0.f;
@@ -950,18 +967,24 @@ k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* _
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0 && m > 0.f)
-    atomicMax((int)blockIdx.x < w_blocks ? &head->w_amax : &head->h_amax, __float_as_int(m));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 8; ++k) m = fmaxf(m, red[k]);
+    if ((int)blockIdx.x < w_blocks) rw.w_max[blockIdx.x] = m;
+    else rw.h_max[blockIdx.x - w_blocks] = m;
+  }
 }
 
 // W [rows, cols] -> f16 planes [planes][rows][ld], times the power of two of its largest value
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_ce_weight(const T* __restrict__ w, int rows, int cols, __half* __restrict__ out, int ld, int planes,
-            const Head* __restrict__ head) {
+            const float* __restrict__ w_max) {
+  __shared__ float red[8];
   ft_pdl_wait();
   ft_pdl_launch();
-  const float S = sizeof(T) == 4 ? power_for(head->w_amax, OPERAND_EXP) : 1.f;
+  const float S = sizeof(T) == 4 ? power_for(block_max_of(w_max, AMAX_BLOCKS, red), OPERAND_EXP) : 1.f;
   const size_t plane = (size_t)rows * ld;
   // a warp takes 1024 columns of a row
   const int c_end = min(ld, ((int)blockIdx.y + 1) * 1024);
@@ -998,6 +1021,7 @@ k_ce_scatter(const float* __restrict__ acc, size_t slab, int splits, int ld, Row
     if (at >= 0) {
       const float* p = acc + (size_t)at * ld + c;
       v = *(const float4*)p;
+#pragma unroll 4
       for (int s = 1; s < splits; ++s) {
         const float4 x = *(const float4*)(p + s * slab);
         v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
@@ -1038,6 +1062,7 @@ k_ce_scatter_exp(const float* __restrict__ acc, size_t slab, int splits, int ld,
         y[0] = *(const uint2*)(wy + (size_t)at * wy_ld + c);
         if (w_planes == 2) y[1] = *(const uint2*)(wy + wy_plane + (size_t)at * wy_ld + c);
       }
+#pragma unroll 4
       for (int s = 1; s < splits; ++s) {
         const float4 x = *(const float4*)(p + s * slab);
         v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
@@ -1048,6 +1073,115 @@ k_ce_scatter_exp(const float* __restrict__ acc, size_t slab, int splits, int ld,
       e[1] = fmaf(f.x, v.y, f.y * (y0.y + z0.y));
       e[2] = fmaf(f.x, v.z, f.y * (y1.x + z1.x));
       e[3] = fmaf(f.x, v.w, f.y * (y1.y + z1.y));
+    }
+    T* o = out + (size_t)r * H + c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < H) {
+        if constexpr (sizeof(T) == 2) o[k] = __float2half_rn(e[k]);
+        else o[k] = e[k];
+      }
+  }
+}
+
+// All that is left after E W when the vocabulary was one piece: the join of the statistics, the loss and
+// grad_hidden, for four rows a block.  Every part of K has its own point of reference (base, [splits]
+// [part_ld]).  `unpacked` rows are the caller's own, with their targets and weights.
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_ce_finish(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int unpacked, const float* __restrict__ weights,
+            float grad_scale, int vocab, float* __restrict__ row_loss, const float* __restrict__ base,
+            const float* __restrict__ acc, size_t slab, int splits, int ld, const __half* __restrict__ wy, size_t wy_plane,
+            int wy_ld, int w_planes, int H, int rows, T* __restrict__ out) {
+  constexpr int ROWS = 4, MAX_SPLITS = 64;
+  __shared__ float2 red[8][ROWS];
+  __shared__ float factor[ROWS][MAX_SPLITS], onehot[ROWS], lse_of[ROWS], weight_of[ROWS];
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int mine = blockIdx.x * ROWS + (threadIdx.x & 3);            // (source row)
+  int at = -1;
+  if (mine < rows) at = unpacked ? (rw.target[mine] == FT_MASKED_CE_SKIP ? -1 : mine) : rw.place[mine];
+  float m = -INFINITY, s = 0.f;
+  if (at >= 0) {
+    constexpr int AT_ONCE = 8;
+    for (int p0 = threadIdx.x >> 2; p0 < parts; p0 += AT_ONCE * 64) {
+      float2 v[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) v[j] = p0 + 64 * j < parts ? part[(size_t)(p0 + 64 * j) * part_ld + at] : make_float2(-INFINITY, 0.f);
+      float mn = m;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) mn = fmaxf(mn, v[j].x);
+      const float ref = finite_max(mn);
+      s *= ex2(m - ref);
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) s += v[j].y * ex2(v[j].x - ref);
+      m = mn;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 4; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    const float mn = fmaxf(m, m2), ref = finite_max(mn);
+    s = s * ex2(m - ref) + s2 * ex2(m2 - ref);
+    m = mn;
+  }
+  if (lane < ROWS) red[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x < ROWS && mine < rows) {
+    const int i = threadIdx.x;
+    float loss = 0.f;
+    if (at >= 0) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) M = fmaxf(M, red[w][i].x);
+      const float ref = finite_max(M);
+      float S = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) S += red[w][i].y * ex2(red[w][i].x - ref);
+      const float l2 = log2f(S), lse2 = ref + l2;
+      const float w = unpacked ? weights[at] * grad_scale : rw.weight[at] * rw.head->w_unscale;
+      float b = 0.f;
+      if (rw.target[at] < (uint32_t)vocab) {
+        loss = loss_of(ref, l2, rw.picked[at], rw.exact[at]);
+        b = expm1f(-loss) - rw.kept[at].x * ex2(rw.kept[at].y - lse2);
+      }
+      onehot[i] = w * b;
+      lse_of[i] = lse2;
+      weight_of[i] = w;
+    }
+    row_loss[mine] = loss;
+  }
+  __syncthreads();
+  if (at >= 0)
+    for (int sp = threadIdx.x >> 2; sp < splits; sp += 64)
+      factor[threadIdx.x & 3][sp] = weight_of[threadIdx.x & 3] * ex2(base[(size_t)sp * part_ld + at] - lse_of[threadIdx.x & 3]);
+  __syncthreads();
+  // two warps a row
+  const int i = warp >> 1, r = blockIdx.x * ROWS + i;
+  if (r >= rows) return;
+  const int place = __shfl_sync(0xffffffffu, at, i);                 // lane i holds row i
+  const float b = place >= 0 ? onehot[i] : 0.f;
+  for (int c = (warp & 1) * 128 + lane * 4; c < ld; c += 256) {
+    float e[4] = {0.f, 0.f, 0.f, 0.f};
+    if (place >= 0) {
+      uint2 y[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+      // a target outside the vocabulary has no column (wy's pitch is a multiple of 8)
+      if (b != 0.f) {
+        y[0] = *(const uint2*)(wy + (size_t)place * wy_ld + c);
+        if (w_planes == 2) y[1] = *(const uint2*)(wy + wy_plane + (size_t)place * wy_ld + c);
+      }
+      const float* p = acc + (size_t)place * ld + c;
+#pragma unroll 4
+      for (int sp = 0; sp < splits; ++sp) {
+        const float4 x = *(const float4*)(p + sp * slab);
+        const float f = factor[i][sp];
+        e[0] = fmaf(f, x.x, e[0]); e[1] = fmaf(f, x.y, e[1]); e[2] = fmaf(f, x.z, e[2]); e[3] = fmaf(f, x.w, e[3]);
+      }
+      const float2 y0 = __half22float2(*(const __half2*)&y[0].x), y1 = __half22float2(*(const __half2*)&y[0].y);
+      const float2 z0 = __half22float2(*(const __half2*)&y[1].x), z1 = __half22float2(*(const __half2*)&y[1].y);
+      e[0] = fmaf(b, y0.x + z0.x, e[0]); e[1] = fmaf(b, y0.y + z0.y, e[1]);
+      e[2] = fmaf(b, y1.x + z1.x, e[2]); e[3] = fmaf(b, y1.y + z1.y, e[3]);
     }
     T* o = out + (size_t)r * H + c;
 #pragma unroll
@@ -1155,11 +1289,11 @@ struct TcPlan {
   Rows rows;
   __half *h, *w, *grad, *wy;
   float2* part;
-  float* acc;
+  float *acc, *base;
   int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld;
   int stat_n, out_n;         // columns of a tile: of the statistics alone, of dh and (vocab-major) dW
   int tile_m;                // rows of a tile of the products whose rows are the packed ones
-  bool pair, w_staged, by_exp, in_place;   // in_place: g is made of E, see k_ce_normalise
+  bool pair, w_staged, by_exp, one_piece, in_place;   // in_place: g is made of E, see k_ce_normalise
   size_t bytes;
 };
 
@@ -1207,7 +1341,8 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
     // equal pieces of whole tiles
     pl.piece = (int)ft_align_up((size_t)ft_cdiv(q.V, pieces), TILE);
     grad_bytes = column * pl.piece;
-    pl.in_place = two && q.grad_weight && pieces == 1;
+    pl.one_piece = pieces == 1;
+    pl.in_place = two && q.grad_weight && pl.one_piece;
     if (pl.by_exp || pl.in_place) part_bytes = (size_t)parts_of(EPI_EXP, two) * (pl.piece / TILE) * pl.Tp * sizeof(float2);
   }
   if (pl.by_exp || pl.in_place) {
@@ -1222,16 +1357,19 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   }
   pl.splits = 1;
   if (q.grad_hidden) {
-    // K parts: as many as fill the pairs in whole waves, each at least 1024 deep, 256 MB of slabs
+    // K parts: as many as fill the workers in whole waves, each at least 1024 deep, 256 MB of slabs
     pl.acc_ld = (int)ft_align_up((size_t)q.H, 4);
     const long long tiles = (long long)ft_cdiv(q.T, pl.tile_m) * ft_cdiv(q.H, pl.out_n);
     double best = 1e30;
-    for (int s = 1; s <= 64 && s * 1024 <= std::max(1024, pl.piece); ++s) {
+    // (parts of 256 where the tiles alone leave workers idle: a small call is bound by its longest one)
+    const int grains = ft_cdiv(std::min(pl.piece, q.V), pl.by_exp ? TILE : BK);   // of the first piece: it fills every slab
+    for (int s = 1; s <= std::min(64, grains) && s * (tiles * s <= workers ? 256 : 1024) <= std::max(1024, pl.piece); ++s) {
       if (s > 1 && (size_t)s * pl.Tp * pl.acc_ld * 4 > ((size_t)256 << 20)) break;
       const double waves = (double)((tiles * s + workers - 1) / workers) / s;
       if (waves < best * 0.97) { best = waves; pl.splits = s; }
     }
     pl.acc = c.take<float>((size_t)pl.splits * pl.Tp * pl.acc_ld);
+    pl.base = c.take<float>((size_t)pl.splits * pl.Tp);
   }
   pl.bytes = c.bytes();
   return pl;
@@ -1249,14 +1387,13 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   const bool vm = q.p.weight_vocab_major != 0, two = pl.g_planes == 2;
   const bool h32 = q.p.hidden_type == FT_TYPE_F32, w32 = q.p.weight_type == FT_TYPE_F32;
   if (h32 || w32) {
-    FT_CUDA(cudaMemsetAsync(pl.rows.head, 0, sizeof(Head), ctx->stream));
-    const int wb = w32 ? ctx->sm_count * 4 : 0, hb = h32 ? std::min(T, ctx->sm_count * 4) : 0;
+    const int wb = w32 ? AMAX_BLOCKS : 0, hb = h32 ? AMAX_BLOCKS : 0;
     FT_LAUNCH_PDL(ctx, k_ce_amax, wb + hb, 256, 0, (const float*)t.weight, (long long)pl.w_rows * pl.w_cols, wb,
-                  (const float*)t.hidden, t.targets, T, H, pl.rows.head);
+                  (const float*)t.hidden, t.targets, T, H, pl.rows);
   }
-  // One tile of rows, no gradient: packing would save nothing, and a row's statistics are its own
-  // whatever the others hold.
-  const bool unpacked = T <= 128 && !t.grad_hidden && !t.grad_weight && !h32 && !w32 && H % 8 == 0 &&
+  // One tile of rows and no dW: packing would save nothing, and what a row gets is its own whatever the
+  // others hold.
+  const bool unpacked = T <= 128 && !t.grad_weight && (!t.grad_hidden || pl.one_piece) && !h32 && !w32 && H % 8 == 0 &&
                         ((uintptr_t)t.hidden & 15) == 0;
   if (!unpacked) FT_TRY(launch_gather_f16(ctx, q, t, pl.rows, pl.h, pl.h_ld, pl.Tp, pl.h_planes));
   const void* w = t.weight;
@@ -1265,10 +1402,10 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     const dim3 grid((unsigned)std::min(ft_cdiv(pl.w_rows, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(pl.w_ld, 1024));
     if (w32)
       FT_LAUNCH_PDL(ctx, k_ce_weight<float>, grid, 256, 0, (const float*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
-                    pl.w_planes, pl.rows.head);
+                    pl.w_planes, pl.rows.w_max);
     else
       FT_LAUNCH_PDL(ctx, k_ce_weight<__half>, grid, 256, 0, (const __half*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
-                    pl.w_planes, pl.rows.head);
+                    pl.w_planes, pl.rows.w_max);
   }
   // K-contiguous operands come in boxes of 64 x 128 rows (B: half a tile's columns), M/N-contiguous ones
   // in two of 64 x 64
@@ -1325,6 +1462,8 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.k0 = v0; p.b_has_k0 = 1;
     p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
     p.part = pl.part; p.part_ld = pl.Tp;
+    p.unpacked = unpacked ? 1 : 0;
+    p.base_out = pl.by_exp && pl.one_piece ? pl.base : nullptr;
     tile(p, pl.pair, pl.out_n, a_rows, vm);
     return p;
   };
@@ -1337,11 +1476,25 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       const bool first = v0 == 0, last = v0 + cols == V;
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
-      FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two) * ft_cdiv(cols, TILE), pl.rows, 0, first ? 1 : 0,
-                    last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
+      if (!pl.one_piece)
+        FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two) * ft_cdiv(cols, TILE),
+                      pl.rows, 0, first ? 1 : 0, last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
       if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       const TcProduct p = dh_product(v0, cols);
       FT_TRY(launch_rows<EPI_FACTOR>(ctx, pl.pair, vm, two, g_k, vm ? w_mn : w_k, acc_out, p));
+    }
+    if (pl.one_piece) {
+      const int parts = parts_of(EPI_EXP, two) * ft_cdiv(V, TILE), grid = ft_cdiv(T, 4);
+      const size_t plane = (size_t)pl.Tp * pl.h_ld;
+      if (q.p.grad_hidden_type == FT_TYPE_F16)
+        FT_LAUNCH_PDL(ctx, k_ce_finish<__half>, grid, 256, 0, pl.part, pl.Tp, parts, z.rw, unpacked ? 1 : 0, t.weights,
+                      q.p.grad_scale, V, t.row_loss, pl.base, pl.acc, slab, pl.splits, pl.acc_ld, pl.wy, plane, pl.h_ld,
+                      pl.w_planes, H, T, (__half*)t.grad_hidden);
+      else
+        FT_LAUNCH_PDL(ctx, k_ce_finish<float>, grid, 256, 0, pl.part, pl.Tp, parts, z.rw, unpacked ? 1 : 0, t.weights,
+                      q.p.grad_scale, V, t.row_loss, pl.base, pl.acc, slab, pl.splits, pl.acc_ld, pl.wy, plane, pl.h_ld,
+                      pl.w_planes, H, T, (float*)t.grad_hidden);
+      return FT_OK;
     }
     if (q.p.grad_hidden_type == FT_TYPE_F16)
       FT_LAUNCH_PDL(ctx, k_ce_scatter_exp<__half>, unpack_grid, 256, 0, pl.acc, slab, pl.splits, pl.acc_ld, pl.rows, pl.wy,
