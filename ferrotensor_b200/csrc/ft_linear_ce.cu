@@ -28,17 +28,6 @@ using namespace ft_ce;
 // ------------------------------------------------------------------------------ row bookkeeping
 constexpr int GATHER_THREADS = 256;
 
-__device__ __forceinline__ int block_sum_int(int v, int* red) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int s = 0;
-#pragma unroll
-  for (int w = 0; w < GATHER_THREADS / 32; ++w) s += red[w];
-  return s;
-}
-
 // One row -> f16 (and its rounding remainder, when `lo` is given), eight values a lane.
 template <typename TH>
 __device__ __forceinline__ void pack_row(const TH* __restrict__ from, int H, float S, __half* __restrict__ hi, int ld,
@@ -83,17 +72,23 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
             const float* __restrict__ weights, float grad_scale, int rows, int H, int per, Rows rw,
             TO* __restrict__ out, int ld, int plane_rows, int planes, int w_scaled,
             float* __restrict__ row_loss) {
-  __shared__ int red[GATHER_THREADS / 32];
-  __shared__ float redf[GATHER_THREADS / 32];
+  constexpr int WARPS = GATHER_THREADS / 32;
+  __shared__ int red[WARPS], counts[2][WARPS];
+  __shared__ float tops[3][WARPS];
   __shared__ int src_row[GATHER_THREADS];
   ft_pdl_wait();
   ft_pdl_launch();
   const int r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(block_max_of(rw.h_max, AMAX_BLOCKS, redf), OPERAND_EXP) : 1.f;
+  // What has to be known of the whole batch, every thread's share first: all loads are under way
+  // before the one join.
   int before = 0, all = 0;
-  float big = 0.f;
+  float big = 0.f, h_top = 0.f, w_top = 0.f;   // of |s w_t|, of the operands
   {
+    if (sizeof(TO) == 2 && sizeof(TH) == 4)
+      for (int i = tid; i < AMAX_BLOCKS; i += GATHER_THREADS) h_top = fmaxf(h_top, rw.h_max[i]);
+    if (sizeof(TO) == 2 && w_scaled && blockIdx.x == 0)
+      for (int i = tid; i < AMAX_BLOCKS; i += GATHER_THREADS) w_top = fmaxf(w_top, rw.w_max[i]);
     auto count = [&](int i, uint32_t y) {
       const int one = y != FT_MASKED_CE_SKIP;
       all += one;
@@ -106,29 +101,41 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
     }
     for (int i = 4 * vec + tid; i < rows; i += GATHER_THREADS) count(i, targets[i]);
     if (blockIdx.x == 0 && weights)
-      for (int i = tid; i < rows; i += GATHER_THREADS)
-        if (targets[i] != FT_MASKED_CE_SKIP) big = fmaxf(big, fabsf(weights[i] * grad_scale));
-  }
-  before = block_sum_int(before, red);
-  all = block_sum_int(all, red);
-  if (blockIdx.x == 0) {
-    const float wu = sizeof(TO) == 2 && w_scaled ? 1.0f / power_for(block_max_of(rw.w_max, AMAX_BLOCKS, redf), OPERAND_EXP) : 1.0f;
-    __syncthreads();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-    if (lane == 0) redf[warp] = big;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < GATHER_THREADS / 32; ++w) big = fmaxf(big, redf[w]);
-      const float S = power_for(big, G_EXP);
-      rw.head->count = all;
-      rw.head->g_scale = S;
-      rw.head->g_unscale = 1.0f / S;
-      if constexpr (sizeof(TO) == 2) {
-        rw.head->h_unscale = 1.0f / h_scale;
-        rw.head->w_unscale = wu;
-        rw.head->z_scale = wu / h_scale;
+      for (int i = tid; i < rows; i += GATHER_THREADS) {
+        const float w = fabsf(weights[i] * grad_scale);
+        if (targets[i] != FT_MASKED_CE_SKIP) big = fmaxf(big, w);
       }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      h_top = fmaxf(h_top, __shfl_xor_sync(0xffffffffu, h_top, o));
+      w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
+    }
+    if (lane == 0) {
+      counts[0][warp] = before; counts[1][warp] = all;
+      tops[0][warp] = big; tops[1][warp] = h_top; tops[2][warp] = w_top;
+    }
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      before += counts[0][w]; all += counts[1][w];
+      big = fmaxf(big, tops[0][w]); h_top = fmaxf(h_top, tops[1][w]); w_top = fmaxf(w_top, tops[2][w]);
+    }
+  }
+  const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(h_top, OPERAND_EXP) : 1.f;
+  if (blockIdx.x == 0 && tid == 0) {
+    const float S = power_for(big, G_EXP);
+    rw.head->count = all;
+    rw.head->g_scale = S;
+    rw.head->g_unscale = 1.0f / S;
+    if constexpr (sizeof(TO) == 2) {
+      const float wu = w_scaled ? 1.0f / power_for(w_top, OPERAND_EXP) : 1.0f;
+      rw.head->h_unscale = 1.0f / h_scale;
+      rw.head->w_unscale = wu;
+      rw.head->z_scale = wu / h_scale;
     }
   }
   int at = before;
@@ -142,7 +149,7 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
     __syncthreads();
     int mine = __popc(mask & ((1u << lane) - 1u)), total = 0;
 #pragma unroll
-    for (int w = 0; w < GATHER_THREADS / 32; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) mine += red[w];
       total += red[w];
     }

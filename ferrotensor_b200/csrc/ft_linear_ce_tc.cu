@@ -50,20 +50,22 @@ enum Epi { EPI_STATS, EPI_EXP, EPI_GRAD, EPI_STORE, EPI_FACTOR };
 // The statistics bound small K (a tile takes eight warps 6100 cycles, sixteen 4400, the products 512
 // for each 64 of K).  Where results are staged or slices summed, sixteen cost a stage or spills:
 // eight there (8 x 4 KiB beside six stages; g at K = 2048 takes 412 thousand cycles, with sixteen and
-// five stages 419).
-constexpr int drain_warps(int epi, bool two) { return epi == EPI_FACTOR || (epi == EPI_STATS && !two) ? 16 : 8; }
+// five stages 419).  With at most 128 rows (single CTAs) nothing is bound by the products: sixteen.
+constexpr int drain_warps(int epi, bool two, bool pair) { return !pair || epi == EPI_FACTOR || (epi == EPI_STATS && !two) ? 16 : 8; }
 // Statistics of a row that a tile leaves: one a warp of its quadrant.
-constexpr int parts_of(int epi, bool two) { return drain_warps(epi, two) / 4; }
+constexpr int parts_of(int epi, bool two, bool pair) { return drain_warps(epi, two, pair) / 4; }
 // The statistics' launches have two warps more, for the targets' logits.
-constexpr int threads_of(int epi, bool two) { return 64 + 32 * drain_warps(epi, two) + (epi <= EPI_EXP ? 64 : 0); }
+constexpr int threads_of(int epi, bool two, bool pair) { return 64 + 32 * drain_warps(epi, two, pair) + (epi <= EPI_EXP ? 64 : 0); }
 // Shared memory: the stages (six, or five, of 32 KiB; more where few rows or narrow tiles make them
 // smaller), 4 KiB for each draining warp that stages results, the barriers (full, empty, tfull, tempty,
 // one a quadrant), and room to align all that.
 constexpr int MAX_STAGES = 16;
-constexpr int epi_offset(int epi) { return (epi == EPI_FACTOR ? 5 : 6) * STAGE_BYTES; }
-constexpr int bar_offset(int epi, bool two) { return epi_offset(epi) + (epi == EPI_STATS ? 16384 : drain_warps(epi, two) * 4096); }
+constexpr int epi_offset(int epi, bool pair) { return (epi == EPI_STATS || (pair && epi != EPI_FACTOR) ? 6 : 5) * STAGE_BYTES; }
+constexpr int bar_offset(int epi, bool two, bool pair) {
+  return epi_offset(epi, pair) + (epi == EPI_STATS ? 16384 : drain_warps(epi, two, pair) * 4096);
+}
 constexpr int BARRIERS = 2 * MAX_STAGES + 2 * MAX_BUFFERS + 4;
-constexpr int smem_bytes(int epi, bool two) { return bar_offset(epi, two) + BARRIERS * 8 + 16 + 1024; }
+constexpr int smem_bytes(int epi, bool two, bool pair) { return bar_offset(epi, two, pair) + BARRIERS * 8 + 16 + 1024; }
 // k-blocks of 64 that are summed in tensor memory; 0: all
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
 
@@ -142,6 +144,8 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // the staging tile may be written again: the copies have read it
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// ... all copies but the last have
+__device__ __forceinline__ void bulk_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -253,11 +257,11 @@ __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, 
 }
 
 template <bool PAIR, int EPI, bool A_MN, bool B_MN, bool TWO>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(threads_of(EPI, TWO), 1)
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(threads_of(EPI, TWO, PAIR), 1)
 k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcProduct g, int* status) {
-  constexpr int WARPS = drain_warps(EPI, TWO), PARTS = parts_of(EPI, TWO);
-  constexpr int EPI_OFFSET = epi_offset(EPI), BAR_OFFSET = bar_offset(EPI, TWO);
+  constexpr int WARPS = drain_warps(EPI, TWO, PAIR), PARTS = parts_of(EPI, TWO, PAIR);
+  constexpr int EPI_OFFSET = epi_offset(EPI, PAIR), BAR_OFFSET = bar_offset(EPI, TWO, PAIR);
   constexpr int CHUNKS = 32 / WARPS;        // of 32 columns, at most, a draining warp
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -456,7 +460,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (row < live) {
 #pragma unroll 8
           for (int s0 = kb0; s0 < kb1; s0 += SLICE)
-            m = fmaxf(m, g.part[(size_t)(parts_of(EPI_EXP, true) * (s0 / SLICE)) * g.part_ld + row].x);
+            m = fmaxf(m, g.part[(size_t)(parts_of(EPI_EXP, false, PAIR) * (s0 / SLICE)) * g.part_ld + row].x);
           base2 = finite_max(m);
           if (un.nt == 0 && grp == 0) g.base_out[(size_t)un.sp * g.part_ld + row] = base2;
         }
@@ -575,50 +579,24 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (c0 >= g.N || y0 >= rows_end) return;                 // the whole block lies outside
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] *= alpha;
-          if (g.direct != nullptr && g.transposed) {
-            // a lane is a column of the output: 32 consecutive ones a store
-            if (row < rows_end) {
+          if (g.direct != nullptr) {
+            // a pitch or a base that TMA cannot address
+            if (g.transposed) {
+              // a lane is a column of the output: 32 consecutive ones a store
+              if (row < rows_end) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const long long at = (long long)(c0 + k) * g.direct_ld + g.out_x0 + row;
-                if (c0 + k >= g.N) break;
-                if (g.out_type == FT_TYPE_F16) ((__half*)g.direct)[at] = __float2half_rn(v[k]);
-                else ((float*)g.direct)[at] = v[k];
+                for (int k = 0; k < 32; ++k) {
+                  const long long at = (long long)(c0 + k) * g.direct_ld + g.out_x0 + row;
+                  if (c0 + k >= g.N) break;
+                  if (g.out_type == FT_TYPE_F16) ((__half*)g.direct)[at] = __float2half_rn(v[k]);
+                  else ((float*)g.direct)[at] = v[k];
+                }
               }
+              return;
             }
-            return;
-          }
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
-          if (g.transposed) {
-            // the block turned over: output row k in staging row k, this lane's value in column `lane`
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              if (g.out_type == FT_TYPE_F16) *(__half*)(st + k * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __float2half_rn(v[k]);
-              else *(float*)(st + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4) = v[k];
-            }
-          } else if (g.direct == nullptr && g.out_type == FT_TYPE_F16) {
-            uint32_t h[16];
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) h[k >> 1] = pack_h2(v[k], v[k + 1]);
-            // 32 columns are 64 bytes: a tile of its own swizzle (64-byte rows)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *(uint4*)(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
-          } else {
-            stage_f32(st, lane, v);
-          }
-          if (g.direct == nullptr) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            // a row at a time, a column a lane
             __syncwarp();
-            if (lane == 0) {
-              const int x = g.out_x0 + (g.transposed ? y0 : c0), y = g.out_y0 + (g.transposed ? c0 : y0);
-              if (g.accumulate) tma_add_3d(&map_o, st_addr, x, y, un.sp);
-              else tma_store_3d(&map_o, st_addr, x, y, un.sp);
-              bulk_commit();
-            }
-          } else {
-            // a pitch or a base that TMA cannot address: a row at a time, a column a lane
+            stage_f32(st, lane, v);
             __syncwarp();
             if (c0 + lane < g.N) {
               for (int r = 0; r < 32 && y0 + r < rows_end; ++r) {
@@ -628,7 +606,40 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 else ((float*)g.direct)[at] = x;
               }
             }
-            __syncwarp();
+            return;
+          }
+          // an f16 block fills half of the staging tile: the halves take turns
+          uint8_t* to = st + (g.out_type == FT_TYPE_F16 ? (i & 1) * 2048 : 0);
+          if (lane == 0) {
+            if (g.out_type == FT_TYPE_F16) bulk_wait_read_but_one();
+            else bulk_wait_read();
+          }
+          __syncwarp();
+          if (g.transposed) {
+            // the block turned over: output row k in staging row k, this lane's value in column `lane`
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              if (g.out_type == FT_TYPE_F16) *(__half*)(to + k * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __float2half_rn(v[k]);
+              else *(float*)(to + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4) = v[k];
+            }
+          } else if (g.out_type == FT_TYPE_F16) {
+            uint32_t h[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) h[k >> 1] = pack_h2(v[k], v[k + 1]);
+            // 32 columns are 64 bytes: a tile of its own swizzle (64-byte rows)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *(uint4*)(to + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+          } else {
+            stage_f32(to, lane, v);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            const int x = g.out_x0 + (g.transposed ? y0 : c0), y = g.out_y0 + (g.transposed ? c0 : y0);
+            if (g.accumulate) tma_add_3d(&map_o, smem_u32(to), x, y, un.sp);
+            else tma_store_3d(&map_o, smem_u32(to), x, y, un.sp);
+            bulk_commit();
           }
         }
       };
@@ -682,7 +693,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               // ahead, kept each at 3900 cycles (390 us for the product above)
 #pragma unroll 4
               for (int j = 0; j < 32 && s0 + SLICE * j < kb1; ++j) {
-                const float m = row < live ? g.part[(size_t)(parts_of(EPI_EXP, true) * (s0 / SLICE + j)) * g.part_ld + row].x : 0.f;
+                const float m = row < live ? g.part[(size_t)(parts_of(EPI_EXP, false, PAIR) * (s0 / SLICE + j)) * g.part_ld + row].x : 0.f;
                 // (a difference of two infinities belongs to a row of NaN anyway)
                 factors[j * 32 + lane] = ex2(finite_max(m) - base2);
               }
@@ -888,7 +899,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
 // the cheaper way.  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
 __global__ void __launch_bounds__(256)
 k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __restrict__ part, int part_ld, Rows rw, int cols,
-               const float* __restrict__ row_loss) {
+               int tile_parts, const float* __restrict__ row_loss) {
   ft_pdl_wait();
   ft_pdl_launch();
   const int live = rw.head->count, end = max(64, (live + 63) / 64 * 64);
@@ -905,7 +916,7 @@ k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __res
       __half* p = e + (size_t)r * ld + c;
       uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
       if (r < live) {
-        const float f = w * ex2(finite_max(part[(size_t)(parts_of(EPI_EXP, true) * (c / TILE)) * part_ld + r].x) - lse2);
+        const float f = w * ex2(finite_max(part[(size_t)(tile_parts * (c / TILE)) * part_ld + r].x) - lse2);
         hi = *(const uint4*)p;
         lo = *(const uint4*)(p + plane);
         uint32_t* a = (uint32_t*)&hi;
@@ -1004,6 +1015,26 @@ k_ce_weight(const T* __restrict__ w, int rows, int cols, __half* __restrict__ ou
   }
 }
 
+// Four columns of a row over the slabs, in their order, each times its factor (none: 1); eight loads at
+// once, since small calls have many slabs and little else to wait for.
+__device__ __forceinline__ float4 sum_slabs(const float* __restrict__ p, size_t slab, int splits, const float* factor) {
+  constexpr int AT_ONCE = 8;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < splits; s0 += AT_ONCE) {
+    float4 x[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      if (s0 + j < splits) x[j] = *(const float4*)(p + (s0 + j) * slab);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      if (s0 + j < splits) {
+        const float f = factor ? factor[s0 + j] : 1.f;
+        v.x = fmaf(f, x[j].x, v.x); v.y = fmaf(f, x[j].y, v.y); v.z = fmaf(f, x[j].z, v.z); v.w = fmaf(f, x[j].w, v.w);
+      }
+  }
+  return v;
+}
+
 // grad_hidden[r] = unscale * (sum of the splits' slabs) at the row's packed place, zero where skipped
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -1011,21 +1042,15 @@ k_ce_scatter(const float* __restrict__ acc, size_t slab, int splits, int ld, Row
   ft_pdl_wait();
   ft_pdl_launch();
   const float alpha = rw.head->g_unscale * rw.head->w_unscale;
-  // a warp takes 256 columns of a row
-  const int c_end = min(ld, ((int)blockIdx.y + 1) * 256);
-  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
-#pragma unroll
-  for (int c = blockIdx.y * 256 + (threadIdx.x % 32) * 4; c < c_end; c += 128) {
+  // a warp takes 128 columns of a row
+  const int c = blockIdx.y * 128 + (threadIdx.x % 32) * 4;
+  if (c >= ld) return;
+  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8) {
     const int at = rw.place[r];
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (at >= 0) {
       const float* p = acc + (size_t)at * ld + c;
-      v = *(const float4*)p;
-#pragma unroll 4
-      for (int s = 1; s < splits; ++s) {
-        const float4 x = *(const float4*)(p + s * slab);
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-      }
+      v = sum_slabs(p, slab, splits, nullptr);
     }
     T* o = out + (size_t)r * H + c;
     const float e[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
@@ -1045,27 +1070,21 @@ k_ce_scatter_exp(const float* __restrict__ acc, size_t slab, int splits, int ld,
                  size_t wy_plane, int wy_ld, int w_planes, int H, int rows, T* __restrict__ out) {
   ft_pdl_wait();
   ft_pdl_launch();
-  // a warp takes 256 columns of a row
-  const int c_end = min(ld, ((int)blockIdx.y + 1) * 256);
-  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
-#pragma unroll
-  for (int c = blockIdx.y * 256 + (threadIdx.x % 32) * 4; c < c_end; c += 128) {
+  // a warp takes 128 columns of a row
+  const int c = blockIdx.y * 128 + (threadIdx.x % 32) * 4;
+  if (c >= ld) return;
+  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8) {
     const int at = rw.place[r];
     float e[4] = {0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
       const float2 f = rw.stat[at];
       const float* p = acc + (size_t)at * ld + c;
-      float4 v = *(const float4*)p;
+      const float4 v = sum_slabs(p, slab, splits, nullptr);
       uint2 y[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
       // a target outside the vocabulary has no column (wy's pitch is a multiple of 8)
       if (f.y != 0.f) {
         y[0] = *(const uint2*)(wy + (size_t)at * wy_ld + c);
         if (w_planes == 2) y[1] = *(const uint2*)(wy + wy_plane + (size_t)at * wy_ld + c);
-      }
-#pragma unroll 4
-      for (int s = 1; s < splits; ++s) {
-        const float4 x = *(const float4*)(p + s * slab);
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
       }
       const float2 y0 = __half22float2(*(const __half2*)&y[0].x), y1 = __half22float2(*(const __half2*)&y[0].y);
       const float2 z0 = __half22float2(*(const __half2*)&y[1].x), z1 = __half22float2(*(const __half2*)&y[1].y);
@@ -1150,19 +1169,19 @@ k_ce_finish(const float2* __restrict__ part, int part_ld, int parts, Rows rw, in
       lse_of[i] = lse2;
       weight_of[i] = w;
     }
-    row_loss[mine] = loss;
+    if (blockIdx.y == 0) row_loss[mine] = loss;
   }
   __syncthreads();
   if (at >= 0)
     for (int sp = threadIdx.x >> 2; sp < splits; sp += 64)
       factor[threadIdx.x & 3][sp] = weight_of[threadIdx.x & 3] * ex2(base[(size_t)sp * part_ld + at] - lse_of[threadIdx.x & 3]);
   __syncthreads();
-  // two warps a row
+  // two warps a row, 256 columns a block of grid.y (which has the rows' numbers from its own join)
   const int i = warp >> 1, r = blockIdx.x * ROWS + i;
   if (r >= rows) return;
   const int place = __shfl_sync(0xffffffffu, at, i);                 // lane i holds row i
   const float b = place >= 0 ? onehot[i] : 0.f;
-  for (int c = (warp & 1) * 128 + lane * 4; c < ld; c += 256) {
+  for (int c = (blockIdx.y * 2 + (warp & 1)) * 128 + lane * 4; c < ld; c += gridDim.y * 256) {
     float e[4] = {0.f, 0.f, 0.f, 0.f};
     if (place >= 0) {
       uint2 y[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
@@ -1171,17 +1190,11 @@ k_ce_finish(const float2* __restrict__ part, int part_ld, int parts, Rows rw, in
         y[0] = *(const uint2*)(wy + (size_t)place * wy_ld + c);
         if (w_planes == 2) y[1] = *(const uint2*)(wy + wy_plane + (size_t)place * wy_ld + c);
       }
-      const float* p = acc + (size_t)place * ld + c;
-#pragma unroll 4
-      for (int sp = 0; sp < splits; ++sp) {
-        const float4 x = *(const float4*)(p + sp * slab);
-        const float f = factor[i][sp];
-        e[0] = fmaf(f, x.x, e[0]); e[1] = fmaf(f, x.y, e[1]); e[2] = fmaf(f, x.z, e[2]); e[3] = fmaf(f, x.w, e[3]);
-      }
+      const float4 v = sum_slabs(acc + (size_t)place * ld + c, slab, splits, factor[i]);
       const float2 y0 = __half22float2(*(const __half2*)&y[0].x), y1 = __half22float2(*(const __half2*)&y[0].y);
       const float2 z0 = __half22float2(*(const __half2*)&y[1].x), z1 = __half22float2(*(const __half2*)&y[1].y);
-      e[0] = fmaf(b, y0.x + z0.x, e[0]); e[1] = fmaf(b, y0.y + z0.y, e[1]);
-      e[2] = fmaf(b, y1.x + z1.x, e[2]); e[3] = fmaf(b, y1.y + z1.y, e[3]);
+      e[0] = fmaf(b, y0.x + z0.x, v.x); e[1] = fmaf(b, y0.y + z0.y, v.y);
+      e[2] = fmaf(b, y1.x + z1.x, v.z); e[3] = fmaf(b, y1.y + z1.y, v.w);
     }
     T* o = out + (size_t)r * H + c;
 #pragma unroll
@@ -1224,11 +1237,11 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   static bool ready[FT_MAX_DEVICES] = {};
   static int most[FT_MAX_DEVICES] = {};
   if (!ready[ctx->device]) {
-    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(EPI, TWO)));
+    FT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(EPI, TWO, PAIR)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctx->sm_count / CTAS * CTAS));
-    cfg.blockDim = dim3(threads_of(EPI, TWO));
-    cfg.dynamicSmemBytes = smem_bytes(EPI, TWO);
+    cfg.blockDim = dim3(threads_of(EPI, TWO, PAIR));
+    cfg.dynamicSmemBytes = smem_bytes(EPI, TWO, PAIR);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = CTAS; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
@@ -1245,7 +1258,7 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
   const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
                                 A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
-  cudaError_t e = ft_launch_ex(ctx, kernel, CTAS * workers, threads_of(EPI, TWO), smem_bytes(EPI, TWO), a, b, o, g, ctx->status_dev);
+  cudaError_t e = ft_launch_ex(ctx, kernel, CTAS * workers, threads_of(EPI, TWO, PAIR), smem_bytes(EPI, TWO, PAIR), a, b, o, g, ctx->status_dev);
   if (ctx->profile_all) ft_prof_end(ctx);
   ctx->launches++;
   if (e == cudaSuccess) e = cudaPeekAtLastError();
@@ -1333,7 +1346,7 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   // few row tiles: the columns of a tile follow the number of waves (the last one may be nearly empty)
   pl.stat_n = q.T <= 2 * TILE && !pl.by_exp ? pick_tile_n(q.V, ft_cdiv(q.T, pl.tile_m), workers) : TILE;
   pl.out_n = pick_tile_n(q.H, 1 << 20, workers);
-  size_t part_bytes = (size_t)parts_of(EPI_STATS, two) * ft_cdiv(q.V, pl.stat_n) * pl.Tp * sizeof(float2), grad_bytes = 0;
+  size_t part_bytes = (size_t)parts_of(EPI_STATS, two, pl.pair) * ft_cdiv(q.V, pl.stat_n) * pl.Tp * sizeof(float2), grad_bytes = 0;
   if (q.grad_hidden || q.grad_weight) {
     const size_t column = (size_t)pl.Tp * 2 * pl.g_planes;
     size_t cols = q.p.vocab_piece ? q.p.vocab_piece : std::max<size_t>(TILE, G_PIECE_BYTES / column);
@@ -1343,7 +1356,7 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
     grad_bytes = column * pl.piece;
     pl.one_piece = pieces == 1;
     pl.in_place = two && q.grad_weight && pl.one_piece;
-    if (pl.by_exp || pl.in_place) part_bytes = (size_t)parts_of(EPI_EXP, two) * (pl.piece / TILE) * pl.Tp * sizeof(float2);
+    if (pl.by_exp || pl.in_place) part_bytes = (size_t)parts_of(EPI_EXP, two, pl.pair) * (pl.piece / TILE) * pl.Tp * sizeof(float2);
   }
   if (pl.by_exp || pl.in_place) {
     pl.part = (float2*)c.take<char>(part_bytes);
@@ -1446,7 +1459,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   const int join_grid = ft_cdiv(T, 32), join_threads = T <= 1024 ? 32 * JOIN_WARPS : 256;
   CUtensorMap acc_out;
   if (t.grad_hidden) FT_TRY(make_map3(ctx, &acc_out, pl.acc, true, pl.acc_ld, pl.Tp, pl.splits, pl.acc_ld, 32, 32));
-  const dim3 unpack_grid((unsigned)std::min(ft_cdiv(T, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(std::max(pl.acc_ld, 1), 256));
+  const dim3 unpack_grid((unsigned)std::min(ft_cdiv(T, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(std::max(pl.acc_ld, 1), 128));
   CUtensorMap g_out, g_k;
   if (t.grad_hidden || t.grad_weight)
     FT_TRY(make_map3(ctx, &g_out, pl.grad, false, pl.piece, pl.Tp, pl.g_planes, pl.piece, 64, 32));
@@ -1477,14 +1490,15 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
       if (!pl.one_piece)
-        FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two) * ft_cdiv(cols, TILE),
+        FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(cols, TILE),
                       pl.rows, 0, first ? 1 : 0, last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
       if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       const TcProduct p = dh_product(v0, cols);
       FT_TRY(launch_rows<EPI_FACTOR>(ctx, pl.pair, vm, two, g_k, vm ? w_mn : w_k, acc_out, p));
     }
     if (pl.one_piece) {
-      const int parts = parts_of(EPI_EXP, two) * ft_cdiv(V, TILE), grid = ft_cdiv(T, 4);
+      const int parts = parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(V, TILE), across = T <= 32 ? ft_cdiv(pl.acc_ld, 256) : 1;
+      const dim3 grid((unsigned)ft_cdiv(T, 4), (unsigned)across);
       const size_t plane = (size_t)pl.Tp * pl.h_ld;
       if (q.p.grad_hidden_type == FT_TYPE_F16)
         FT_LAUNCH_PDL(ctx, k_ce_finish<__half>, grid, 256, 0, pl.part, pl.Tp, parts, z.rw, unpacked ? 1 : 0, t.weights,
@@ -1509,11 +1523,11 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     tile(z, pl.pair, TILE, a_rows, !vm);
     if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(TILE)));
     FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
-    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two) * ft_cdiv(V, TILE), pl.rows,
+    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(V, TILE), pl.rows,
                   0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
     const dim3 grid(ft_cdiv(V, 2048), std::max(1, std::min(pl.Tp, ctx->sm_count * 32 / ft_cdiv(V, 2048))));
     FT_LAUNCH_PDL(ctx, k_ce_normalise, grid, 256, 0, pl.grad, (size_t)pl.Tp * pl.piece, pl.piece, pl.part, pl.Tp, pl.rows, pl.piece,
-                  t.row_loss);
+                  parts_of(EPI_EXP, two, pl.pair), t.row_loss);
   } else {
     tile(z, pl.pair, pl.stat_n, a_rows, !vm);
     z.w_early = !pl.w_staged;
@@ -1522,7 +1536,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(pl.stat_n)));
     FT_TRY(launch_rows<EPI_STATS>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, h_k, z, &workers));
     FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp,
-                  parts_of(EPI_STATS, two) * (z.carry ? workers : ft_cdiv(V, pl.stat_n)), z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss,
+                  parts_of(EPI_STATS, two, pl.pair) * (z.carry ? workers : ft_cdiv(V, pl.stat_n)), z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss,
                   (float*)nullptr, (size_t)0, 0, 0, 0);
   }
   if (!t.grad_hidden && !t.grad_weight) return FT_OK;
