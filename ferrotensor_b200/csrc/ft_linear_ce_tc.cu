@@ -1370,16 +1370,24 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
   }
   pl.splits = 1;
   if (q.grad_hidden) {
-    // K parts: as many as fill the workers in whole waves, each at least 1024 deep, 256 MB of slabs
+    // Parts of K, by what they should take: rounds of tiles at the workers' rate and 2 us each to fill and
+    // drain, and the slabs written and read once more (1225 x 575 x 50021: as many as fit 256 MB were
+    // 57, and 97 us for dh and its unpacking where 9 take 82).  How many rows are supervised is not
+    // known here: the sum of the times for all of them and for half (4096 rows, 2048 of them
+    // supervised: 4% of the whole call between the best number for 4096 and this one).
     pl.acc_ld = (int)ft_align_up((size_t)q.H, 4);
-    const long long tiles = (long long)ft_cdiv(q.T, pl.tile_m) * ft_cdiv(q.H, pl.out_n);
-    double best = 1e30;
-    // (parts of 256 where the tiles alone leave workers idle: a small call is bound by its longest one)
+    const double rate = 1.2e9 / (pl.pair ? 74 : 148);              // flops of a worker in a microsecond
+    const double tile_us = 2.0 * pl.tile_m * pl.out_n * std::min(pl.piece, q.V) * (pl.g_planes + pl.w_planes - 1) / rate;
     const int grains = ft_cdiv(std::min(pl.piece, q.V), pl.by_exp ? TILE : BK);   // of the first piece: it fills every slab
-    for (int s = 1; s <= std::min(64, grains) && s * (tiles * s <= workers ? 256 : 1024) <= std::max(1024, pl.piece); ++s) {
-      if (s > 1 && (size_t)s * pl.Tp * pl.acc_ld * 4 > ((size_t)256 << 20)) break;
-      const double waves = (double)((tiles * s + workers - 1) / workers) / s;
-      if (waves < best * 0.97) { best = waves; pl.splits = s; }
+    auto cost = [&](int rows, int s) {
+      const int row_tiles = ft_cdiv(std::max(rows, 1), pl.tile_m);
+      const long long units = (long long)row_tiles * ft_cdiv(q.H, pl.out_n) * s;
+      return (double)((units + workers - 1) / workers) * (tile_us / s + 2.0) + 2.0 * s * row_tiles * pl.tile_m * pl.acc_ld * 4.0 / 4e6;
+    };
+    double best = 1e30;
+    for (int s = 1; s <= std::min(64, grains); ++s) {
+      const double us = cost(q.T, s) + cost(q.T / 2, s);
+      if (us < best) { best = us; pl.splits = s; }
     }
     pl.acc = c.take<float>((size_t)pl.splits * pl.Tp * pl.acc_ld);
     pl.base = c.take<float>((size_t)pl.splits * pl.Tp);
@@ -1456,7 +1464,8 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   z.wy = pl.wy; z.wy_ld = pl.h_ld;
   z.pieces = pl.by_exp ? ft_cdiv(V, pl.piece) : 1;
   const size_t slab = (size_t)pl.Tp * pl.acc_ld;
-  const int join_grid = ft_cdiv(T, 32), join_threads = T <= 1024 ? 32 * JOIN_WARPS : 256;
+  const int join_grid = ft_cdiv(T, 32);
+  auto join_threads = [](int parts) { return parts > 256 ? 32 * JOIN_WARPS : 256; };
   CUtensorMap acc_out;
   if (t.grad_hidden) FT_TRY(make_map3(ctx, &acc_out, pl.acc, true, pl.acc_ld, pl.Tp, pl.splits, pl.acc_ld, 32, 32));
   const dim3 unpack_grid((unsigned)std::min(ft_cdiv(T, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(std::max(pl.acc_ld, 1), 128));
@@ -1489,8 +1498,9 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       const bool first = v0 == 0, last = v0 + cols == V;
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
+      const int parts = parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(cols, TILE);
       if (!pl.one_piece)
-        FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(cols, TILE),
+        FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads(parts), 0, pl.part, pl.Tp, parts,
                       pl.rows, 0, first ? 1 : 0, last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
       if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       const TcProduct p = dh_product(v0, cols);
@@ -1523,7 +1533,8 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     tile(z, pl.pair, TILE, a_rows, !vm);
     if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(TILE)));
     FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
-    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp, parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(V, TILE), pl.rows,
+    const int parts = parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(V, TILE);
+    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads(parts), 0, pl.part, pl.Tp, parts, pl.rows,
                   0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
     const dim3 grid(ft_cdiv(V, 2048), std::max(1, std::min(pl.Tp, ctx->sm_count * 32 / ft_cdiv(V, 2048))));
     FT_LAUNCH_PDL(ctx, k_ce_normalise, grid, 256, 0, pl.grad, (size_t)pl.Tp * pl.piece, pl.piece, pl.part, pl.Tp, pl.rows, pl.piece,
@@ -1535,8 +1546,8 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     int workers = 0;
     if (vm) FT_TRY(k_map(&w_k, w, pl.w_cols, pl.w_rows, pl.w_planes, pl.w_ld, b_box(pl.stat_n)));
     FT_TRY(launch_rows<EPI_STATS>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, h_k, z, &workers));
-    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads, 0, pl.part, pl.Tp,
-                  parts_of(EPI_STATS, two, pl.pair) * (z.carry ? workers : ft_cdiv(V, pl.stat_n)), z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss,
+    const int parts = parts_of(EPI_STATS, two, pl.pair) * (z.carry ? workers : ft_cdiv(V, pl.stat_n));
+    FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads(parts), 0, pl.part, pl.Tp, parts, z.rw, unpacked ? T : 0, 1, 1, V, t.row_loss,
                   (float*)nullptr, (size_t)0, 0, 0, 0);
   }
   if (!t.grad_hidden && !t.grad_weight) return FT_OK;
