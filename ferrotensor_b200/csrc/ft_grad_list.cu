@@ -14,7 +14,7 @@
 #include <string.h>
 
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <type_traits>
 #include <vector>
 
@@ -443,9 +443,9 @@ extern "C" int ft_grad_list_create(FtContext* ctx, size_t count, void* const* pt
       free_list(l);
       return r;
     }
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception& e) {   // out of host memory, or a count beyond it
     if (l) free_list(l);
-    ft_set_error("ft_grad_list_create: out of host memory");
+    ft_set_error("ft_grad_list_create: %zu tensors: %s", count, e.what());
     return FT_ERR_INVALID;
   }
   *out = l;

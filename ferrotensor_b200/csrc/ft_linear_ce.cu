@@ -333,6 +333,7 @@ k_ce_exact_scatter(const float* __restrict__ acc, Rows rw, int H, T* __restrict_
 
 // ------------------------------------------------------------------------------ the exact path
 constexpr size_t EXACT_PIECE_BYTES = (size_t)256 << 20;
+constexpr size_t EXACT_PIECE_COLUMNS = (size_t)1 << 22;   // of 65535 x 128 that a grid reaches
 
 struct ExactPlan {
   Rows rows;
@@ -361,7 +362,7 @@ ExactPlan exact_plan(const Problem& q, void* base) {
   Carver c(base);
   pl.rows = carve_rows(c, q.T);
   size_t cols = q.p.vocab_piece ? q.p.vocab_piece : std::max<size_t>(64, EXACT_PIECE_BYTES / 4 / std::max(q.T, 1) / 64 * 64);
-  pl.piece = (int)std::min<size_t>(cols, (size_t)q.V);
+  pl.piece = (int)std::min({cols, (size_t)q.V, EXACT_PIECE_COLUMNS});
   pl.hidden = c.take<float>((size_t)q.T * q.H);
   pl.z = c.take<float>((size_t)q.T * pl.piece);
   pl.acc = q.grad_hidden ? c.take<float>((size_t)q.T * q.H) : nullptr;
@@ -372,7 +373,6 @@ ExactPlan exact_plan(const Problem& q, void* base) {
 int launch_exact(FtContext* ctx, const ExactProduct& p, bool b_f16, bool c_f16, const Head* head) {
   if (p.M <= 0 || p.N <= 0) return FT_OK;
   const dim3 grid(ft_cdiv(p.M, ET), ft_cdiv(p.N, ET));
-  FT_REQUIRE(grid.y <= 65535, "ft_linear_cross_entropy: the exact products reach %d columns", 65535 * ET);
   if (b_f16) {
     if (c_f16) FT_LAUNCH_PDL(ctx, (k_ce_exact<__half, __half>), grid, 256, 0, p, head);
     else FT_LAUNCH_PDL(ctx, (k_ce_exact<__half, float>), grid, 256, 0, p, head);

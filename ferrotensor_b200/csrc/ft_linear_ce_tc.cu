@@ -87,7 +87,7 @@ struct TcProduct {
   Rows rw;
   float2* part;                     // [parts of a tile * column tiles][part_ld]: {maximum in log2 units, sum}
   int part_ld;
-  int w_early;                      // STATS: W may be read before the launch before this one has ended
+  int w_early;                      // STATS: W is the caller's, not made by a launch of this call
   int piece, pieces;                // STATS, EXP: which launch this is, of how many
   float* base_out;                  // FACTOR: a part of K chooses its own point of reference, [splits][part_ld]
   __half* wy;                       // EXP: the targets' columns of W, [planes][part_ld][wy_ld]
@@ -311,8 +311,8 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t stages = (uint32_t)min(MAX_STAGES, EPI_OFFSET / g.stage_bytes);
   if (EPI == EPI_STATS && g.w_early && warp == 0 && elect_one()) {
-    // W is the caller's and older than the launch before this one: its first tile may be on its way
-    // into L2 while that packs the rows
+    // the first tile of W, where it is the caller's: on its way into L2 while the launch before this
+    // one ends (nothing is read here, and L2 is where later writes to it would go too)
     const int first = pair / ((g.M + TM - 1) / TM);
     const int bn = first * g.tile_n + (PAIR ? (int)rank * (g.tile_n / 2) : 0);
     for (int k = 0; k < g.K && bn < g.N; k += BK) {

@@ -221,6 +221,22 @@ def test_refusals(cuda_ctx, eng):
 
 
 @gpu
+def test_more_than_two_to_the_32_values(cuda_ctx, eng):
+    """One tensor of 2^32 + 9 f16 ones and a half in its last place, clipped in place."""
+    from ferrotensor_b200.engine import GradientList
+    n = (1 << 32) + 9
+    x = torch.ones(n, dtype=F16, device="cuda")
+    x[-1] = 0.5
+    norm = torch.zeros(4, device="cuda")
+    want = (n - 0.75) ** 0.5
+    eng.clip_grad_global_norm(cuda_ctx, GradientList(cuda_ctx, [_ut(x)]), want / 4, _ut(norm))
+    assert abs(float(norm[0]) - want) <= 2.0 ** -23 * want
+    factor = float(norm[2])
+    assert abs(factor - 0.25) <= 1e-6
+    assert float(x[-1]) == 0.125 and all(bool((p == 0.25).all()) for p in x[:-1].split(1 << 30))
+
+
+@gpu
 def test_captured_and_replayed(cuda_ctx):
     from ferrotensor_b200.engine import ComputeEngine, CudaContext, GradientList
     side = torch.cuda.Stream()

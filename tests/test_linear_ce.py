@@ -510,3 +510,67 @@ def test_losses_alone(cuda_ctx, eng, mode, vocab_major):
             q = _truth(x, w, y, a, 1.0, vocab_major)
             got = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, vocab_major, want="none")
             _check(got, q, _bounds(q, mode, types, (F32, F32)), vocab_major, f"{(t, h, v)}")
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+def test_a_very_large_vocabulary(cuda_ctx, eng, mode):
+    """More columns than one grid of the exact products reaches, a hidden size of one."""
+    v = (1 << 23) + 1001
+    x, w, y, a = _make(3, 1, v, (F32, F32), False, "none", 61)
+    y[1] = v - 1
+    q = _truth(x, w, y, a, 1.0, False)
+    got = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, False, want="none")
+    _check(got, q, _bounds(q, mode, (F32, F32), (F32, F32)), False)
+
+
+@gpu
+def test_a_weight_beyond_two_to_the_31_elements(cuda_ctx, eng):
+    """1.1 million columns of 2048 f16 values: offsets pass 32 bits in the weight and in its gradient.  The
+    last columns count, everything is checked where it can be told cheaply: losses and dh against sums
+    over blocks in f64, dW at its first and last columns."""
+    from ferrotensor_b200.engine import GemmMode
+    t, h, v = 5, 2048, 1_100_000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.empty((v, h), dtype=F16, device="cuda")
+    for part in w.split(100_000):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda") * 0.02)
+    x = torch.randn((t, h), generator=g, device="cuda").to(F16)
+    y = torch.tensor([0, v - 1, v // 2, SKIP, v - 2], device="cuda")
+    w[v - 1] += x[1] * 0.003
+    a = torch.full((t,), 0.25, device="cuda")
+    loss, gh, gw = torch.empty(t, device="cuda"), torch.empty_like(x), torch.empty_like(w)
+    cuda_ctx.set_gemm_mode(GemmMode.F16)
+    try:
+        eng.linear_cross_entropy_bt(cuda_ctx, _ut(x), _ut(w), _ut(_targets(y)), _ut(a), _ut(loss), _ut(gh), _ut(gw), grad_scale=4096.0)
+        cuda_ctx.synchronize()
+    finally:
+        cuda_ctx.set_gemm_mode(GemmMode.F32)
+    X = x.double()
+    lse = torch.logsumexp(torch.stack([torch.logsumexp(X @ p.double().t(), 1) for p in w.split(100_000)]), 0)
+    live = y != SKIP
+    yy = torch.where(live, y, 0)
+    want = torch.where(live, lse - (X * w[yy].double()).sum(1), 0.0)
+    assert ((loss.double() - want).abs() <= 1e-5 * (1 + want.abs())).all()
+    c = torch.where(live, 0.25 * 4096.0, 0.0)[:, None]
+    dh = -c * w[yy].double()
+    mag = dh.abs()
+    at = 0
+    for p in w.split(100_000):
+        P = torch.exp(X @ p.double().t() - lse[:, None]) * c
+        dh += P @ p.double()
+        mag += P @ p.double().abs()
+        for cols in (slice(0, 3), slice(len(p) - 3, len(p))):
+            G = P[:, cols].clone()
+            for r in range(t):
+                k = int(yy[r]) - at - cols.start
+                if live[r] and 0 <= k < 3:
+                    G[r, k] -= float(c[r])
+            dw = G.t() @ X
+            # g and the result are rounded to f16 once each, relative to each row's share
+            tol = 2.0 ** -10 * (G.abs().t() @ X.abs()) + 2.0 ** -24
+            assert ((gw[at + cols.start:at + cols.stop].double() - dw).abs() <= tol).all(), at
+        at += len(p)
+    # every term of the sum carries a g (or E) rounded to f16, the sum loses at most 2^-23 of what it has come
+    # to for each group of 16, the result is rounded to f16: against the sum of magnitudes
+    assert ((gh.double() - dh).abs() <= (2.0 ** -11 + v / 16 * 2.0 ** -23) * mag + 2.0 ** -11 * dh.abs() + 2.0 ** -24).all()
