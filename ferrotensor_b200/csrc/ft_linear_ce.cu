@@ -196,49 +196,78 @@ struct ExactProduct {
   int M, N, K;
   int live_m, live_k;        // 1: M (K) is the number of supervised rows
   int accumulate;
+  int splits;                // parts of K, each into its own slab of C (few tiles would leave most of the
+  long long slab;            // multiprocessors idle through a long K)
 };
 
 template <typename TB, typename TC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 k_ce_exact(ExactProduct p, const Head* __restrict__ head) {
-  __shared__ float As[EK][ET + 4], Bs[EK][ET + 4];
+  // two buffers: while a step is multiplied the next one's values travel into registers
+  __shared__ __align__(16) float As[2][EK][ET + 4], Bs[2][EK][ET + 4];
   ft_pdl_wait();
   ft_pdl_launch();
   const int M = p.live_m ? head->count : p.M, K = p.live_k ? head->count : p.K;
   const int m0 = blockIdx.x * ET, n0 = blockIdx.y * ET;
   if (m0 >= M) return;
+  const int steps = (K + EK - 1) / EK;
+  const int k_begin = (int)((long long)steps * blockIdx.z / p.splits) * EK;
+  const int k_end = min(K, (int)((long long)steps * (blockIdx.z + 1) / p.splits) * EK);
   const TB* bp = (const TB*)p.b;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  // A warp reads along whichever index is contiguous: value i of a thread lies at (mn, k) or, i steps
+  // further, 16 of M/N (K contiguous) or 2 of K.
+  constexpr int PER = ET * EK / 256;
+  const bool a_kfast = p.sak == 1, b_kfast = p.sbk == 1;
+  const int am = a_kfast ? tid / EK : tid % ET, ak = a_kfast ? tid % EK : tid / ET;
+  const int bn = b_kfast ? tid / EK : tid % ET, bk = b_kfast ? tid % EK : tid / ET;
+  const long long a_step = a_kfast ? 16 * p.sam : 2 * p.sak, b_step = b_kfast ? 16 * p.sbn : 2 * p.sbk;
+  const float* ap = p.a + (m0 + am) * p.sam + (k_begin + ak) * p.sak;
+  const TB* bq = bp + (n0 + bn) * p.sbn + (k_begin + bk) * p.sbk;
+  const int a_left = M - m0 - am, b_left = p.N - n0 - bn;          // of M/N, for this thread's first value
+  float ar[PER], br[PER];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool oka = a_kfast ? 16 * i < a_left && k0 + ak < k_end : a_left > 0 && k0 + ak + 2 * i < k_end;
+      const bool okb = b_kfast ? 16 * i < b_left && k0 + bk < k_end : b_left > 0 && k0 + bk + 2 * i < k_end;
+      ar[i] = oka ? ap[i * a_step] : 0.f;
+      br[i] = okb ? (float)bq[i * b_step] : 0.f;
+    }
+    ap += EK * p.sak;
+    bq += EK * p.sbk;
+  };
+  auto settle = [&](int buf) {
+    float* as = &As[buf][ak][am];
+    float* bs = &Bs[buf][bk][bn];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      as[a_kfast ? 16 * i : 2 * i * (ET + 4)] = ar[i];
+      bs[b_kfast ? 16 * i : 2 * i * (ET + 4)] = br[i];
+    }
+  };
   float acc[8][8] = {};
-  for (int k0 = 0; k0 < K; k0 += EK) {
-#pragma unroll
-    for (int i = 0; i < ET * EK / 256; ++i) {
-      const int e = tid + i * 256;
-      int m, k;
-      if (p.sak == 1) { k = e % EK; m = e / EK; } else { m = e % ET; k = e / ET; }
-      As[k][m] = (m0 + m < M && k0 + k < K) ? p.a[(m0 + m) * p.sam + (k0 + k) * p.sak] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < ET * EK / 256; ++i) {
-      const int e = tid + i * 256;
-      int n, k;
-      if (p.sbk == 1) { k = e % EK; n = e / EK; } else { n = e % ET; k = e / ET; }
-      Bs[k][n] = (n0 + n < p.N && k0 + k < K) ? (float)bp[(k0 + k) * p.sbk + (n0 + n) * p.sbn] : 0.f;
-    }
-    __syncthreads();
+  if (k_begin < k_end) {
+    fetch(k_begin);
+    settle(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += EK, buf ^= 1) {
+    if (k0 + EK < k_end) fetch(k0 + EK);
 #pragma unroll
     for (int k = 0; k < EK; ++k) {
       float av[8], bv[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        av[i] = As[k][ty * 4 + i]; av[4 + i] = As[k][64 + ty * 4 + i];
-        bv[i] = Bs[k][tx * 4 + i]; bv[4 + i] = Bs[k][64 + tx * 4 + i];
-      }
+      *(float4*)av = *(const float4*)&As[buf][k][ty * 4];
+      *(float4*)(av + 4) = *(const float4*)&As[buf][k][64 + ty * 4];
+      *(float4*)bv = *(const float4*)&Bs[buf][k][tx * 4];
+      *(float4*)(bv + 4) = *(const float4*)&Bs[buf][k][64 + tx * 4];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
     }
+    if (k0 + EK < k_end) settle(buf ^ 1);
     __syncthreads();
   }
 #pragma unroll
@@ -249,7 +278,7 @@ k_ce_exact(ExactProduct p, const Head* __restrict__ head) {
     for (int j = 0; j < 8; ++j) {
       const int n = n0 + (j & 4) * 16 + tx * 4 + (j & 3);
       if (n >= p.N) continue;
-      TC* c = (TC*)p.c + m * p.scm + n * p.scn;
+      TC* c = (TC*)p.c + blockIdx.z * p.slab + m * p.scm + n * p.scn;
       *c = (TC)(p.accumulate ? (float)*c + acc[i][j] : acc[i][j]);
     }
   }
@@ -322,13 +351,17 @@ k_ce_exact_grad(float* __restrict__ z, int v0, int cols, Rows rw) {
 // packed f32 rows -> grad_hidden, zeros for the rows that were skipped
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_ce_exact_scatter(const float* __restrict__ acc, Rows rw, int H, T* __restrict__ out) {
+k_ce_exact_scatter(const float* __restrict__ acc, size_t slab, int splits, Rows rw, int H, T* __restrict__ out) {
   ft_pdl_wait();
   ft_pdl_launch();
   const int r = blockIdx.x;
   const int at = rw.place[r];
-  for (int c = threadIdx.x; c < H; c += 256)
-    out[(size_t)r * H + c] = (T)(at >= 0 ? acc[(size_t)at * H + c] : 0.f);
+  for (int c = threadIdx.x; c < H; c += 256) {
+    float v = 0.f;
+    if (at >= 0)
+      for (int s = 0; s < splits; ++s) v += acc[s * slab + (size_t)at * H + c];
+    out[(size_t)r * H + c] = (T)v;
+  }
 }
 
 // ------------------------------------------------------------------------------ the exact path
@@ -338,7 +371,7 @@ constexpr size_t EXACT_PIECE_COLUMNS = (size_t)1 << 22;   // of 65535 x 128 that
 struct ExactPlan {
   Rows rows;
   float *hidden, *z, *acc;
-  int piece;
+  int piece, splits;
   size_t bytes;
 };
 
@@ -357,7 +390,7 @@ int launch_gather(FtContext* ctx, const Problem& q, const Tensors& t, const Rows
   return FT_OK;
 }
 
-ExactPlan exact_plan(const Problem& q, void* base) {
+ExactPlan exact_plan(const FtContext* ctx, const Problem& q, void* base) {
   ExactPlan pl;
   Carver c(base);
   pl.rows = carve_rows(c, q.T);
@@ -365,14 +398,19 @@ ExactPlan exact_plan(const Problem& q, void* base) {
   pl.piece = (int)std::min({cols, (size_t)q.V, EXACT_PIECE_COLUMNS});
   pl.hidden = c.take<float>((size_t)q.T * q.H);
   pl.z = c.take<float>((size_t)q.T * pl.piece);
-  pl.acc = q.grad_hidden ? c.take<float>((size_t)q.T * q.H) : nullptr;
+  // parts of the vocabulary for dh: two blocks for every multiprocessor, 512 columns each at least, 256 MB of slabs
+  const size_t slab = (size_t)std::max(q.T, 1) * q.H * 4;
+  const long long tiles = (long long)ft_cdiv(std::max(q.T, 1), ET) * ft_cdiv(q.H, ET);
+  pl.splits = (int)std::max<long long>(1, std::min({2ll * ctx->sm_count / tiles, (long long)pl.piece / 512,
+                                                    (long long)(((size_t)256 << 20) / slab), 32ll}));
+  pl.acc = q.grad_hidden ? c.take<float>((size_t)pl.splits * q.T * q.H) : nullptr;
   pl.bytes = c.bytes();
   return pl;
 }
 
 int launch_exact(FtContext* ctx, const ExactProduct& p, bool b_f16, bool c_f16, const Head* head) {
   if (p.M <= 0 || p.N <= 0) return FT_OK;
-  const dim3 grid(ft_cdiv(p.M, ET), ft_cdiv(p.N, ET));
+  const dim3 grid(ft_cdiv(p.M, ET), ft_cdiv(p.N, ET), p.splits);
   if (b_f16) {
     if (c_f16) FT_LAUNCH_PDL(ctx, (k_ce_exact<__half, __half>), grid, 256, 0, p, head);
     else FT_LAUNCH_PDL(ctx, (k_ce_exact<__half, float>), grid, 256, 0, p, head);
@@ -384,7 +422,7 @@ int launch_exact(FtContext* ctx, const ExactProduct& p, bool b_f16, bool c_f16, 
 }
 
 int exact_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
-  const ExactPlan pl = exact_plan(q, ws);
+  const ExactPlan pl = exact_plan(ctx, q, ws);
   const int T = q.T, H = q.H, V = q.V;
   FT_TRY(launch_gather<float>(ctx, q, t, pl.rows, pl.hidden, H, T, 1));
   const bool w16 = q.p.weight_type == FT_TYPE_F16;
@@ -395,7 +433,7 @@ int exact_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.a = pl.hidden; p.sam = H; p.sak = 1;
     p.b = (const char*)t.weight + (size_t)v0 * swv * we; p.sbk = swk; p.sbn = swv;
     p.c = pl.z; p.scm = cols; p.scn = 1;
-    p.M = T; p.N = cols; p.K = H; p.live_m = 1;
+    p.M = T; p.N = cols; p.K = H; p.live_m = 1; p.splits = 1;
     return launch_exact(ctx, p, w16, false, pl.rows.head);
   };
   for (int v0 = 0; v0 < V; v0 += pl.piece) {
@@ -415,6 +453,7 @@ int exact_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       p.b = (const char*)t.weight + (size_t)v0 * swv * we; p.sbk = swv; p.sbn = swk;
       p.c = pl.acc; p.scm = H; p.scn = 1;
       p.M = T; p.N = H; p.K = cols; p.live_m = 1; p.accumulate = v0 > 0;
+      p.splits = pl.splits; p.slab = (long long)T * H;
       FT_TRY(launch_exact(ctx, p, w16, false, pl.rows.head));
     }
     if (t.grad_weight) {
@@ -423,15 +462,15 @@ int exact_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       p.a = pl.z; p.sam = 1; p.sak = cols;
       p.b = pl.hidden; p.sbk = H; p.sbn = 1;
       p.c = (char*)t.grad_weight + (size_t)v0 * swv * ge; p.scm = swv; p.scn = swk;
-      p.M = cols; p.N = H; p.K = T; p.live_k = 1;
+      p.M = cols; p.N = H; p.K = T; p.live_k = 1; p.splits = 1;
       FT_TRY(launch_exact(ctx, p, false, ge == 2, pl.rows.head));
     }
   }
   if (t.grad_hidden) {
     if (q.p.grad_hidden_type == FT_TYPE_F16)
-      FT_LAUNCH_PDL(ctx, k_ce_exact_scatter<__half>, T, 256, 0, pl.acc, pl.rows, H, (__half*)t.grad_hidden);
+      FT_LAUNCH_PDL(ctx, k_ce_exact_scatter<__half>, T, 256, 0, pl.acc, (size_t)T * H, pl.splits, pl.rows, H, (__half*)t.grad_hidden);
     else
-      FT_LAUNCH_PDL(ctx, k_ce_exact_scatter<float>, T, 256, 0, pl.acc, pl.rows, H, (float*)t.grad_hidden);
+      FT_LAUNCH_PDL(ctx, k_ce_exact_scatter<float>, T, 256, 0, pl.acc, (size_t)T * H, pl.splits, pl.rows, H, (float*)t.grad_hidden);
   }
   return FT_OK;
 }
@@ -468,7 +507,7 @@ extern "C" int ft_linear_cross_entropy_workspace(FtContext* ctx, const void* wei
   FT_TRY(check_params("ft_linear_cross_entropy_workspace", ctx, p));
   FT_REQUIRE(bytes, "ft_linear_cross_entropy_workspace: NULL argument");
   const Problem q = make_problem(*p, want_grad_hidden != 0, want_grad_weight != 0);
-  *bytes = ctx->gemm_mode == FT_GEMM_F32 ? exact_plan(q, nullptr).bytes : tc_workspace(ctx, q, weight);
+  *bytes = ctx->gemm_mode == FT_GEMM_F32 ? exact_plan(ctx, q, nullptr).bytes : tc_workspace(ctx, q, weight);
   return FT_OK;
 }
 
