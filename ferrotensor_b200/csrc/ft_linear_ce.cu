@@ -507,7 +507,8 @@ extern "C" int ft_linear_cross_entropy_workspace(FtContext* ctx, const void* wei
   FT_TRY(check_params("ft_linear_cross_entropy_workspace", ctx, p));
   FT_REQUIRE(bytes, "ft_linear_cross_entropy_workspace: NULL argument");
   const Problem q = make_problem(*p, want_grad_hidden != 0, want_grad_weight != 0);
-  *bytes = ctx->gemm_mode == FT_GEMM_F32 ? exact_plan(ctx, q, nullptr).bytes : tc_workspace(ctx, q, weight);
+  *bytes = few_serves(ctx, q)              ? few_workspace(ctx, q, weight)
+           : ctx->gemm_mode == FT_GEMM_F32 ? exact_plan(ctx, q, nullptr).bytes : tc_workspace(ctx, q, weight);
   return FT_OK;
 }
 
@@ -550,5 +551,6 @@ extern "C" int ft_linear_cross_entropy(FtContext* ctx, const void* hidden, const
   }
   const Problem q = make_problem(*p, grad_hidden != nullptr, grad_weight != nullptr);
   const Tensors t = {hidden, weight, targets, weights, row_loss, grad_hidden, grad_weight};
+  if (few_serves(ctx, q)) return few_path(ctx, q, t, workspace);
   return ctx->gemm_mode == FT_GEMM_F32 ? exact_path(ctx, q, t, workspace) : tc_path(ctx, q, t, workspace);
 }

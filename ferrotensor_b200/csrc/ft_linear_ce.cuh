@@ -120,6 +120,10 @@ inline int gather_rows(int T) { return std::max(8, ft_cdiv(T, 1024)); }
 // ft_linear_ce_tc.cu
 size_t tc_workspace(const FtContext* ctx, const Problem& q, const void* weight);
 int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws);
+// ft_linear_ce_few.cu: calls of a few rows
+bool few_serves(const FtContext* ctx, const Problem& q);
+size_t few_workspace(const FtContext* ctx, const Problem& q, const void* weight);
+int few_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws);
 // ft_linear_ce.cu: packs the supervised rows as f16 planes [planes][plane_rows][ld]
 int launch_gather_f16(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, __half* out, int ld,
                       int plane_rows, int planes);

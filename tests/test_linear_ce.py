@@ -574,3 +574,66 @@ def test_a_weight_beyond_two_to_the_31_elements(cuda_ctx, eng):
     # every term of the sum carries a g (or E) rounded to f16, the sum loses at most 2^-23 of what it has come
     # to for each group of 16, the result is rounded to f16: against the sum of magnitudes
     assert ((gh.double() - dh).abs() <= (2.0 ** -11 + v / 16 * 2.0 ** -23) * mag + 2.0 ** -11 * dh.abs() + 2.0 ** -24).all()
+
+
+# (rows, hidden, vocab): every number of rows that a kernel is built for and the first that it is not, hidden
+# sizes and vocabularies off every vector width, slices that end inside a warp, vocabularies wide enough
+# for one, two and four columns a lane, and one row of one value
+FEW = [(1, 1, 1), (1, 576, 14400), (2, 130, 7111), (4, 36, 129), (5, 2, 3), (7, 513, 7106), (8, 260, 1000), (9, 64, 2050),
+       (13, 67, 515), (16, 132, 4097), (16, 20, 15000), (17, 40, 300), (3, 2700, 200), (16, 2700, 90)]
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("types,gtypes", [((F16, F16), (F16, F16)), ((F32, F16), (F32, F32)), ((F32, F32), (F32, F32)),
+                                          ((F16, F32), (F16, F16))])
+@pytest.mark.parametrize("vocab_major", [False, True])
+def test_few_rows(cuda_ctx, eng, mode, types, gtypes, vocab_major):
+    for i, (t, h, v) in enumerate(FEW):
+        mask = ("none", "half", "beyond", "last")[i % 4]
+        s = 64.0 if F16 in gtypes else 1.0
+        x, w, y, a = _make(t, h, v, types, vocab_major, mask, 300 + i)
+        x[y == SKIP] = float("nan")
+        a[y == SKIP] = float("inf")
+        q = _truth(x, w, y, a, s, vocab_major)
+        tols = _bounds(q, mode, types, gtypes)
+        for want in ("both", "hidden", "none"):
+            got = _call(cuda_ctx, eng, mode, x, w, y, a, s, vocab_major, gtypes, want)
+            _check(got, q, tols, vocab_major, f"{(t, h, v)} {want}")
+            again = _call(cuda_ctx, eng, mode, x, w, y, a, s, vocab_major, gtypes, want)
+            assert all(p is None or torch.equal(p, r) for p, r in zip(got, again))
+
+
+@gpu
+@pytest.mark.parametrize("vocab_major", [False, True])
+def test_few_rows_beside_infinite_weights(cuda_ctx, eng, vocab_major):
+    """A skipped row's gradient is zero whatever the weights hold; so is what it adds to theirs."""
+    x, w, y, a = _make(6, 40, 200, (F32, F32), vocab_major, "none", 3)
+    y[[1, 4]] = SKIP
+    x[1] = float("inf")
+    if vocab_major:
+        w[7, 3] = float("inf")
+    else:
+        w[3, 7] = float("inf")
+    for mode in MODES:
+        loss, gh, gw = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, vocab_major)
+        assert (loss[[1, 4]] == 0).all() and (gh[[1, 4]] == 0).all()
+        assert not loss[0].isfinite() and gw.isnan().any()
+    y[:] = SKIP
+    for mode in MODES:
+        loss, gh, gw = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, vocab_major)
+        assert (loss == 0).all() and (gh == 0).all() and (gw == 0).all()
+
+
+@gpu
+def test_few_rows_agree_with_many(cuda_ctx, eng):
+    """The same rows alone and in a batch: both within the bound of the exact products, so within twice
+    that of each other."""
+    for vocab_major in (False, True):
+        x, w, y, a = _make(40, 200, 3000, (F32, F32), vocab_major, "none", 21)
+        many = _call(cuda_ctx, eng, "F32", x, w, y, a, 1.0, vocab_major, want="hidden")
+        for r in (slice(0, 1), slice(3, 9), slice(20, 36)):
+            q = _truth(x[r], w, y[r], a[r], 1.0, vocab_major)
+            tol = _bounds(q, "F32", (F32, F32), (F32, F32))
+            few = _call(cuda_ctx, eng, "F32", x[r], w, y[r], a[r], 1.0, vocab_major, want="hidden")
+            assert ((few[0] - many[0][r]).abs() <= 2 * tol[0]).all() and ((few[1] - many[1][r]).abs() <= 2 * tol[1]).all()
