@@ -61,11 +61,25 @@ __device__ __forceinline__ void pack_row(const TH* __restrict__ from, int H, flo
   }
 }
 
+// largest finite magnitude of a row, in every lane
+template <typename TH>
+__device__ __forceinline__ float row_amax(const TH* __restrict__ from, int H, int lane) {
+  float m = 0.f;
+#pragma unroll 8
+  for (int c = lane; c < H; c += 32) {
+    const float x = fabsf((float)from[c]);
+    if (x < INFINITY) m = fmaxf(m, x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
 // One block packs rows [blockIdx.x * per, ...).  Every block counts the supervised rows of the
 // whole batch itself (targets are 4 bytes a row and come from L2), which gives it the place of its
 // first row and the total without a launch of its own or a wait on its neighbours.
 // TO = __half: as `planes` f16 planes of `plane_rows` rows, times the power of two of the largest
-// value where they are f32, and with zero rows up to the next multiple of 64 (a K block of dW).
+// value (of each row's, with rw.unscale) where they are f32, and with zero rows up to the next multiple of 64 (a K block of dW).
 template <typename TH, typename TO>
 __global__ void __launch_bounds__(GATHER_THREADS)
 k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
@@ -85,7 +99,7 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
   int before = 0, all = 0;
   float big = 0.f, h_top = 0.f, w_top = 0.f;   // of |s w_t|, of the operands
   {
-    if (sizeof(TO) == 2 && sizeof(TH) == 4)
+    if (sizeof(TO) == 2 && sizeof(TH) == 4 && !rw.unscale)
       for (int i = tid; i < AMAX_BLOCKS; i += GATHER_THREADS) h_top = fmaxf(h_top, rw.h_max[i]);
     if (sizeof(TO) == 2 && w_scaled && blockIdx.x == 0)
       for (int i = tid; i < AMAX_BLOCKS; i += GATHER_THREADS) w_top = fmaxf(w_top, rw.w_max[i]);
@@ -169,7 +183,12 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
       if constexpr (sizeof(TO) == 4) {
         for (int c = lane; c < H; c += 32) to[c] = (float)from[c];
       } else {
-        pack_row(from, H, h_scale, to, ld, planes == 2 ? to + (size_t)plane_rows * ld : nullptr, lane);
+        float S = h_scale;
+        if (sizeof(TH) == 4 && rw.unscale) {
+          S = power_for(row_amax(from, H, lane), OPERAND_EXP);
+          if (lane == 0) rw.unscale[at + k] = 1.0f / S;
+        }
+        pack_row(from, H, S, to, ld, planes == 2 ? to + (size_t)plane_rows * ld : nullptr, lane);
       }
     }
     at += total;

@@ -28,7 +28,7 @@ struct Head {
   float g_scale;      // power of two that g carries while it is held in f16
   float g_unscale;
   float h_scale, h_unscale, w_unscale;   // of the f16 planes of f32 operands, else 1
-  float z_scale;      // h_unscale * w_unscale
+  float z_scale;      // h_unscale * w_unscale (w_unscale alone where rows have scales of their own)
 };
 
 // Blocks of k_ce_amax for each operand, and the values that it leaves.
@@ -56,6 +56,7 @@ struct Rows {
   int* source;        // its row in the caller's tensors
   uint32_t* target;
   float* weight;      // grad_scale * weights[row]
+  float* unscale;     // of the row's f16 planes, or null: all rows have the head's
   float2* stat;       // running {maximum, sum of exponentials against it}; E, at the end: factors of dh's two terms
   float* picked;      // logit of the target
   float* exact;       // the same from f32 products, beside the tensor cores' sum
@@ -104,6 +105,7 @@ inline Rows carve_rows(Carver& c, int T) {
   r.source = c.take<int>(T);
   r.target = c.take<uint32_t>(T);
   r.weight = c.take<float>(T);
+  r.unscale = c.take<float>(T);
   r.stat = c.take<float2>(T);
   r.picked = c.take<float>(T);
   r.exact = c.take<float>(T);
