@@ -8,7 +8,7 @@
 // the logits are computed twice: one pass over the vocabulary that keeps the running maximum and
 // sum of each row, then piece by piece the logits again, g of that piece, and g's two products.
 //
-// Only supervised rows take part.  k_ce_gather packs them (in order) into the workspace, so a batch
+// Only supervised rows take part.  gather_block packs them (in order) into the workspace, so a batch
 // whose prompt is masked costs its supervised tokens only, and what a skipped row holds (NaN
 // included) reaches nothing.  How many there are is known on the device alone: launches are sized
 // for all rows, and the kernels read the count.
@@ -25,182 +25,14 @@ namespace {
 
 using namespace ft_ce;
 
-// ------------------------------------------------------------------------------ row bookkeeping
-constexpr int GATHER_THREADS = 256;
-
-// One row -> f16 (and its rounding remainder, when `lo` is given), eight values a lane.
 template <typename TH>
-__device__ __forceinline__ void pack_row(const TH* __restrict__ from, int H, float S, __half* __restrict__ hi, int ld,
-                                         __half* __restrict__ lo, int lane) {
-  const bool vec = (((uintptr_t)from) & 15) == 0;
-  for (int c = lane * 8; c < ld; c += 256) {
-    if constexpr (sizeof(TH) == 2) {
-      if (vec && c + 8 <= H) {
-        *(uint4*)(hi + c) = *(const uint4*)(from + c);
-        continue;
-      }
-    }
-    float v[8];
-    if (vec && c + 8 <= H && sizeof(TH) == 4) {
-      const float4 a = *(const float4*)(from + c), b = *(const float4*)(from + c + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = c + k < H ? (float)from[c + k] : 0.f;
-    }
-    __half2 h[4], l[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float a = v[2 * k] * S, b = v[2 * k + 1] * S;
-      h[k] = __floats2half2_rn(a, b);
-      const float2 f = __half22float2(h[k]);
-      l[k] = __floats2half2_rn(a - f.x, b - f.y);
-    }
-    *(uint4*)(hi + c) = *(const uint4*)h;
-    if (lo) *(uint4*)(lo + c) = *(const uint4*)l;
-  }
-}
-
-// largest finite magnitude of a row, in every lane
-template <typename TH>
-__device__ __forceinline__ float row_amax(const TH* __restrict__ from, int H, int lane) {
-  float m = 0.f;
-#pragma unroll 8
-  for (int c = lane; c < H; c += 32) {
-    const float x = fabsf((float)from[c]);
-    if (x < INFINITY) m = fmaxf(m, x);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
-
-// One block packs rows [blockIdx.x * per, ...).  Every block counts the supervised rows of the
-// whole batch itself (targets are 4 bytes a row and come from L2), which gives it the place of its
-// first row and the total without a launch of its own or a wait on its neighbours.
-// TO = __half: as `planes` f16 planes of `plane_rows` rows, times the power of two of the largest
-// value (of each row's, with rw.unscale) where they are f32, and with zero rows up to the next multiple of 64 (a K block of dW).
-template <typename TH, typename TO>
 __global__ void __launch_bounds__(GATHER_THREADS)
-k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
-            const float* __restrict__ weights, float grad_scale, int rows, int H, int per, Rows rw,
-            TO* __restrict__ out, int ld, int plane_rows, int planes, int w_scaled,
-            float* __restrict__ row_loss) {
-  constexpr int WARPS = GATHER_THREADS / 32;
-  __shared__ int red[WARPS], counts[2][WARPS];
-  __shared__ float tops[3][WARPS];
-  __shared__ int src_row[GATHER_THREADS];
+k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets, const float* __restrict__ weights,
+            float grad_scale, int rows, int H, int per, Rows rw, float* __restrict__ out, float* __restrict__ row_loss) {
   ft_pdl_wait();
   ft_pdl_launch();
-  const int r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // What has to be known of the whole batch, every thread's share first: all loads are under way
-  // before the one join.
-  int before = 0, all = 0;
-  float big = 0.f, h_top = 0.f, w_top = 0.f;   // of |s w_t|, of the operands
-  {
-    if (sizeof(TO) == 2 && sizeof(TH) == 4 && !rw.unscale)
-      for (int i = tid; i < AMAX_BLOCKS; i += GATHER_THREADS) h_top = fmaxf(h_top, rw.h_max[i]);
-    if (sizeof(TO) == 2 && w_scaled && blockIdx.x == 0)
-      for (int i = tid; i < AMAX_BLOCKS; i += GATHER_THREADS) w_top = fmaxf(w_top, rw.w_max[i]);
-    auto count = [&](int i, uint32_t y) {
-      const int one = y != FT_MASKED_CE_SKIP;
-      all += one;
-      before += i < r0 ? one : 0;
-    };
-    const int vec = (((uintptr_t)targets) & 15) == 0 ? rows / 4 : 0;
-    for (int i = tid; i < vec; i += GATHER_THREADS) {
-      const uint4 y = ((const uint4*)targets)[i];
-      count(4 * i, y.x); count(4 * i + 1, y.y); count(4 * i + 2, y.z); count(4 * i + 3, y.w);
-    }
-    for (int i = 4 * vec + tid; i < rows; i += GATHER_THREADS) count(i, targets[i]);
-    if (blockIdx.x == 0 && weights)
-      for (int i = tid; i < rows; i += GATHER_THREADS) {
-        const float w = fabsf(weights[i] * grad_scale);
-        if (targets[i] != FT_MASKED_CE_SKIP) big = fmaxf(big, w);
-      }
-    before = __reduce_add_sync(0xffffffffu, before);
-    all = __reduce_add_sync(0xffffffffu, all);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-      h_top = fmaxf(h_top, __shfl_xor_sync(0xffffffffu, h_top, o));
-      w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
-    }
-    if (lane == 0) {
-      counts[0][warp] = before; counts[1][warp] = all;
-      tops[0][warp] = big; tops[1][warp] = h_top; tops[2][warp] = w_top;
-    }
-    __syncthreads();
-    before = all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      before += counts[0][w]; all += counts[1][w];
-      big = fmaxf(big, tops[0][w]); h_top = fmaxf(h_top, tops[1][w]); w_top = fmaxf(w_top, tops[2][w]);
-    }
-  }
-  const float h_scale = sizeof(TO) == 2 && sizeof(TH) == 4 ? power_for(h_top, OPERAND_EXP) : 1.f;
-  if (blockIdx.x == 0 && tid == 0) {
-    const float S = power_for(big, G_EXP);
-    rw.head->count = all;
-    rw.head->g_scale = S;
-    rw.head->g_unscale = 1.0f / S;
-    if constexpr (sizeof(TO) == 2) {
-      const float wu = w_scaled ? 1.0f / power_for(w_top, OPERAND_EXP) : 1.0f;
-      rw.head->h_unscale = 1.0f / h_scale;
-      rw.head->w_unscale = wu;
-      rw.head->z_scale = wu / h_scale;
-    }
-  }
-  int at = before;
-  for (int base = r0; base < r1; base += GATHER_THREADS) {
-    const int r = base + tid;
-    const uint32_t y = r < r1 ? targets[r] : FT_MASKED_CE_SKIP;
-    const bool live = y != FT_MASKED_CE_SKIP;
-    const uint32_t mask = __ballot_sync(0xffffffffu, live);
-    __syncthreads();
-    if (lane == 0) red[warp] = __popc(mask);
-    __syncthreads();
-    int mine = __popc(mask & ((1u << lane) - 1u)), total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) mine += red[w];
-      total += red[w];
-    }
-    if (live) {
-      src_row[mine] = r;
-      rw.source[at + mine] = r;
-      rw.target[at + mine] = y;
-      rw.weight[at + mine] = weights ? weights[r] * grad_scale : 0.f;
-    } else if (r < r1) {
-      row_loss[r] = 0.f;
-    }
-    if (r < r1) rw.place[r] = live ? at + mine : -1;
-    __syncthreads();
-    for (int k = warp; k < total; k += GATHER_THREADS / 32) {
-      const TH* from = hidden + (size_t)src_row[k] * H;
-      TO* to = out + (size_t)(at + k) * ld;
-      if constexpr (sizeof(TO) == 4) {
-        for (int c = lane; c < H; c += 32) to[c] = (float)from[c];
-      } else {
-        float S = h_scale;
-        if (sizeof(TH) == 4 && rw.unscale) {
-          S = power_for(row_amax(from, H, lane), OPERAND_EXP);
-          if (lane == 0) rw.unscale[at + k] = 1.0f / S;
-        }
-        pack_row(from, H, S, to, ld, planes == 2 ? to + (size_t)plane_rows * ld : nullptr, lane);
-      }
-    }
-    at += total;
-    __syncthreads();
-  }
-  if constexpr (sizeof(TO) == 2) {
-    const int end = max(64, (all + 63) / 64 * 64);
-    for (int p = 0; p < planes; ++p)
-      for (int r = all + (int)blockIdx.x * (GATHER_THREADS / 32) + warp; r < end; r += gridDim.x * (GATHER_THREADS / 32))
-        for (int c = lane * 8; c < ld; c += 256)
-          *(uint4*)(out + ((size_t)p * plane_rows + r) * ld + c) = make_uint4(0u, 0u, 0u, 0u);
-  }
+  gather_block<TH, float>(blockIdx.x, gridDim.x, hidden, targets, weights, grad_scale, rows, H, per, rw, out, H, rows, 1, 0,
+                          row_loss);
 }
 
 // ------------------------------------------------------------------------------ exact products
@@ -394,18 +226,14 @@ struct ExactPlan {
   size_t bytes;
 };
 
-template <typename TO>
-int launch_gather(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, TO* out, int ld, int plane_rows,
-                  int planes) {
+int launch_gather(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, float* out) {
   const int per = gather_rows(q.T), blocks = ft_cdiv(q.T, per);
   if (q.p.hidden_type == FT_TYPE_F16)
-    FT_LAUNCH_PDL(ctx, (k_ce_gather<__half, TO>), blocks, GATHER_THREADS, 0, (const __half*)t.hidden, t.targets, t.weights,
-                  q.p.grad_scale, q.T, q.H, per, rw, out, ld, plane_rows, planes,
-                  q.p.weight_type == FT_TYPE_F32 ? 1 : 0, t.row_loss);
+    FT_LAUNCH_PDL(ctx, k_ce_gather<__half>, blocks, GATHER_THREADS, 0, (const __half*)t.hidden, t.targets, t.weights,
+                  q.p.grad_scale, q.T, q.H, per, rw, out, t.row_loss);
   else
-    FT_LAUNCH_PDL(ctx, (k_ce_gather<float, TO>), blocks, GATHER_THREADS, 0, (const float*)t.hidden, t.targets, t.weights,
-                  q.p.grad_scale, q.T, q.H, per, rw, out, ld, plane_rows, planes,
-                  q.p.weight_type == FT_TYPE_F32 ? 1 : 0, t.row_loss);
+    FT_LAUNCH_PDL(ctx, k_ce_gather<float>, blocks, GATHER_THREADS, 0, (const float*)t.hidden, t.targets, t.weights,
+                  q.p.grad_scale, q.T, q.H, per, rw, out, t.row_loss);
   return FT_OK;
 }
 
@@ -443,7 +271,7 @@ int launch_exact(FtContext* ctx, const ExactProduct& p, bool b_f16, bool c_f16, 
 int exact_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   const ExactPlan pl = exact_plan(ctx, q, ws);
   const int T = q.T, H = q.H, V = q.V;
-  FT_TRY(launch_gather<float>(ctx, q, t, pl.rows, pl.hidden, H, T, 1));
+  FT_TRY(launch_gather(ctx, q, t, pl.rows, pl.hidden));
   const bool w16 = q.p.weight_type == FT_TYPE_F16;
   const long long swk = q.p.weight_vocab_major ? 1 : V, swv = q.p.weight_vocab_major ? H : 1;   // strides of W(k, v)
   const size_t we = w16 ? 2 : 4;
@@ -515,11 +343,6 @@ Problem make_problem(const FtLinearCeParams& p, bool gh, bool gw) {
 size_t type_size(uint32_t t) { return t == FT_TYPE_F16 ? 2 : 4; }
 
 }  // namespace
-
-int ft_ce::launch_gather_f16(FtContext* ctx, const Problem& q, const Tensors& t, const Rows& rw, __half* out, int ld,
-                             int plane_rows, int planes) {
-  return launch_gather<__half>(ctx, q, t, rw, out, ld, plane_rows, planes);
-}
 
 extern "C" int ft_linear_cross_entropy_workspace(FtContext* ctx, const void* weight, const FtLinearCeParams* p,
                                                  int want_grad_hidden, int want_grad_weight, size_t* bytes) {

@@ -988,20 +988,17 @@ k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* _
   }
 }
 
-// W [rows, cols] -> f16 planes [planes][rows][ld], times the power of two of its largest value
+// W [rows, cols] -> f16 planes [planes][rows][ld], times the power of two of its largest value; block
+// (bx, by) of (gx, ...): a warp takes 1024 columns of a row
 template <typename T>
-__global__ void __launch_bounds__(256)
-k_ce_weight(const T* __restrict__ w, int rows, int cols, __half* __restrict__ out, int ld, int planes,
-            const float* __restrict__ w_max) {
+__device__ __forceinline__ void weight_block(int bx, int by, int gx, const T* __restrict__ w, int rows, int cols,
+                                             __half* __restrict__ out, int ld, int planes, const float* __restrict__ w_max) {
   __shared__ float red[8];
-  ft_pdl_wait();
-  ft_pdl_launch();
   const float S = sizeof(T) == 4 ? power_for(block_max_of(w_max, AMAX_BLOCKS, red), OPERAND_EXP) : 1.f;
   const size_t plane = (size_t)rows * ld;
-  // a warp takes 1024 columns of a row
-  const int c_end = min(ld, ((int)blockIdx.y + 1) * 1024);
-  for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
-  for (int c = blockIdx.y * 1024 + (threadIdx.x % 32) * 8; c < c_end; c += 256) {
+  const int c_end = min(ld, (by + 1) * 1024);
+  for (int r = bx * 8 + threadIdx.x / 32; r < rows; r += gx * 8)
+  for (int c = by * 1024 + (threadIdx.x % 32) * 8; c < c_end; c += 256) {
     const T* p = w + (size_t)r * cols + c;
     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -1013,6 +1010,36 @@ k_ce_weight(const T* __restrict__ w, int rows, int cols, __half* __restrict__ ou
     }
     *(uint4*)(out + (size_t)r * ld + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (planes == 2) *(uint4*)(out + plane + (size_t)r * ld + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+
+// The operands as the products want them: the first `gather_blocks` blocks pack rows, the others (a grid of
+// gx x ...; none where W is taken as it lies) write W's planes.
+struct PackArgs {
+  const void *hidden, *weight;
+  const uint32_t* targets;
+  const float* weights;
+  float grad_scale;
+  int rows, H, per, gather_blocks, gx;
+  Rows rw;
+  __half* h;
+  int h_ld, plane_rows, h_planes, w_scaled;
+  float* row_loss;
+  __half* w;
+  int w_rows, w_cols, w_ld, w_planes;
+};
+template <typename TH, typename TW>
+__global__ void __launch_bounds__(GATHER_THREADS)
+k_ce_pack(const __grid_constant__ PackArgs a) {
+  ft_pdl_wait();
+  ft_pdl_launch();
+  const int block = blockIdx.x;
+  if (block < a.gather_blocks) {
+    gather_block<TH, __half>(block, a.gather_blocks, (const TH*)a.hidden, a.targets, a.weights, a.grad_scale, a.rows, a.H, a.per,
+                             a.rw, a.h, a.h_ld, a.plane_rows, a.h_planes, a.w_scaled, a.row_loss);
+  } else {
+    const int b = block - a.gather_blocks;
+    weight_block<TW>(b % a.gx, b / a.gx, a.gx, (const TW*)a.weight, a.w_rows, a.w_cols, a.w, a.w_ld, a.w_planes, a.rw.w_max);
   }
 }
 
@@ -1421,17 +1448,23 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   // others hold.
   const bool unpacked = T <= 128 && !t.grad_weight && (!t.grad_hidden || pl.one_piece) && !h32 && !w32 && H % 8 == 0 &&
                         ((uintptr_t)t.hidden & 15) == 0;
-  if (!unpacked) FT_TRY(launch_gather_f16(ctx, q, t, pl.rows, pl.h, pl.h_ld, pl.Tp, pl.h_planes));
-  const void* w = t.weight;
-  if (pl.w_staged) {
-    w = pl.w;
-    const dim3 grid((unsigned)std::min(ft_cdiv(pl.w_rows, 8), ctx->sm_count * 16), (unsigned)ft_cdiv(pl.w_ld, 1024));
-    if (w32)
-      FT_LAUNCH_PDL(ctx, k_ce_weight<float>, grid, 256, 0, (const float*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
-                    pl.w_planes, pl.rows.w_max);
-    else
-      FT_LAUNCH_PDL(ctx, k_ce_weight<__half>, grid, 256, 0, (const __half*)t.weight, pl.w_rows, pl.w_cols, pl.w, pl.w_ld,
-                    pl.w_planes, pl.rows.w_max);
+  const void* w = pl.w_staged ? pl.w : t.weight;
+  if (!unpacked || pl.w_staged) {
+    PackArgs a = {};
+    a.hidden = t.hidden; a.weight = t.weight; a.targets = t.targets; a.weights = t.weights;
+    a.grad_scale = q.p.grad_scale;
+    a.rows = T; a.H = H; a.per = gather_rows(T);
+    a.rw = pl.rows;
+    a.h = pl.h; a.h_ld = pl.h_ld; a.plane_rows = pl.Tp; a.h_planes = pl.h_planes; a.w_scaled = w32 ? 1 : 0;
+    a.row_loss = t.row_loss;
+    a.w = pl.w; a.w_rows = pl.w_rows; a.w_cols = pl.w_cols; a.w_ld = pl.w_ld; a.w_planes = pl.w_planes;
+    a.gather_blocks = unpacked ? 0 : ft_cdiv(T, a.per);
+    a.gx = std::min(ft_cdiv(pl.w_rows, 8), ctx->sm_count * 16);
+    const int blocks = a.gather_blocks + (pl.w_staged ? a.gx * ft_cdiv(pl.w_ld, 1024) : 0);
+    if (h32 && w32) FT_LAUNCH_PDL(ctx, (k_ce_pack<float, float>), blocks, GATHER_THREADS, 0, a);
+    else if (h32) FT_LAUNCH_PDL(ctx, (k_ce_pack<float, __half>), blocks, GATHER_THREADS, 0, a);
+    else if (w32) FT_LAUNCH_PDL(ctx, (k_ce_pack<__half, float>), blocks, GATHER_THREADS, 0, a);
+    else FT_LAUNCH_PDL(ctx, (k_ce_pack<__half, __half>), blocks, GATHER_THREADS, 0, a);
   }
   // K-contiguous operands come in boxes of 64 x 128 rows (B: half a tile's columns), M/N-contiguous ones
   // in two of 64 x 64

@@ -223,9 +223,11 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  *   grad_weight grad_weight_type, shaped like the weight, or NULL
  * The context's GEMM mode chooses the arithmetic of the products: FT_GEMM_F32 exact f32 FMA,
  * FT_GEMM_F16 operands and g rounded to f16, FT_GEMM_F16X2 f32 operands and g carried as two f16
- * halves.  (f16 operands are exact in every mode; sums are f32 in every mode.)
+ * halves.  (f16 operands are exact in every mode; sums are f32 in every mode.)  Calls of at most 16
+ * rows may be computed on f32 FMA in any mode, where that is the faster way.
  * The vocabulary is worked through in pieces of vocab_piece columns (0: chosen by size), of which
- * only one piece of g exists at a time; workspace holds it and must have the bytes that
+ * only one piece of g exists at a time (with 0, at most 16 rows may have all their logits kept
+ * there, 64 bytes a column); workspace holds it and must have the bytes that
  * ft_linear_cross_entropy_workspace gives for the same arguments, context and GEMM mode (of the
  * weight it looks at the alignment alone).  The
  * call allocates nothing, keeps nothing there for a later call, and may be captured into a

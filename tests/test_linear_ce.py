@@ -637,3 +637,44 @@ def test_few_rows_agree_with_many(cuda_ctx, eng):
             tol = _bounds(q, "F32", (F32, F32), (F32, F32))
             few = _call(cuda_ctx, eng, "F32", x[r], w, y[r], a[r], 1.0, vocab_major, want="hidden")
             assert ((few[0] - many[0][r]).abs() <= 2 * tol[0]).all() and ((few[1] - many[1][r]).abs() <= 2 * tol[1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("vocab_major", [False, True])
+def test_few_rows_captured(eng, mode, vocab_major):
+    """A graph of a call of five rows follows its inputs, which rows are skipped included."""
+    from ferrotensor_b200.engine import ComputeEngine, CudaContext, DType, GemmMode, UnifiedTensor
+    first, second = (_make(5, 72, 1900, (F32, F32), vocab_major, "none", 61 + k) for k in range(2))
+    second[2][3] = SKIP
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ctx = CudaContext(0)
+    ctx.set_gemm_mode(GemmMode[mode])
+    e = ComputeEngine(ctx)
+    x, w, y, a = (v.clone() for v in first)
+    y = _targets(y)
+    loss, gh, gw = torch.empty(5, device="cuda"), torch.empty_like(x), torch.empty_like(w)
+    n = e.linear_cross_entropy_workspace(ctx, _ut(x), _ut(w), _ut(gh), _ut(gw), vocab_major=vocab_major)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    f = e.linear_cross_entropy_bt if vocab_major else e.linear_cross_entropy
+
+    def call():
+        f(ctx, _ut(x), _ut(w), _ut(y), _ut(a), _ut(loss), _ut(gh), _ut(gw), 1.0, workspace=UnifiedTensor(ws, [n // 4], DType.U32))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        call()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            call()
+    torch.cuda.synchronize()
+    for to, new in ((x, second[0]), (w, second[1]), (y, _targets(second[2])), (a, second[3])):
+        to.copy_(new)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph.replay()
+        graph.replay()
+    torch.cuda.synchronize()
+    q = _truth(second[0], second[1], second[2], second[3], 1.0, vocab_major)
+    _check((loss, gh, gw), q, _bounds(q, mode, (F32, F32), (F32, F32)), vocab_major)
