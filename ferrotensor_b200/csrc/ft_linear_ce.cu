@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "ft_linear_ce.cuh"
+#include "ft_tc.cuh"
 
 namespace {
 
@@ -116,7 +117,8 @@ k_ce_exact(ExactProduct p, const Head* __restrict__ head) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+        for (int j = 0; j < 8; j += 2)
+          ft_tc::ffma2(acc[i][j], acc[i][j + 1], av[i], av[i], bv[j], bv[j + 1], acc[i][j], acc[i][j + 1]);
     }
     if (k0 + EK < k_end) settle(buf ^ 1);
     __syncthreads();
