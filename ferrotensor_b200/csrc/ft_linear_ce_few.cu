@@ -22,10 +22,12 @@
 #include <math.h>
 
 #include "ft_linear_ce.cuh"
+#include "ft_tc.cuh"
 
 namespace {
 
 using namespace ft_ce;
+using ft_tc::ffma2;
 
 constexpr int MAX_ROWS = 16;
 constexpr int THREADS = 512, WARPS = THREADS / 32;
@@ -131,6 +133,7 @@ template <typename TW, int TR, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1)
 k_ce_few_logits_vh(const FewArgs a) {
   constexpr int VR = TR == 4 ? 8 : 4, N = TR * VR, NV = N / 32;
+  // A pair of rows side by side, for packed pairs of multiply-adds: value (t, k) at [t / 2][k / 2 % 2][k / 4][k % 2][t % 2].
   extern __shared__ __align__(16) float hs[];                        // [TR][ld]
   __shared__ float2 red[WARPS][TR];
   ft_pdl_wait();
@@ -141,7 +144,7 @@ k_ce_few_logits_vh(const FewArgs a) {
   for (int t = 0; t < TR; ++t) {
     const bool live = t < a.T && a.targets[t] != FT_MASKED_CE_SKIP;
 #pragma unroll 4
-    for (int k = threadIdx.x; k < ld; k += THREADS) hs[t * ld + k] = live && k < H ? value_at(a.hidden, a.h16, (size_t)t * H + k) : 0.f;
+    for (int k = threadIdx.x; k < ld; k += THREADS) hs[(t / 2 * 2 + k / 2 % 2) * ld + k / 4 * 4 + k % 2 * 2 + t % 2] = live && k < H ? value_at(a.hidden, a.h16, (size_t)t * H + k) : 0.f;
   }
   __syncthreads();
   const int t = lane * NV / VR, r0 = lane * NV % VR;                 // what a lane has of a warp's sums
@@ -165,12 +168,15 @@ k_ce_few_logits_vh(const FewArgs a) {
         x[r].load(w + row_at[r] + k, H - k);
       }
 #pragma unroll
-      for (int i = 0; i < TR; ++i) {
-        const float4 h = *(const float4*)(hs + i * ld + k);
+      for (int i = 0; i < TR; i += 2) {
+        const float4 h0 = *(const float4*)(hs + i * ld + k), h1 = *(const float4*)(hs + (i + 1) * ld + k);
 #pragma unroll
         for (int r = 0; r < VR; ++r) {
-          float& c = acc[i * VR + r];
-          c = fmaf(h.x, x[r].at(0), c); c = fmaf(h.y, x[r].at(1), c); c = fmaf(h.z, x[r].at(2), c); c = fmaf(h.w, x[r].at(3), c);
+          float &c = acc[i * VR + r], &d = acc[(i + 1) * VR + r];
+          ffma2(c, d, h0.x, h0.y, x[r].at(0), x[r].at(0), c, d);
+          ffma2(c, d, h0.z, h0.w, x[r].at(1), x[r].at(1), c, d);
+          ffma2(c, d, h1.x, h1.y, x[r].at(2), x[r].at(2), c, d);
+          ffma2(c, d, h1.z, h1.w, x[r].at(3), x[r].at(3), c, d);
         }
       }
     }
@@ -265,6 +271,7 @@ k_ce_few_logits_hv(const FewArgs a) {
           const float4 h = *(const float4*)(hs + k * TR + 4 * q);
 #pragma unroll
           for (int j = 0; j < COLS; ++j) {
+            // (packed pairs cost 8% here: four columns of 16 rows leave them no registers)
             acc[4 * q][j] = fmaf(h.x, x[j], acc[4 * q][j]);
             acc[4 * q + 1][j] = fmaf(h.y, x[j], acc[4 * q + 1][j]);
             acc[4 * q + 2][j] = fmaf(h.z, x[j], acc[4 * q + 2][j]);
@@ -402,26 +409,30 @@ k_ce_few_grad_vh(const FewArgs a) {
       const int v = warp + WARPS * u;
       const bool on = v0 + v < v_end && c < H;
       const size_t at = (size_t)(v0 + v) * H + c;
-      float o[COLS];
+      float o[COLS], o2[COLS];                                       // of even and odd rows
 #pragma unroll
-      for (int j = 0; j < COLS; ++j) o[j] = 0.f;
+      for (int j = 0; j < COLS; ++j) o[j] = o2[j] = 0.f;
 #pragma unroll
       for (int q = 0; q < TR; q += 4) {
         const float4 e = *(const float4*)&g[buf][v][q];
-        const float gv[4] = {e.x, e.y, e.z, e.w};
         if (dw) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < COLS; ++j) o[j] = fmaf(gv[i], h[q + i][j], o[j]);
+          for (int j = 0; j < COLS; ++j) {
+            ffma2(o[j], o2[j], e.x, e.y, h[q][j], h[q + 1][j], o[j], o2[j]);
+            ffma2(o[j], o2[j], e.z, e.w, h[q + 2][j], h[q + 3][j], o[j], o2[j]);
+          }
         }
         if (dh && on) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < COLS; ++j) acc[q + i][j] = fmaf(gv[i], x[u].at(j), acc[q + i][j]);
+          for (int j = 0; j < COLS; ++j) {
+            const float w = x[u].at(j);
+            ffma2(acc[q][j], acc[q + 1][j], e.x, e.y, w, w, acc[q][j], acc[q + 1][j]);
+            ffma2(acc[q + 2][j], acc[q + 3][j], e.z, e.w, w, w, acc[q + 2][j], acc[q + 3][j]);
+          }
         }
       }
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) o[j] += o2[j];
       load_w(v0 + SUB, u);
       if (dw && on) {
         if (VEC && !a.dw16) {
@@ -497,18 +508,23 @@ k_ce_few_grad_hv(const FewArgs a) {
           for (int t = 0; t < TR; ++t) e[t] = g[t * a.slice + v];
           if (dh) {
 #pragma unroll
-            for (int p = 0; p < HP; ++p)
+            for (int p = 0; p < HP; ++p) {
+              const float w = x[u][p].at(0);
 #pragma unroll
-              for (int t = 0; t < TR; ++t) acc[p * TR + t] = fmaf(e[t], x[u][p].at(0), acc[p * TR + t]);
+              for (int t = 0; t < TR; t += 2) {
+                float &c = acc[p * TR + t], &d = acc[p * TR + t + 1];
+                ffma2(c, d, e[t], e[t + 1], w, w, c, d);
+              }
+            }
           }
           if (dw) {
 #pragma unroll
             for (int p = 0; p < HP; ++p) {
               if (k + p >= H) break;
-              float o = 0.f;
+              float o = 0.f, o2 = 0.f;                               // of even and odd rows
 #pragma unroll
-              for (int t = 0; t < TR; ++t) o = fmaf(e[t], h[t][p], o);
-              put(a, first + (size_t)p * V + v, o);
+              for (int t = 0; t < TR; t += 2) ffma2(o, o2, e[t], e[t + 1], h[t][p], h[t + 1][p], o, o2);
+              put(a, first + (size_t)p * V + v, o + o2);
             }
           }
         }
