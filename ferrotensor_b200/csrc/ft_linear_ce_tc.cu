@@ -988,6 +988,38 @@ k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* _
   }
 }
 
+// Eight values from any place of a tensor that begins at `first`, of which the first n are there; the rest are zeros.
+__device__ __forceinline__ void load_eight(const float* p, const float*, int n, float (&v)[8]) {
+  if (n >= 8 && ((uintptr_t)p & 15) == 0) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < n ? p[k] : 0.f;
+}
+// f16 rows of an odd length begin between two words: whole words, shifted (the neighbours that come along
+// are values of the same tensor)
+__device__ __forceinline__ void load_eight(const __half* p, const __half* first, int n, float (&v)[8]) {
+  if (n > 8 && p > first) {
+    const bool odd = (uintptr_t)p & 2;
+    const uint32_t* q = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+    uint32_t w[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = k < 4 || odd ? q[k] : 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t x = odd ? __funnelshift_r(w[k], w[k + 1], 16) : w[k];
+      const float2 f = __half22float2(*(const __half2*)&x);
+      v[2 * k] = f.x;
+      v[2 * k + 1] = f.y;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < n ? (float)p[k] : 0.f;
+}
+
 // W [rows, cols] -> f16 planes [planes][rows][ld], times the power of two of its largest value; block
 // (bx, by) of (gx, ...): a warp takes 1024 columns of a row
 template <typename T>
@@ -999,11 +1031,12 @@ __device__ __forceinline__ void weight_block(int bx, int by, int gx, const T* __
   const int c_end = min(ld, (by + 1) * 1024);
   for (int r = bx * 8 + threadIdx.x / 32; r < rows; r += gx * 8)
   for (int c = by * 1024 + (threadIdx.x % 32) * 8; c < c_end; c += 256) {
-    const T* p = w + (size_t)r * cols + c;
+    float v[8];
+    load_eight(w + (size_t)r * cols + c, w, cols - c, v);
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
-      const float a = c + k < cols ? (float)p[k] * S : 0.f, b = c + k + 1 < cols ? (float)p[k + 1] * S : 0.f;
+      const float a = v[k] * S, b = v[k + 1] * S;
       hi[k >> 1] = pack_h2(a, b);
       const float2 f = __half22float2(*(const __half2*)&hi[k >> 1]);
       lo[k >> 1] = pack_h2(a - f.x, b - f.y);
