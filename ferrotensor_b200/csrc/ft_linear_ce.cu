@@ -32,7 +32,7 @@ k_ce_gather(const TH* __restrict__ hidden, const uint32_t* __restrict__ targets,
             float grad_scale, int rows, int H, int per, Rows rw, float* __restrict__ out, float* __restrict__ row_loss) {
   ft_pdl_wait();
   ft_pdl_launch();
-  gather_block<TH, float>(blockIdx.x, gridDim.x, hidden, targets, weights, grad_scale, rows, H, per, rw, out, H, rows, 1, 0,
+  gather_block<TH, float>(blockIdx.x, gridDim.x, hidden, targets, weights, grad_scale, rows, H, per, rw, out, H, rows, 1, 0, 0,
                           row_loss);
 }
 

@@ -939,7 +939,7 @@ k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __res
   }
 }
 
-// Largest finite magnitudes of W (first `w_blocks` blocks, AMAX_BLOCKS or none) and of the supervised rows
+// Largest finite magnitudes of W (first `w_blocks` blocks) and of the supervised rows
 // (the others), one value a block.
 __global__ void __launch_bounds__(256)
 k_ce_amax(const float* __restrict__ w, long long n, int w_blocks, const float* __restrict__ hidden,
@@ -1024,9 +1024,10 @@ __device__ __forceinline__ void load_eight(const __half* p, const __half* first,
 // (bx, by) of (gx, ...): a warp takes 1024 columns of a row
 template <typename T>
 __device__ __forceinline__ void weight_block(int bx, int by, int gx, const T* __restrict__ w, int rows, int cols,
-                                             __half* __restrict__ out, int ld, int planes, const float* __restrict__ w_max) {
+                                             __half* __restrict__ out, int ld, int planes, const float* __restrict__ w_max,
+                                             int w_parts) {
   __shared__ float red[8];
-  const float S = sizeof(T) == 4 ? power_for(block_max_of(w_max, AMAX_BLOCKS, red), OPERAND_EXP) : 1.f;
+  const float S = sizeof(T) == 4 ? power_for(block_max_of(w_max, w_parts, red), OPERAND_EXP) : 1.f;
   const size_t plane = (size_t)rows * ld;
   const int c_end = min(ld, (by + 1) * 1024);
   for (int r = bx * 8 + threadIdx.x / 32; r < rows; r += gx * 8)
@@ -1056,7 +1057,7 @@ struct PackArgs {
   int rows, H, per, gather_blocks, gx;
   Rows rw;
   __half* h;
-  int h_ld, plane_rows, h_planes, w_scaled;
+  int h_ld, plane_rows, h_planes, h_parts, w_parts;
   float* row_loss;
   __half* w;
   int w_rows, w_cols, w_ld, w_planes;
@@ -1069,10 +1070,11 @@ k_ce_pack(const __grid_constant__ PackArgs a) {
   const int block = blockIdx.x;
   if (block < a.gather_blocks) {
     gather_block<TH, __half>(block, a.gather_blocks, (const TH*)a.hidden, a.targets, a.weights, a.grad_scale, a.rows, a.H, a.per,
-                             a.rw, a.h, a.h_ld, a.plane_rows, a.h_planes, a.w_scaled, a.row_loss);
+                             a.rw, a.h, a.h_ld, a.plane_rows, a.h_planes, a.h_parts, a.w_parts, a.row_loss);
   } else {
     const int b = block - a.gather_blocks;
-    weight_block<TW>(b % a.gx, b / a.gx, a.gx, (const TW*)a.weight, a.w_rows, a.w_cols, a.w, a.w_ld, a.w_planes, a.rw.w_max);
+    weight_block<TW>(b % a.gx, b / a.gx, a.gx, (const TW*)a.weight, a.w_rows, a.w_cols, a.w, a.w_ld, a.w_planes, a.rw.w_max,
+                     a.w_parts);
   }
 }
 
@@ -1472,9 +1474,10 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   // (3072 of 4096 f32 rows x 960 x 49152: 419 -> 407 us)
   if (!h32 || t.grad_weight) pl.rows.unscale = nullptr;
   const bool h_scan = h32 && t.grad_weight;
-  if (h_scan || w32) {
-    const int wb = w32 ? AMAX_BLOCKS : 0, hb = h_scan ? AMAX_BLOCKS : 0;
-    FT_LAUNCH_PDL(ctx, k_ce_amax, wb + hb, 256, 0, (const float*)t.weight, (long long)pl.w_rows * pl.w_cols, wb,
+  const long long w_values = (long long)pl.w_rows * pl.w_cols;
+  const int wb = w32 ? (int)std::min<long long>(AMAX_BLOCKS, ft_cdiv(w_values, 4096)) : 0, hb = h_scan ? std::min(T, AMAX_BLOCKS) : 0;
+  if (wb + hb) {
+    FT_LAUNCH_PDL(ctx, k_ce_amax, wb + hb, 256, 0, (const float*)t.weight, w_values, wb,
                   (const float*)t.hidden, t.targets, T, H, pl.rows);
   }
   // One tile of rows and no dW: packing would save nothing, and what a row gets is its own whatever the
@@ -1488,7 +1491,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     a.grad_scale = q.p.grad_scale;
     a.rows = T; a.H = H; a.per = gather_rows(T);
     a.rw = pl.rows;
-    a.h = pl.h; a.h_ld = pl.h_ld; a.plane_rows = pl.Tp; a.h_planes = pl.h_planes; a.w_scaled = w32 ? 1 : 0;
+    a.h = pl.h; a.h_ld = pl.h_ld; a.plane_rows = pl.Tp; a.h_planes = pl.h_planes; a.h_parts = hb; a.w_parts = wb;
     a.row_loss = t.row_loss;
     a.w = pl.w; a.w_rows = pl.w_rows; a.w_cols = pl.w_cols; a.w_ld = pl.w_ld; a.w_planes = pl.w_planes;
     a.gather_blocks = unpacked ? 0 : ft_cdiv(T, a.per);
