@@ -600,7 +600,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             stage_f32(st, lane, v);
             __syncwarp();
             if (c0 + lane < g.N) {
-              for (int r = 0; r < 32 && y0 + r < rows_end; ++r) {
+#pragma unroll 8
+              for (int r = 0; r < 32; ++r) {
+                if (y0 + r >= rows_end) break;
                 const float x = *(const float*)(st + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
                 const long long at = (long long)(g.out_y0 + y0 + r) * g.direct_ld + g.out_x0 + c0 + lane;
                 if (g.out_type == FT_TYPE_F16) ((__half*)g.direct)[at] = __float2half_rn(x);
@@ -775,7 +777,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (EPI != EPI_STATS || !g.carry) g.part[(size_t)(un.nt * PARTS + grp) * g.part_ld + row] = make_float2(run_m, run_s);
       }
     }
-    if (EPI == EPI_STATS && g.carry) {
+    if (EPI == EPI_STATS && g.carry && pair < units) {
       const int row = (int)rank * 128 + quad * 32 + lane;
       g.part[(size_t)(pair * PARTS + grp) * g.part_ld + row] = make_float2(run_m, run_s);
     }
@@ -896,8 +898,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
 
 // E -> g in place, both planes, for a vocabulary that is one piece: g = w (2^(ref - lse) E - onehot), with the
 // gradient at the target from the row's loss (as k_ce_join has it), and zero rows up to a K block of dW.
-// One read and one write of E against a second product for the logits: from hidden = 300 or so on
-// the cheaper way.  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
+// One read and one write of E against a second product for the logits (makes_g_in_place).  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
 __global__ void __launch_bounds__(256)
 k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __restrict__ part, int part_ld, Rows rw, int cols,
                int tile_parts, const float* __restrict__ row_loss) {
@@ -1316,8 +1317,10 @@ int launch_gemm(FtContext* ctx, const CUtensorMap& a, const CUtensorMap& b, cons
     ready[ctx->device] = true;
   }
   const long long units = (long long)ft_cdiv(g.M, CTAS * 128) * ft_cdiv(g.N, g.tile_n) * g.splits;
-  const int workers = (int)std::max<long long>(1, std::min<long long>(units, most[ctx->device]));
-  if (workers_used) *workers_used = workers;
+  // the targets' logits want a warp a row, of two a CTA, however few tiles there are
+  const long long wanted = EPI <= EPI_EXP ? std::max(units, (long long)ft_cdiv(g.M, 2 * CTAS * g.pieces)) : units;
+  const int workers = (int)std::max<long long>(1, std::min<long long>(wanted, most[ctx->device]));
+  if (workers_used) *workers_used = (int)std::min<long long>(units, workers);   // that have a tile
   const char* const names[5] = {"k_ce_gemm<statistics>", "k_ce_gemm<E>", "k_ce_gemm<g>",
                                 A_MN ? "k_ce_gemm<dW>" : "k_ce_gemm<dh>", "k_ce_gemm<dh of E>"};
   if (ctx->profile_all) ft_prof_begin(ctx, names[EPI]);
@@ -1361,6 +1364,15 @@ void set_terms(TcProduct& g, int pa, int pb) {
 // piece (805 MB: half of the logits in f32), 2048 x 896 x 151936 2.34, 2.17, 2.10 and 2.05.
 constexpr size_t G_PIECE_BYTES = (size_t)512 << 20;
 
+// Where g is made of E in place and not of a second product for the logits, in the split mode: from hidden =
+// 320 or so on (512 rows x 128 x 49152, both gradients: 176 us in place, 160 by the product; hidden 256: 212 and
+// 207, 384: 271 and 290; 7002 x 128 x 15104: 508 and 416), and always for few rows, where E stays in L2 (200 x 256 x
+// 15104: 64 and 71).
+bool makes_g_in_place(int rows, int hidden) { return hidden > 256 || rows <= 256; }
+// Up to here one launch after E W costs less than one before it and one after (150 rows x 832 x 2048: 34 against
+// 36 us; 1000 x 832 x 15104: 80 both ways; 7002 x 128 x 15104: 180 against 163).
+constexpr int FINISH_ROWS = 1024;
+
 struct TcPlan {
   Rows rows;
   __half *h, *w, *grad, *wy;
@@ -1369,7 +1381,9 @@ struct TcPlan {
   int Tp, h_ld, h_planes, w_ld, w_planes, w_rows, w_cols, g_planes, piece, splits, acc_ld;
   int stat_n, out_n;         // columns of a tile: of the statistics alone, of dh and (vocab-major) dW
   int tile_m;                // rows of a tile of the products whose rows are the packed ones
-  bool pair, w_staged, by_exp, one_piece, in_place;   // in_place: g is made of E, see k_ce_normalise
+  bool pair, w_staged, by_exp, one_piece;
+  bool in_place;             // g is made of E, see k_ce_normalise
+  bool finish;               // of E W alone: k_ce_finish does what is left
   size_t bytes;
 };
 
@@ -1418,7 +1432,8 @@ TcPlan tc_plan(const FtContext* ctx, const Problem& q, const void* weight, void*
     pl.piece = (int)ft_align_up((size_t)ft_cdiv(q.V, pieces), TILE);
     grad_bytes = column * pl.piece;
     pl.one_piece = pieces == 1;
-    pl.in_place = two && q.grad_weight && pl.one_piece;
+    pl.in_place = two && q.grad_weight && pl.one_piece && makes_g_in_place(q.T, q.H);
+    pl.finish = pl.one_piece && q.T <= FINISH_ROWS;
     if (pl.by_exp || pl.in_place) part_bytes = (size_t)parts_of(EPI_EXP, two, pl.pair) * (pl.piece / TILE) * pl.Tp * sizeof(float2);
   }
   if (pl.by_exp || pl.in_place) {
@@ -1482,7 +1497,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   }
   // One tile of rows and no dW: packing would save nothing, and what a row gets is its own whatever the
   // others hold.
-  const bool unpacked = T <= 128 && !t.grad_weight && (!t.grad_hidden || pl.one_piece) && !h32 && !w32 && H % 8 == 0 &&
+  const bool unpacked = T <= 128 && !t.grad_weight && (!t.grad_hidden || pl.finish) && !h32 && !w32 && H % 8 == 0 &&
                         ((uintptr_t)t.hidden & 15) == 0;
   const void* w = pl.w_staged ? pl.w : t.weight;
   if (!unpacked || pl.w_staged) {
@@ -1559,7 +1574,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
     p.part = pl.part; p.part_ld = pl.Tp;
     p.unpacked = unpacked ? 1 : 0;
-    p.base_out = pl.by_exp && pl.one_piece ? pl.base : nullptr;
+    p.base_out = pl.by_exp && pl.finish ? pl.base : nullptr;
     tile(p, pl.pair, pl.out_n, a_rows, vm);
     return p;
   };
@@ -1573,14 +1588,14 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       z.N = cols; z.v0 = v0; z.b_mn0 = v0; z.piece = v0 / pl.piece;
       FT_TRY(launch_rows<EPI_EXP>(ctx, pl.pair, !vm, two, h_k, vm ? w_k : w_mn, g_out, z));
       const int parts = parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(cols, TILE);
-      if (!pl.one_piece)
+      if (!pl.finish)
         FT_LAUNCH_PDL(ctx, k_ce_join, join_grid, join_threads(parts), 0, pl.part, pl.Tp, parts,
                       pl.rows, 0, first ? 1 : 0, last ? 1 : 0, V, t.row_loss, pl.acc, slab, pl.splits, pl.acc_ld, H);
       if (first || cols != pl.piece) FT_TRY(k_map(&g_k, pl.grad, cols, pl.Tp, pl.g_planes, pl.piece, a_rows));
       const TcProduct p = dh_product(v0, cols);
       FT_TRY(launch_rows<EPI_FACTOR>(ctx, pl.pair, vm, two, g_k, vm ? w_mn : w_k, acc_out, p));
     }
-    if (pl.one_piece) {
+    if (pl.finish) {
       const int parts = parts_of(EPI_EXP, two, pl.pair) * ft_cdiv(V, TILE), across = T <= 32 ? ft_cdiv(pl.acc_ld, 256) : 1;
       const dim3 grid((unsigned)ft_cdiv(T, 4), (unsigned)across);
       const size_t plane = (size_t)pl.Tp * pl.h_ld;
