@@ -198,7 +198,7 @@ __device__ __forceinline__ void scale_chunk(const TI* x, TO* out, uint32_t n, fl
 }
 
 // What follows from the sum of squares.
-struct Verdict {
+struct Outcome {
   float norm, factor;
   bool finite;
   __device__ __forceinline__ void publish(float* o) const {
@@ -207,9 +207,9 @@ struct Verdict {
     o[2] = factor;
   }
 };
-__device__ __forceinline__ Verdict judge(double squares, float grad_scale, float max_norm) {
+__device__ __forceinline__ Outcome decide(double squares, float grad_scale, float max_norm) {
   const double norm = sqrt(squares) * fabs((double)grad_scale);
-  Verdict d;
+  Outcome d;
   d.norm = (float)norm;
   d.finite = isfinite(d.norm);
   d.factor = grad_scale;
@@ -231,7 +231,7 @@ k_list_scale(const Chunk* __restrict__ chunks, const Chunk* __restrict__ out, in
   ft_pdl_launch();
   double acc = 0.0;
   for (int i = threadIdx.x; i < parts; i += LIST_THREADS) acc += partials[i];
-  const Verdict d = judge(block_sum_f64(acc, red), grad_scale, max_norm);
+  const Outcome d = decide(block_sum_f64(acc, red), grad_scale, max_norm);
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) d.publish(norm_out);
   if (!out || !d.finite || (in_place && d.factor == 1.0f)) return;
   const float factor = d.factor;
@@ -295,7 +295,7 @@ k_list_small(const Chunk* __restrict__ chunks, const Chunk* __restrict__ out, in
   double sum = red[lane];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const Verdict d = judge(sum, grad_scale, max_norm);
+  const Outcome d = decide(sum, grad_scale, max_norm);
   if (threadIdx.x == 0 && norm_out) d.publish(norm_out);
   if (!out || !d.finite || (in_place && d.factor == 1.0f)) return;
 #pragma unroll

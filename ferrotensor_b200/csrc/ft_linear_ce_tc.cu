@@ -1486,7 +1486,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
   const bool vm = q.p.weight_vocab_major != 0, two = pl.g_planes == 2;
   const bool h32 = q.p.hidden_type == FT_TYPE_F32, w32 = q.p.weight_type == FT_TYPE_F32;
   // dW sums over the rows, which then need one scale, found by a pass of its own; else a row has its own
-  // (3072 of 4096 f32 rows x 960 x 49152: 419 -> 407 us)
+  // (4096 f32 rows, a quarter of them skipped, x 960 x 49152: 419 -> 407 us)
   if (!h32 || t.grad_weight) pl.rows.unscale = nullptr;
   const bool h_scan = h32 && t.grad_weight;
   const long long w_values = (long long)pl.w_rows * pl.w_cols;
