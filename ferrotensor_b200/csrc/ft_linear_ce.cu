@@ -13,7 +13,8 @@
 // included) reaches nothing.  How many there are is known on the device alone: launches are sized
 // for all rows, and the kernels read the count.
 //
-// This file holds the entry points, the row bookkeeping and the exact f32 products (FT_GEMM_F32).
+// This file holds the entry points and the exact f32 products (FT_GEMM_F32); ft_linear_ce_tc.cu those on the
+// tensor cores, ft_linear_ce_few.cu the calls of a few rows, ft_linear_ce.cuh the row bookkeeping.
 #include <math.h>
 #include <string.h>
 

@@ -8,8 +8,8 @@
 //   dW       A = g,              B = packed rows  K = rows (turned over for [hidden, vocab] weights)
 //
 // dW's K runs over rows, so its operand g must be normalised, which needs every row's log-sum-exp
-// first: the logits are computed twice (or, in the split mode when the vocabulary is one piece, g is made
-// of E in place).  dh alone does not need that.  The pass that finds the
+// first: the logits are computed twice (or, in the split mode when the vocabulary is one piece and that is
+// cheaper, g is made of E in place).  dh alone does not need that.  The pass that finds the
 // statistics writes E = 2^(z2 - ref) for each column tile (z2 in log2 units, ref the row's maximum in
 // that tile: E has f16's full precision whatever the row's normaliser turns out to be), and the
 // product E W is drained from tensor memory once a tile of K and scaled there, in f32, by the
@@ -24,7 +24,7 @@
 // also sums at most 512 of K in tensor memory and adds the slices up in registers.
 //
 // Roles and barriers as in ft_gemm_tc.cu's pair kernel: warp 0 loads (TMA), warp 1 of the even CTA
-// issues the products, warps 2..9 drain.  Every wait is bounded; a wait that runs out sets the
+// issues the products, the eight or sixteen after them drain, and two more compute the targets' logits.  Every wait is bounded; a wait that runs out sets the
 // status word, and all roles fall through.
 #include <math.h>
 #include <string.h>
