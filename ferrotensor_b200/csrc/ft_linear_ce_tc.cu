@@ -24,8 +24,8 @@
 // also sums at most 512 of K in tensor memory and adds the slices up in registers.
 //
 // Roles and barriers as in ft_gemm_tc.cu's pair kernel: warp 0 loads (TMA), warp 1 of the even CTA
-// issues the products, the eight or sixteen after them drain, and two more compute the targets' logits.  Every wait is bounded; a wait that runs out sets the
-// status word, and all roles fall through.
+// issues the products, the eight or sixteen after them drain, and two more compute the targets' logits.
+// Every wait is bounded; a wait that runs out sets the status word, and all roles fall through.
 #include <math.h>
 #include <string.h>
 
