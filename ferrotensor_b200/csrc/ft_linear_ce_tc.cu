@@ -436,6 +436,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const int rows_end = g.live_m ? live : g.M;
     int local = 0;
     uint32_t quad_phase = 0;
+    uint32_t stored = 0;                                           // STORE: blocks handed to TMA, over all tiles
     float run_m = -INFINITY, run_s = 0.f;
     for (int u = pair; u < units && !*abort_flag; u += npairs) {
       const Unit un = decode_unit(u, tiles_m, tiles_n, g);
@@ -611,8 +612,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
             return;
           }
-          // an f16 block fills half of the staging tile: the halves take turns
-          uint8_t* to = st + (g.out_type == FT_TYPE_F16 ? (i & 1) * 2048 : 0);
+          // An f16 block fills half of the staging tile: the halves take turns, over all tiles and the blocks
+          // left out (with the chunk's number an odd count of them would put two blocks in a row in one
+          // half, and the wait below lets the last copy go on reading).
+          uint8_t* to = st + (g.out_type == FT_TYPE_F16 ? (stored++ & 1) * 2048 : 0);
           if (lane == 0) {
             if (g.out_type == FT_TYPE_F16) bulk_wait_read_but_one();
             else bulk_wait_read();
