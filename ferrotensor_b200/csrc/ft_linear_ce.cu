@@ -183,9 +183,12 @@ k_ce_exact_loss(Rows rw, int vocab, float* __restrict__ row_loss) {
   const int r = blockIdx.x * 256 + threadIdx.x;
   if (r >= rw.head->count) return;
   const float2 st = rw.stat[r];
-  const float lse = finite_max(st.x) + logf(st.y);
-  rw.lse[r] = lse;
-  row_loss[rw.source[r]] = rw.target[r] < (uint32_t)vocab ? lse - rw.picked[r] : 0.f;
+  const float ref = finite_max(st.x), l = logf(st.y);
+  rw.lse[r] = ref + l;
+  // (ref - z) first: a row that is sure of its target loses nothing to the size of its logits
+  const float loss = rw.target[r] < (uint32_t)vocab ? (ref - rw.picked[r]) + l : 0.f;
+  row_loss[rw.source[r]] = loss;
+  rw.at_target[r] = expm1f(-loss);
 }
 
 // logits -> g, in place
@@ -196,11 +199,10 @@ k_ce_exact_grad(float* __restrict__ z, int v0, int cols, Rows rw) {
   const int r = blockIdx.x;
   if (r >= rw.head->count) return;
   float* row = z + (size_t)r * cols;
-  const float lse = rw.lse[r], w = rw.weight[r];
+  const float lse = rw.lse[r], w = rw.weight[r], at_target = w * rw.at_target[r];
   const uint32_t y = rw.target[r] - (uint32_t)v0;
   for (int i = threadIdx.x; i < cols; i += 256) {
-    const float p = expf(row[i] - lse);
-    row[i] = w * ((uint32_t)i == y ? p - 1.0f : p);
+    row[i] = (uint32_t)i == y ? at_target : w * expf(row[i] - lse);
   }
 }
 

@@ -62,6 +62,7 @@ struct Rows {
   float* picked;      // logit of the target
   float* exact;       // the same from f32 products, beside the tensor cores' sum
   float* lse;
+  float* at_target;   // p - 1 at the target, from the loss: -(1 - e^-loss) is exact where 1 - p is small
   float* base;        // E: the point R that the row's sums are scaled against, in log2 units
   float2* kept;       // E: {value, reference point} of the target
 };
@@ -111,6 +112,7 @@ inline Rows carve_rows(Carver& c, int T) {
   r.picked = c.take<float>(T);
   r.exact = c.take<float>(T);
   r.lse = c.take<float>(T);
+  r.at_target = c.take<float>(T);
   r.base = c.take<float>(T);
   r.kept = c.take<float2>(T);
   return r;

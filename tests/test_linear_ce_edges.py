@@ -5,7 +5,7 @@ in 64 bits and the bounds are those of the tests of its values; a tighter bound 
 import pytest
 import torch
 
-from tests.test_linear_ce import F16, _bounds, _call, _check, _make, _truth
+from tests.test_linear_ce import F16, F32, _bounds, _call, _check, _make, _truth
 
 gpu = pytest.mark.gpu
 
@@ -32,3 +32,75 @@ def test_f16_weight_gradients_of_many_tiles(cuda_ctx, eng, mode, vocab_major, ro
     for _ in range(4):
         again = _call(cuda_ctx, eng, mode, x, w, y, a, 512.0, vocab_major, (F16, F16))
         assert all(torch.equal(p, r) for p, r in zip(first, again))
+
+
+def _sure(t, h, v, types, vocab_major, offset, seed):
+    """Rows whose target stands 12 to 20 above a spread of others, all logits `offset` higher than that."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randn((v, h), generator=g, device="cuda") * 0.1
+    w[:, 0] = 32.0 if offset else 0.0
+    y = torch.randint(0, v, (t,), generator=g, device="cuda")
+    rest = w[y].clone()
+    rest[:, 0] = 0.0
+    lift = 12.0 + 8.0 * torch.rand((t, 1), generator=g, device="cuda")
+    x = rest * (lift / rest.square().sum(dim=1, keepdim=True))
+    x[:, 0] = offset / 32.0
+    a = (torch.rand(t, generator=g, device="cuda") + 0.5) / t
+    x, w = x.to(types[0]), w.to(types[1])
+    return x, (w if vocab_major else w.t().contiguous()), y, a
+
+
+def _sure_bounds(q, y, mode, types):
+    """The bounds of the values' tests, but relative for every element of g: one with probability p is wrong by
+    a share of p (its logit's error, against the target's and the sum's), the target's by a share of 1 - p
+    and by the sum of the exponentials, which is f32 near 1 and takes at most v / 64 + 32 roundings in a row.
+    (What is held as f16 is scaled so that the largest lies in 2^13 to 2^14: f16's smallest step, of which a
+    rounding is half, is then at most 2^-37 of the largest, with a second half too.)"""
+    X, W, p, c, g = q["X"].abs(), q["W"].abs(), q["p"], q["c"].abs(), q["g"].abs()
+    (t, h), v = X.shape, W.shape[0]
+    u, u16 = 2.0 ** -24, 2.0 ** -11
+
+    def op(kind, m):
+        if kind is F16 or mode == "F32":
+            return 0.0, 0.0
+        return (u16 if mode == "F16" else 2.0 ** -21), float(m.max()) * 2.0 ** -37
+    (rx, ax), (rw, aw) = op(types[0], X), op(types[1], W)
+    dX, dW_ = rx * X + ax, rw * W + aw
+    dz = dX @ W.t() + X @ dW_.t() + dX @ dW_.t() + (h + 8) * u * (X @ W.t())
+    worst = dz.max(dim=1, keepdim=True).values
+    soft = 2.0 ** -20 + 2 * u * (q["z"].abs().max(dim=1, keepdim=True).values + q["lse"].abs()[:, None])
+    rel = torch.expm1(dz + worst + soft + 2 * u * (q["z"] - q["lse"][:, None]).abs()) + 4 * u
+    at = torch.zeros_like(p, dtype=torch.bool)
+    at[torch.arange(t, device="cuda"), y] = True
+    off = -torch.expm1(-q["loss"])[:, None]
+    sure = off * rel.max(dim=1, keepdim=True).values + (v / 64 + 32) * u
+    loss = (sure / (1 - off))[:, 0] * 1.01 + 2 * u * q["loss"]
+    dg = c * torch.where(at, sure, p * rel)
+    rg = {"F32": 0.0, "F16": u16, "F16X2": 2.0 ** -21}[mode]
+    dg = dg + rg * (g + dg) + (0.0 if mode == "F32" else float(c.max()) * 2.0 ** -37)
+    G = g + dg
+    dh = dg @ (W + dW_) + g @ dW_ + (v + 64) * u * (G @ (W + dW_))
+    dW = dg.t() @ (X + dX) + g.t() @ dX + (t + 64) * u * (G.t() @ (X + dX))
+    return loss, dh + 2 * u * (q["dh"].abs() + dh) + 1e-40, dW + 2 * u * (q["dW"].abs() + dW) + 1e-40
+
+
+def _sure_case(ctx, eng, mode, offset, size, wants):
+    """Loss and gradients keep their relative accuracy where 1 - p is 1e-2 to 1e-5: at the target, and at tokens
+    that share its tile; whatever all logits have in common."""
+    rows, hidden, vocab, piece = size
+    for types in ((F16, F16), (F32, F32)):
+        for vocab_major in (False, True):
+            x, w, y, a = _sure(rows, hidden, vocab, types, vocab_major, offset, 800 + rows)
+            q = _truth(x, w, y, a, 1.0, vocab_major)
+            assert 1e-8 < float(-torch.expm1(-q["loss"]).min()) and float(q["loss"].max()) < 0.2
+            tols = _sure_bounds(q, y, mode, types)
+            for want in wants:
+                got = _call(ctx, eng, mode, x, w, y, a, 1.0, vocab_major, (F32, F32), want, piece)
+                _check(got, q, tols, vocab_major, f"{types} {vocab_major} {want}")
+
+
+@gpu
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+@pytest.mark.parametrize("size", [(16, 64, 3000, 0), (17, 64, 3000, 0), (120, 64, 3000, 0), (300, 64, 3000, 1024), (300, 288, 3000, 0)])
+def test_sure_rows_exact(cuda_ctx, eng, offset, size):
+    _sure_case(cuda_ctx, eng, "F32", offset, size, ("both", "hidden", "none"))
