@@ -153,6 +153,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 2^((v - ref) c2) of a chunk in place, its sum.  (The difference first: 2^(v c2 - ref c2) with a rounded second
+// product is not 1 at the maximum but off by half a step of the logits, 4e-5 at 1000, which a row that is
+// sure of its target has as the error of its loss.)
+__device__ __forceinline__ float exponentials(float (&v)[32], float ref, float c2) {
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 32; k += 2) {
+    fadd2(v[k], v[k + 1], v[k], v[k + 1], -ref, -ref);
+    fmul2(v[k], v[k + 1], v[k], v[k + 1], c2, c2);
+    v[k] = ex2(v[k]);
+    v[k + 1] = ex2(v[k + 1]);
+    s[k & 2] += v[k];
+    s[(k & 2) + 1] += v[k + 1];
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
 // an arrival in every CTA of the tile once the products issued so far are complete
 template <bool PAIR>
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -437,7 +454,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     int local = 0;
     uint32_t quad_phase = 0;
     uint32_t stored = 0;                                           // STORE: blocks handed to TMA, over all tiles
-    float run_m = -INFINITY, run_s = 0.f;
+    float run_m = -INFINITY, run_s = 0.f, run_c2 = 0.f;              // the maximum as the accumulators have it
     for (int u = pair; u < units && !*abort_flag; u += npairs) {
       const Unit un = decode_unit(u, tiles_m, tiles_n, g);
       const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
@@ -473,6 +490,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       // last one are zeros that dW reads)
       const bool idle = (EPI <= EPI_EXP || EPI == EPI_FACTOR) && y0 >= live;
       if (EPI != EPI_STATS || !g.carry || u == pair) { run_m = -INFINITY; run_s = 0.f; }
+      run_c2 = c2;                                                  // (a carried row keeps its scale)
       uint32_t low[TWO && (EPI == EPI_EXP || EPI == EPI_GRAD) ? 2 : 1][16];   // the second plane, until its store
 
       auto mask_columns = [&](int c0, float (&v)[32]) {
@@ -531,13 +549,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t y = target - 32u * (uint32_t)i;
         if constexpr (EPI == EPI_STATS) {
           mask_columns(c0, v);
-          const float m = fmaxf(run_m, max_of(v) * c2);
-          const float ref = finite_max(m);
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < 32; ++k) s[k & 3] += ex2(fmaf(v[k], c2, -ref));
-          run_s = run_s * ex2(run_m - ref) + ((s[0] + s[1]) + (s[2] + s[3]));
-          run_m = m;
+          const float m = fmaxf(run_m, max_of(v));
           if (y < 32u) {
             float z = 0.f;
 #pragma unroll
@@ -545,6 +557,9 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               if (y == (uint32_t)k) z = v[k];
             g.rw.picked[row] = z * c2;
           }
+          const float ref = finite_max(m);
+          run_s = run_s * ex2((run_m - ref) * c2) + exponentials(v, ref, c2);
+          run_m = m;
         } else if constexpr (EPI == EPI_EXP) {
           // (run_m is the whole tile's maximum by now)
           mask_columns(c0, v);
@@ -554,19 +569,13 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (y == (uint32_t)k) z = v[k];
-            const float e = ex2(fmaf(z, c2, -ref));
+            const float e = ex2((z - ref) * c2);
             float kept = __half2float(__float2half_rn(e));         // as the product will see it
             if (TWO) kept += __half2float(__float2half_rn(e - kept));
             g.rw.picked[row] = z * c2;
-            g.rw.kept[row] = make_float2(kept, ref);
+            g.rw.kept[row] = make_float2(kept, ref * c2);
           }
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            v[k] = ex2(fmaf(v[k], c2, -ref));
-            s[k & 3] += v[k];
-          }
-          run_s += (s[0] + s[1]) + (s[2] + s[3]);
+          run_s += exponentials(v, ref, c2);
           put_f16(i, c0, v);
         } else if constexpr (EPI == EPI_GRAD) {
 #pragma unroll
@@ -739,7 +748,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             mask_columns(col + 32 * i, acc[i]);
             m = fmaxf(m, max_of(acc[i]));
           }
-          run_m = join_max(m * c2);
+          run_m = join_max(m);
         }
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i)
@@ -763,7 +772,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             mask_columns(col + 32 * i, v);
             m = fmaxf(m, max_of(v));
           }
-          run_m = join_max(m * c2);
+          run_m = join_max(m);
         }
         if (mine == 0) release(buf);
 #pragma unroll
@@ -777,12 +786,12 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
       }
       if constexpr (EPI <= EPI_EXP) {
-        if (EPI != EPI_STATS || !g.carry) g.part[(size_t)(un.nt * PARTS + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+        if (EPI != EPI_STATS || !g.carry) g.part[(size_t)(un.nt * PARTS + grp) * g.part_ld + row] = make_float2(run_m * c2, run_s);
       }
     }
     if (EPI == EPI_STATS && g.carry && pair < units) {
       const int row = (int)rank * 128 + quad * 32 + lane;
-      g.part[(size_t)(pair * PARTS + grp) * g.part_ld + row] = make_float2(run_m, run_s);
+      g.part[(size_t)(pair * PARTS + grp) * g.part_ld + row] = make_float2(run_m * run_c2, run_s);
     }
     // what was stored is complete before the launch ends
     if (lane == 0) bulk_wait_all();

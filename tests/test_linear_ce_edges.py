@@ -104,3 +104,11 @@ def _sure_case(ctx, eng, mode, offset, size, wants):
 @pytest.mark.parametrize("size", [(16, 64, 3000, 0), (17, 64, 3000, 0), (120, 64, 3000, 0), (300, 64, 3000, 1024), (300, 288, 3000, 0)])
 def test_sure_rows_exact(cuda_ctx, eng, offset, size):
     _sure_case(cuda_ctx, eng, "F32", offset, size, ("both", "hidden", "none"))
+
+
+@gpu
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+@pytest.mark.parametrize("mode", ["F16", "F16X2"])
+@pytest.mark.parametrize("rows", [1, 17, 120, 300, 600])
+def test_sure_rows_losses_alone(cuda_ctx, eng, mode, offset, rows):
+    _sure_case(cuda_ctx, eng, mode, offset, (rows, 64, 3000, 0), ("none",))
