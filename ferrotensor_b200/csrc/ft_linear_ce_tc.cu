@@ -462,7 +462,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       const int row = y0 + lane;
       const int col = un.nt * tile_n + grp * share * 32;            // its first column, from the launch's first
       uint32_t target = FT_MASKED_CE_SKIP;
-      float lse2 = 0.f, wg = 0.f, alpha = 1.f, base2 = 0.f, c2 = c2_all;
+      float lse2 = 0.f, wg = 0.f, g_target = 0.f, alpha = 1.f, base2 = 0.f, c2 = c2_all;
       if constexpr (EPI <= EPI_GRAD) {
         if (row < live) {
           if (EPI <= EPI_EXP && g.rw.unscale) c2 *= g.rw.unscale[row];
@@ -470,6 +470,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if constexpr (EPI == EPI_GRAD) {
             lse2 = g.rw.lse[row];
             wg = g.rw.weight[row] * g.rw.head->g_scale;
+            g_target = wg * g.rw.at_target[row];
           }
         }
       } else if constexpr (EPI == EPI_STORE) {
@@ -580,10 +581,11 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         } else if constexpr (EPI == EPI_GRAD) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
-            v[k] = ex2(fmaf(v[k], c2, -lse2));
-            if (y == (uint32_t)k) v[k] -= 1.f;
+            v[k] = wg * ex2(fmaf(v[k], c2, -lse2));
+            // (p - 1 would be as wrong as the tensor cores' sum: a row that is sure of its target loses it all)
+            if (y == (uint32_t)k) v[k] = g_target;
             // rows behind the last supervised one hold zeros: they are part of dW's K
-            v[k] = row < live ? v[k] * wg : 0.f;
+            if (row >= live) v[k] = 0.f;
           }
           put_f16(i, c0, v);
         } else {
@@ -887,6 +889,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
           loss = loss_of(ref, l2, rw.picked[row], rw.exact[row]);
         }
         row_loss[unpacked_rows ? row : rw.source[row]] = loss;
+        if (!unpacked_rows) rw.at_target[row] = expm1f(-loss);
         if (acc) {
           // the gradient at the target, p - 1, is -(1 - e^-loss), exact for a row that is sure of its
           // target; what E W holds of it already goes off
@@ -909,11 +912,11 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
 }
 
 // E -> g in place, both planes, for a vocabulary that is one piece: g = w (2^(ref - lse) E - onehot), with the
-// gradient at the target from the row's loss (as k_ce_join has it), and zero rows up to a K block of dW.
+// gradient at the target as k_ce_join has it, and zero rows up to a K block of dW.
 // One read and one write of E against a second product for the logits (makes_g_in_place).  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
 __global__ void __launch_bounds__(256)
 k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __restrict__ part, int part_ld, Rows rw, int cols,
-               int tile_parts, const float* __restrict__ row_loss) {
+               int tile_parts) {
   ft_pdl_wait();
   ft_pdl_launch();
   const int live = rw.head->count, end = max(64, (live + 63) / 64 * 64);
@@ -924,7 +927,7 @@ k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __res
       lse2 = rw.lse[r];
       w = rw.weight[r] * rw.head->g_scale;
       y = rw.target[r];
-      at_target = w * expm1f(-row_loss[rw.source[r]]);
+      at_target = w * rw.at_target[r];
     }
     for (int c = (blockIdx.x * 256 + threadIdx.x) * 8; c < cols; c += gridDim.x * 2048) {
       __half* p = e + (size_t)r * ld + c;
@@ -1639,7 +1642,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
                   0, 1, 1, V, t.row_loss, (float*)nullptr, (size_t)0, 0, 0, 0);
     const dim3 grid(ft_cdiv(V, 2048), std::max(1, std::min(pl.Tp, ctx->sm_count * 32 / ft_cdiv(V, 2048))));
     FT_LAUNCH_PDL(ctx, k_ce_normalise, grid, 256, 0, pl.grad, (size_t)pl.Tp * pl.piece, pl.piece, pl.part, pl.Tp, pl.rows, pl.piece,
-                  parts_of(EPI_EXP, two, pl.pair), t.row_loss);
+                  parts_of(EPI_EXP, two, pl.pair));
   } else {
     tile(z, pl.pair, pl.stat_n, a_rows, !vm);
     z.w_early = !pl.w_staged;

@@ -112,3 +112,11 @@ def test_sure_rows_exact(cuda_ctx, eng, offset, size):
 @pytest.mark.parametrize("rows", [1, 17, 120, 300, 600])
 def test_sure_rows_losses_alone(cuda_ctx, eng, mode, offset, rows):
     _sure_case(cuda_ctx, eng, mode, offset, (rows, 64, 3000, 0), ("none",))
+
+
+@gpu
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+@pytest.mark.parametrize("mode,size", [("F16", (16, 64, 3000, 0)), ("F16", (17, 64, 3000, 0)), ("F16", (120, 64, 3000, 0)), ("F16", (300, 288, 3000, 0)),
+                                       ("F16", (140, 64, 3000, 1024)), ("F16X2", (300, 64, 3000, 0)), ("F16X2", (140, 64, 3000, 1024))])
+def test_sure_rows_both_gradients(cuda_ctx, eng, mode, offset, size):
+    _sure_case(cuda_ctx, eng, mode, offset, size, ("both", "none"))
