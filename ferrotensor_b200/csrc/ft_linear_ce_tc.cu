@@ -10,8 +10,9 @@
 // dW's K runs over rows, so its operand g must be normalised, which needs every row's log-sum-exp
 // first: the logits are computed twice (or, in the split mode when the vocabulary is one piece and that is
 // cheaper, g is made of E in place).  dh alone does not need that.  The pass that finds the
-// statistics writes E = 2^(z2 - ref) for each column tile (z2 in log2 units, ref the row's maximum in
-// that tile: E has f16's full precision whatever the row's normaliser turns out to be), and the
+// statistics writes E = 2^(z2 - ref + 14) for each column tile (z2 in log2 units, ref the row's maximum in
+// that tile: E has f16's full precision whatever the row's normaliser turns out to be, down to 2^-28 of
+// that maximum), and the
 // product E W is drained from tensor memory once a tile of K and scaled there, in f32, by the
 // row's 2^(ref - R).  R is the row's maximum when its first piece was done; the rest of the
 // normaliser and the one-hot term, -w W(:, y), are applied by the pass that unpacks the rows.
@@ -19,7 +20,8 @@
 //
 // Planes: an f16 operand, and an f32 one in FT_GEMM_F16, is one f16 plane.  FT_GEMM_F16X2 carries an
 // f32 operand and g (or E) as two planes, hi = f16(x) and lo = f16(x - hi), of which the products
-// hi.hi, hi.lo and lo.hi are summed: 22 bits.  The tensor core adds each group of 16 products into
+// hi.hi, hi.lo and lo.hi are summed: 22 bits, and 2^-38 of the largest for values so small that lo meets
+// f16's smallest step (all are scaled to end near 2^14).  The tensor core adds each group of 16 products into
 // its f32 accumulator with the low bits cut off, a loss of up to K/16 x 2^-24 of the sum, so that mode
 // also sums at most 512 of K in tensor memory and adds the slices up in registers.
 //
@@ -66,6 +68,8 @@ constexpr int bar_offset(int epi, bool two, bool pair) {
 }
 constexpr int BARRIERS = 2 * MAX_STAGES + 2 * MAX_BUFFERS + 4;
 constexpr int smem_bytes(int epi, bool two, bool pair) { return bar_offset(epi, two, pair) + BARRIERS * 8 + 16 + 1024; }
+// what E is held times: unscaled, a token below 2^-14 of its tile's maximum would fall under f16's normal range
+constexpr float E_SCALE = 16384.f;
 // k-blocks of 64 that are summed in tensor memory; 0: all
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
 
@@ -570,13 +574,16 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (y == (uint32_t)k) z = v[k];
-            const float e = ex2((z - ref) * c2);
+            const float e = E_SCALE * ex2((z - ref) * c2);
             float kept = __half2float(__float2half_rn(e));         // as the product will see it
             if (TWO) kept += __half2float(__float2half_rn(e - kept));
+            kept *= 1.f / E_SCALE;
             g.rw.picked[row] = z * c2;
             g.rw.kept[row] = make_float2(kept, ref * c2);
           }
           run_s += exponentials(v, ref, c2);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) fmul2(v[k], v[k + 1], v[k], v[k + 1], E_SCALE, E_SCALE);
           put_f16(i, c0, v);
         } else if constexpr (EPI == EPI_GRAD) {
 #pragma unroll
@@ -712,7 +719,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               for (int j = 0; j < 32 && s0 + SLICE * j < kb1; ++j) {
                 const float m = row < live ? g.part[(size_t)(parts_of(EPI_EXP, false, PAIR) * (s0 / SLICE + j)) * g.part_ld + row].x : 0.f;
                 // (a difference of two infinities belongs to a row of NaN anyway)
-                factors[j * 32 + lane] = ex2(finite_max(m) - base2);
+                factors[j * 32 + lane] = ex2(finite_max(m) - base2) * (1.f / E_SCALE);
               }
             }
             f = factors[at * 32 + lane];
@@ -911,7 +918,7 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
   }
 }
 
-// E -> g in place, both planes, for a vocabulary that is one piece: g = w (2^(ref - lse) E - onehot), with the
+// E -> g in place, both planes, for a vocabulary that is one piece: g = w (2^(ref - lse) 2^-14 E - onehot), with the
 // gradient at the target as k_ce_join has it, and zero rows up to a K block of dW.
 // One read and one write of E against a second product for the logits (makes_g_in_place).  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
 __global__ void __launch_bounds__(256)
@@ -933,7 +940,7 @@ k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __res
       __half* p = e + (size_t)r * ld + c;
       uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
       if (r < live) {
-        const float f = w * ex2(finite_max(part[(size_t)(tile_parts * (c / TILE)) * part_ld + r].x) - lse2);
+        const float f = w * (1.f / E_SCALE) * ex2(finite_max(part[(size_t)(tile_parts * (c / TILE)) * part_ld + r].x) - lse2);
         hi = *(const uint4*)p;
         lo = *(const uint4*)(p + plane);
         uint32_t* a = (uint32_t*)&hi;

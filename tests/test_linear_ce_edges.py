@@ -120,3 +120,18 @@ def test_sure_rows_losses_alone(cuda_ctx, eng, mode, offset, rows):
                                        ("F16", (140, 64, 3000, 1024)), ("F16X2", (300, 64, 3000, 0)), ("F16X2", (140, 64, 3000, 1024))])
 def test_sure_rows_both_gradients(cuda_ctx, eng, mode, offset, size):
     _sure_case(cuda_ctx, eng, mode, offset, size, ("both", "none"))
+
+
+@gpu
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+@pytest.mark.parametrize("mode,size", [(m, z) for m in ("F16", "F16X2") for z in [(16, 64, 3000, 0), (17, 64, 3000, 0), (120, 64, 3000, 0), (300, 288, 3000, 0),
+                                                                                  (140, 64, 3000, 1024), (1100, 64, 3000, 0)]])
+def test_sure_rows_hidden_gradient_alone(cuda_ctx, eng, mode, offset, size):
+    _sure_case(cuda_ctx, eng, mode, offset, size, ("hidden",))
+
+
+@gpu
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+@pytest.mark.parametrize("size", [(17, 64, 3000, 0), (200, 64, 3000, 0), (300, 288, 3000, 0)])
+def test_sure_rows_gradient_made_in_place(cuda_ctx, eng, offset, size):
+    _sure_case(cuda_ctx, eng, "F16X2", offset, size, ("both",))
