@@ -828,7 +828,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 // (ref - z) first: a row that is sure of its target loses nothing to the size of its logits.
 __device__ __forceinline__ float loss_of(float ref, float l2, float z, float exact) {
   const float above = ((ref - z) + l2) * 0.6931471805599453f;
-  const float d = (exact - z) * 0.6931471805599453f;
+  const float d = exact == z ? 0.f : (exact - z) * 0.6931471805599453f;   // (both may be -inf: the loss is +inf)
   return above - d + log1pf(expf(-above) * expm1f(d));
 }
 

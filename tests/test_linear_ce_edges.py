@@ -5,7 +5,7 @@ in 64 bits and the bounds are those of the tests of its values; a tighter bound 
 import pytest
 import torch
 
-from tests.test_linear_ce import F16, F32, _bounds, _call, _check, _make, _truth
+from tests.test_linear_ce import F16, F32, MODES, SKIP, _bounds, _call, _check, _make, _truth
 
 gpu = pytest.mark.gpu
 
@@ -135,3 +135,44 @@ def test_sure_rows_hidden_gradient_alone(cuda_ctx, eng, mode, offset, size):
 @pytest.mark.parametrize("size", [(17, 64, 3000, 0), (200, 64, 3000, 0), (300, 288, 3000, 0)])
 def test_sure_rows_gradient_made_in_place(cuda_ctx, eng, offset, size):
     _sure_case(cuda_ctx, eng, "F16X2", offset, size, ("both",))
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("rows", [3, 17, 100, 300])
+def test_logits_of_minus_infinity(cuda_ctx, eng, mode, rows):
+    """Columns of the vocabulary masked by a weight of -inf: they take no probability, a row whose target is
+    masked has an infinite loss, and dW stays finite (its row pulls the masked column by -w h).  dh, which
+    has 0 x -inf in its sum, is not looked at."""
+    for kind in ((F16,) if mode == "F16X2" else (F16, F32)):
+        x, w, y, a = _make(rows, 40, 700, (kind, kind), True, "none", 51)
+        x[:, 0] = 0.5
+        w[5::7, 0] = float("-inf")
+        y = torch.where(y % 7 == 5, y - 1, y)
+        y[1::2] = 5
+        W, X = w.double(), x.double()
+        z = X @ W.t()
+        keep = torch.ones(700, dtype=torch.bool, device="cuda")
+        keep[5::7] = False
+        finite = dict(zip(("x", "w"), (x, w[keep])))
+        inner = torch.where(y == 5, 0, torch.cumsum(keep, 0)[y] - 1)
+        q = _truth(finite["x"], finite["w"], torch.where(y == 5, SKIP, inner), a, 1.0, True)
+        tols = _bounds(q, mode, (kind, kind), (F32, F32))
+        got = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, True)
+        masked = y == 5
+        assert (z[:, 5] == float("-inf")).all() and (got[0][masked] == float("inf")).all()
+        assert ((got[0].double() - q["loss"]).abs() <= tols[0])[~masked].all()
+        # dW of all rows: the ones with a masked target have the same softmax and no one-hot term inside
+        zk = z[:, keep]
+        p = torch.softmax(zk, dim=1)
+        p[~masked, inner[~masked]] -= 1
+        g = p * a.double()[:, None]
+        full = torch.zeros(700, 40, dtype=torch.float64, device="cuda")
+        full[keep] = g.t() @ X
+        full[5] = -(a.double()[masked] @ X[masked])
+        size = torch.zeros(700, 40, dtype=torch.float64, device="cuda")
+        size[keep] = g.abs().t() @ X.abs()
+        size[5] = a.double()[masked].abs() @ X[masked].abs()
+        # operands and g within half a step of f16 (2^-21 and exact in the other modes), logits within 1e-2 for that
+        rel = {"F32": 1e-4, "F16": 2e-2 if kind is F32 else 2e-3, "F16X2": 1e-4}[mode]
+        assert ((got[2].double() - full).abs() <= rel * size + 1e-7).all()
