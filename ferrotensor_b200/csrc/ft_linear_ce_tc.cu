@@ -157,6 +157,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Accumulator -> logit in log2 units: the operands' scales undone.  Their product may leave f32 at either end where
+// every logit of the row that is neither 0 nor infinite does so too; 0 times a masked -inf, or
+// infinity times 0, would be NaN.
+__device__ __forceinline__ float logit_factor(float scales) {
+  return fminf(fmaxf(scales * 1.4426950408889634f, 1.17549435e-38f), 3.40282347e38f);
+}
+
 // 2^((v - ref) c2) of a chunk in place, its sum.  (The difference first: 2^(v c2 - ref c2) with a rounded second
 // product is not 1 at the maximum but off by half a step of the logits, 4e-5 at 1000, which a row that is
 // sure of its target has as the error of its loss.)
@@ -225,7 +232,7 @@ __device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const
 // so that DRAM reads a row of W once for all targets in it (with a row a warp, 4096 rows x 2048
 // read 540 MB for 100 MB of W and the products waited for them: 390 against 277 us).
 // With g.wy the columns are kept, for the one-hot term of dh.
-__device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, int worker, int workers, float c2, int lane) {
+__device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, int worker, int workers, float scale, int lane) {
   const int rows = r1 - r0;
   int R = 1;
   if (g.w_sk != 1)
@@ -273,7 +280,7 @@ __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, 
       }
     }
     for (int o = share / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (sub == 0 && on) g.rw.exact[r] = acc * (g.rw.unscale ? c2 * g.rw.unscale[r] : c2);
+    if (sub == 0 && on) g.rw.exact[r] = acc * logit_factor(g.rw.unscale ? scale * g.rw.unscale[r] : scale);
   }
 }
 
@@ -439,10 +446,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     __syncwarp();
   } else if (EPI <= EPI_EXP && warp >= 2 + WARPS) {
     // ------------------------------------------------------------------ the targets' logits
-    const float c2 = (unpacked ? 1.f : g.rw.head->z_scale) * 1.4426950408889634f;
+    const float scale = unpacked ? 1.f : g.rw.head->z_scale;
     // each launch of a vocabulary in pieces takes its share of the rows
     const int r0 = (int)((long long)live * g.piece / g.pieces), r1 = (int)((long long)live * (g.piece + 1) / g.pieces);
-    target_dots(g, r0, r1, (int)blockIdx.x * 2 + warp - 2 - WARPS, (int)gridDim.x * 2, c2, lane);
+    target_dots(g, r0, r1, (int)blockIdx.x * 2 + warp - 2 - WARPS, (int)gridDim.x * 2, scale, lane);
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
     // A warp reaches the 32 TMEM lanes (rows) of its quadrant; the warps of a quadrant share the
@@ -452,7 +459,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     uint8_t* st = gbase + EPI_OFFSET + (warp - 2) * 4096;
     const uint32_t st_addr = smem_u32(st);
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + grp * share * 32;
-    const float c2_all = (unpacked ? 1.f : g.rw.head->z_scale) * 1.4426950408889634f;   // accumulator -> logit in log2 units
+    const float z_scale = unpacked ? 1.f : g.rw.head->z_scale, c2_all = logit_factor(z_scale);
     // rows that a store may reach (packed ones: whole warps of them, their buffers end with a tile)
     const int rows_end = g.live_m ? live : g.M;
     int local = 0;
@@ -469,7 +476,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       float lse2 = 0.f, wg = 0.f, g_target = 0.f, alpha = 1.f, base2 = 0.f, c2 = c2_all;
       if constexpr (EPI <= EPI_GRAD) {
         if (row < live) {
-          if (EPI <= EPI_EXP && g.rw.unscale) c2 *= g.rw.unscale[row];
+          if (EPI <= EPI_EXP && g.rw.unscale) c2 = logit_factor(z_scale * g.rw.unscale[row]);
           target = g.rw.target[row] - (uint32_t)(g.v0 + col);      // relative to this warp's columns
           if constexpr (EPI == EPI_GRAD) {
             lse2 = g.rw.lse[row];

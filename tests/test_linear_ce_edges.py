@@ -2,6 +2,7 @@
 are sure of their target, tokens far below the likeliest, sums over many rows, infinite logits.  The formula
 in 64 bits and the bounds are those of the tests of its values; a tighter bound is derived where it is used."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -176,3 +177,29 @@ def test_logits_of_minus_infinity(cuda_ctx, eng, mode, rows):
         # operands and g within half a step of f16 (2^-21 and exact in the other modes), logits within 1e-2 for that
         rel = {"F32": 1e-4, "F16": 2e-2 if kind is F32 else 2e-3, "F16X2": 1e-4}[mode]
         assert ((got[2].double() - full).abs() <= rel * size + 1e-7).all()
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("size", [1e-25, 1e-30])
+def test_operands_whose_scales_multiply_to_nothing(cuda_ctx, eng, mode, size):
+    """f32 operands far below 1: every logit is 0 to f32, so each loss is log(vocab) to a few units of 2^-24 of
+    it, every probability 1 / vocab, and the gradients follow in the operands' own size."""
+    for rows, hidden, vocab in ((70, 40, 300), (300, 40, 300), (300, 320, 600)):
+        x, w, y, a = _make(rows, hidden, vocab, (F32, F32), True, "half", 9)
+        x, w, a = x * size, w * size, a.abs() + 0.01
+        q = _truth(x / size, w / size, y, a, 1.0, True)
+        live = q["live"]
+        one = torch.zeros_like(q["z"])
+        one[live, y[live]] = 1.0
+        g = torch.where(live[:, None], (1.0 / vocab - one) * a.double()[:, None], 0.0)
+        # 22 bits of each operand and of g (11 in FT_GEMM_F16), f32 sums
+        rel = 2.0 ** -9 if mode == "F16" else 2.0 ** -16
+        dh, dW = g @ q["W"], g.t() @ q["X"]
+        for want in ("both", "hidden", "none"):
+            loss, gh, gw = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, True, want=want)
+            assert ((loss.double() - torch.where(live, np.log(vocab), 0.0)).abs() <= 8 * 2.0 ** -24 * np.log(vocab)).all()
+            if gh is not None:
+                assert ((gh.double() / size - dh).abs() <= rel * (g.abs() @ q["W"].abs()) + 2.0 ** -149 / size).all()
+            if gw is not None:
+                assert ((gw.double() / size - dW).abs() <= rel * (g.abs().t() @ q["X"].abs()) + 2.0 ** -149 / size).all()
