@@ -70,8 +70,13 @@ constexpr int BARRIERS = 2 * MAX_STAGES + 2 * MAX_BUFFERS + 4;
 constexpr int smem_bytes(int epi, bool two, bool pair) { return bar_offset(epi, two, pair) + BARRIERS * 8 + 16 + 1024; }
 // what E is held times: unscaled, a token below 2^-14 of its tile's maximum would fall under f16's normal range
 constexpr float E_SCALE = 16384.f;
-// k-blocks of 64 that are summed in tensor memory; 0: all
+// k-blocks of 64 that are summed in tensor memory; 0: all.  TWO for STORE means slices, of TcProduct::slice blocks: 512
+// of K with two planes.  With one plane its sums, which run over rows or the vocabulary and have no limit to
+// their length, are taken over 2048 at most (128 groups of 16: 2^-16 of the sum is cut off; a million rows
+// in one sum lose 0.4%): where there are more, by the instance in slices (2048 of 4096 rows x 896 x 151936,
+// whole call: 2.01 -> 2.02 ms).
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
+constexpr int ONE_PLANE_SLICE = 32;
 
 struct TcProduct {
   int M, N, K;
@@ -79,6 +84,7 @@ struct TcProduct {
   int unpacked;                     // STATS, EXP, FACTOR: the rows are the caller's own, all M of them (no head, no scales)
   int carry;                        // STATS: one tile of rows; a pair joins its column tiles before it writes them
   int splits;                       // parts of K, each with a slab of its own
+  int slice;                        // STORE in slices: k-blocks of one
   int tile_n;                       // columns of a tile: a multiple of 32 up to TILE
   int n_fast, band;                 // order of the tiles
   int a_bytes, stage_bytes;         // of A in a stage, of a stage (multiples of 1024)
@@ -364,7 +370,7 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const int units = tiles_m * tiles_n * g.splits;
   const int kb_all = g.live_k ? max(1, (live + BK - 1) / BK) : (g.K + BK - 1) / BK;
   constexpr int SLICE = slice_of(EPI, TWO);
-  const int slice = SLICE ? SLICE : kb_all;
+  const int slice = SLICE == 0 ? kb_all : EPI == EPI_STORE ? g.slice : SLICE;
   // FACTOR: parts of K begin with a tile of E
   constexpr int GRAIN = EPI == EPI_FACTOR ? SLICE : 1;
   const int grains = (kb_all + GRAIN - 1) / GRAIN;
@@ -1605,6 +1611,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.unpacked = unpacked ? 1 : 0;
     p.base_out = pl.by_exp && pl.finish ? pl.base : nullptr;
     tile(p, pl.pair, pl.out_n, a_rows, vm);
+    p.slice = two ? slice_of(EPI_STORE, true) : ONE_PLANE_SLICE;
     return p;
   };
 
@@ -1690,7 +1697,8 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     }
     if (t.grad_hidden) {
       const TcProduct p = dh_product(v0, cols);
-      FT_TRY(launch_rows<EPI_STORE>(ctx, pl.pair, vm, two, g_k, vm ? w_mn : w_k, acc_out, p));
+      const bool slices = two || ft_cdiv(ft_cdiv(cols, BK), p.splits) > ONE_PLANE_SLICE;
+      FT_TRY(launch_rows<EPI_STORE>(ctx, pl.pair, vm, slices, g_k, vm ? w_mn : w_k, acc_out, p));
     }
     if (t.grad_weight) {
       TcProduct p = {};
@@ -1708,7 +1716,8 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
       tile(p, true, pl.out_n, 128, true);
       p.n_fast = p.M >= p.N; p.band = ft_cdiv(p.M, TILE);
       const CUtensorMap& po = dw_tma ? dw_out : g_mn;
-      if (two) FT_TRY((launch_gemm<true, EPI_STORE, true, true, true>(ctx, g_mn, h_mn, po, p, nullptr)));
+      p.slice = two ? slice_of(EPI_STORE, true) : ONE_PLANE_SLICE;
+      if (two || ft_cdiv(T, BK) > ONE_PLANE_SLICE) FT_TRY((launch_gemm<true, EPI_STORE, true, true, true>(ctx, g_mn, h_mn, po, p, nullptr)));
       else FT_TRY((launch_gemm<true, EPI_STORE, true, true, false>(ctx, g_mn, h_mn, po, p, nullptr)));
     }
   }

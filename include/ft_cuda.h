@@ -223,8 +223,11 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  *   grad_weight grad_weight_type, shaped like the weight, or NULL
  * The context's GEMM mode chooses the arithmetic of the products: FT_GEMM_F32 exact f32 FMA,
  * FT_GEMM_F16 operands and g rounded to f16, FT_GEMM_F16X2 f32 operands and g carried as two f16
- * halves.  (f16 operands are exact in every mode; sums are f32 in every mode.)  Calls of at most 16
- * rows may be computed on f32 FMA in any mode, where that is the faster way.
+ * halves.  f16 operands are exact in every mode.  Sums are held in f32 in every mode; a tensor core
+ * cuts off the low bits of every group of 16 products (at most 2^-23 of the sum so far), so sums over
+ * rows and over the vocabulary pass through it 2048 terms at a time and are joined by f32 adds, in
+ * FT_GEMM_F16X2 all sums 512 terms at a time; FT_GEMM_F16 takes a logit's `hidden` terms at once.
+ * Calls of at most 16 rows may be computed on f32 FMA in any mode, where that is the faster way.
  * The vocabulary is worked through in pieces of vocab_piece columns (0: chosen by size), of which
  * only one piece of g exists at a time (with 0, at most 16 rows may have all their logits kept
  * there, 64 bytes a column); workspace holds it and must have the bytes that

@@ -203,3 +203,26 @@ def test_operands_whose_scales_multiply_to_nothing(cuda_ctx, eng, mode, size):
                 assert ((gh.double() / size - dh).abs() <= rel * (g.abs() @ q["W"].abs()) + 2.0 ** -149 / size).all()
             if gw is not None:
                 assert ((gw.double() / size - dW).abs() <= rel * (g.abs().t() @ q["X"].abs()) + 2.0 ** -149 / size).all()
+
+
+@gpu
+def test_f16_products_over_a_million_rows(cuda_ctx, eng):
+    """dW sums one product for each row.  All terms of a column are positive here, so what a sum in the tensor
+    cores loses, which cuts low bits off with each group of 16 products, would add up: 65536 groups, 2^-23
+    of the sum each at most, is 0.8%.  Rounding g to f16 gives 2^-11, logits a relative error of 72 x 2^-24 x
+    sum |h W| < 2^-14 in p; the sums themselves are taken over 2048 rows (128 groups) and then in f32."""
+    t, h, v = 1 << 20, 8, 256
+    g = torch.Generator(device="cuda").manual_seed(77)
+    x = (torch.rand((t, h), generator=g, device="cuda") + 0.5).to(F16)
+    w = (torch.randn((v, h), generator=g, device="cuda") * 0.1).to(F16)
+    y = torch.full((t,), 3, device="cuda")
+    a = torch.rand(t, generator=g, device="cuda") / t
+    dW = torch.zeros((v, h), dtype=torch.float64, device="cuda")
+    for s in range(0, t, 1 << 17):
+        X, A = x[s:s + (1 << 17)].double(), a[s:s + (1 << 17)].double()
+        p = torch.softmax(X @ w.double().t(), dim=1)
+        p[:, 3] -= 1
+        dW += (p * A[:, None]).t() @ X
+    got = _call(cuda_ctx, eng, "F16", x, w, y, a, 1.0, True, (F32, F32))
+    rel = 2.0 ** -11 + 2.0 ** -14 + 128 * 2.0 ** -23 + (t / 2048 + 64) * 2.0 ** -24
+    assert ((got[2].double() - dW).abs() <= rel * dW.abs()).all()
