@@ -108,6 +108,7 @@ extern "C" int ft_ctx_destroy(FtContext* ctx) {
   if (!ctx) return FT_OK;
   cudaSetDevice(ctx->device);
   cudaStreamSynchronize(ctx->stream);
+  ft_free_retired_lists(ctx);
   if (ctx->scratch) cudaFree(ctx->scratch);
   if (ctx->scale_buf) cudaFree(ctx->scale_buf);
   if (ctx->pre_flags) cudaFree(ctx->pre_flags);

@@ -61,6 +61,7 @@ struct FtContext {
   struct ProfRec { const char* name; cudaEvent_t e0, e1; };
   std::vector<ProfRec> prof_recs;
   std::vector<cudaEvent_t> prof_pool;
+  FtGradList* retired_lists = nullptr;   // destroyed, their device memory not yet released
   // cuTensorMapEncodeTiled, resolved through the runtime (no link against libcuda)
   void* encode_tiled = nullptr;
 };
@@ -152,6 +153,9 @@ inline cudaError_t ft_launch_ex(FtContext* ctx, void (*kernel)(KArgs...), dim3 g
 // Scratch of at least `bytes`, 256-byte aligned.  Stream order makes reuse by consecutive
 // calls safe; growth synchronises the stream before the old block is released.
 int ft_scratch(FtContext* ctx, size_t bytes, void** out);
+
+// Releases the device memory of destroyed gradient lists, once the stream is done with it.
+void ft_free_retired_lists(FtContext* ctx);
 
 // Makes the context's device current for a scope.  Launches and attribute queries need it when
 // the calling thread works on several devices.

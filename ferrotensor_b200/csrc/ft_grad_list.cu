@@ -329,6 +329,7 @@ struct FtGradList {
   bool small = false;           // chunks of SMALL_CHUNK for k_list_small, else of CHUNK
   Chunk* table = nullptr;       // [chunks] on the device
   double* partials = nullptr;   // one sum for each block of k_list_squares
+  FtGradList* next = nullptr;   // in the context's list of destroyed ones
 };
 
 namespace {
@@ -448,16 +449,27 @@ extern "C" int ft_grad_list_create(FtContext* ctx, size_t count, void* const* pt
     ft_set_error("ft_grad_list_create: %zu tensors: %s", count, e.what());
     return FT_ERR_INVALID;
   }
+  ft_free_retired_lists(ctx);
   *out = l;
   return FT_OK;
 }
 
+// Makes no CUDA call: a garbage collector may come here in the middle of a stream capture, which a
+// wait or a cudaFree would end.  The next list or the context's end releases the memory.
 extern "C" int ft_grad_list_destroy(FtGradList* l) {
   if (!l) return FT_OK;
-  FtDeviceScope on(l->ctx);
-  cudaStreamSynchronize(l->ctx->stream);
-  free_list(l);
+  l->next = l->ctx->retired_lists;
+  l->ctx->retired_lists = l;
   return FT_OK;
+}
+
+void ft_free_retired_lists(FtContext* ctx) {
+  if (!ctx->retired_lists) return;
+  cudaStreamSynchronize(ctx->stream);
+  while (FtGradList* l = ctx->retired_lists) {
+    ctx->retired_lists = l->next;
+    free_list(l);
+  }
 }
 
 extern "C" int ft_global_grad_norm(FtContext* ctx, FtGradList* grads, float grad_scale, float* norm_out) {

@@ -273,7 +273,8 @@ _TYPE_CODE = {DType.F32: _lib.FT_TYPE_F32, DType.FP16: _lib.FT_TYPE_F16}
 
 class GradientList:
     """The tensors that a norm or a clip runs over (F32 or FP16, any shapes), laid out once for the
-    device.  It keeps the tensors alive; every call reads their values anew."""
+    device.  It keeps the tensors alive; every call reads their values anew.  A graph that holds calls
+    on a list needs the list kept as long as itself."""
 
     def __init__(self, ctx: CudaContext, tensors: Sequence[UnifiedTensor]):
         self.ctx, self.tensors, self.handle = ctx, list(tensors), None

@@ -273,7 +273,10 @@ int ft_adamw_update(FtContext* ctx, float* w, const float* g, float* m, float* v
  * must live as long as the list; their values are read anew by every call.  Creating a list
  * allocates and copies (not inside a stream capture), calls on it do neither.  A list belongs to
  * its context: calls on it run in the order of the context's stream, and graphs that hold calls
- * on one list must not run at the same time.
+ * on one list must not run at the same time, nor after it was destroyed.  Destroying a list makes no
+ * CUDA call, so it may happen during a capture; its device memory (16 bytes for each 8192 values)
+ * is released when the context's next list is created, or with the context, before which all
+ * its lists have to be destroyed.
  * norm_out: device f32[4] = {norm, applied, factor, unused}, as ft_model_apply_gradients:
  *   norm    = |grad_scale| * sqrt(sum of all squares), squares and sums in f64
  *   applied = 1, or 0 when the norm is not finite in f32

@@ -317,3 +317,42 @@ def test_a_step_with_a_trained_head(cuda_ctx, eng):
             assert (w.double() - W).abs().max() <= 10 * 1e-4 * float(DW.abs().max()) * 2 + 1e-6
     finally:
         cuda_ctx.set_gemm_mode(GemmMode.F32)
+
+
+@gpu
+def test_a_list_that_goes_away_during_a_capture(cuda_ctx):
+    """The garbage collector may meet a list while the stream is being captured: the capture stands, and the
+    graph and lists made later work."""
+    from ferrotensor_b200.engine import ComputeEngine, CudaContext, GradientList
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ctx = CudaContext(0)
+    eng = ComputeEngine(ctx)
+    xs, _ = _tensors([30000, 77], [F32, F16], 11)
+    norm = torch.zeros(4, device="cuda")
+    src, other = (GradientList(ctx, [_ut(x) for x in xs]) for _ in range(2))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        eng.global_grad_norm(ctx, src, _ut(norm))
+        eng.global_grad_norm(ctx, other, _ut(norm))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            eng.global_grad_norm(ctx, src, _ut(norm))
+            other.close()
+            eng.global_grad_norm(ctx, src, _ut(norm), grad_scale=2.0)
+    for k in range(3):
+        later = GradientList(ctx, [_ut(x) for x in xs])
+        norm.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        want = _true_norm(xs, 2.0)
+        assert abs(float(norm[0]) - want) <= 2.0 ** -23 * want
+        with torch.cuda.stream(side):
+            eng.global_grad_norm(ctx, later, _ut(norm))
+        torch.cuda.synchronize()
+        assert abs(float(norm[0]) - want / 2) <= 2.0 ** -23 * want
+        later.close()
+    src.close()
+    ctx.close()
