@@ -566,6 +566,8 @@ class ComputeEngine:
         writes nothing but norm_out = {norm, applied, factor, unused}."""
         _require(norm_out is None or (norm_out.dtype is DType.F32 and norm_out.numel() >= 4),
                  "clip_grad_global_norm: norm_out holds 4 F32 values")
+        # (a NULL list of outputs would mean: in place)
+        _require(out is None or bool(out.handle), "clip_grad_global_norm: the list of outputs is closed")
         call("ft_clip_grad_global_norm", ctx.handle, grads.handle, out.handle if out is not None else None,
              float(grad_scale), float(max_norm), norm_out.ptr if norm_out is not None else None)
 

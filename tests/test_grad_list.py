@@ -356,3 +356,23 @@ def test_a_list_that_goes_away_during_a_capture(cuda_ctx):
         later.close()
     src.close()
     ctx.close()
+
+
+def test_a_closed_list_of_outputs_is_refused(lib, monkeypatch):
+    """It must not turn into "no list of outputs", which scales the gradients themselves."""
+    from ferrotensor_b200 import engine
+    made = []
+    monkeypatch.setattr(engine, "call", lambda name, *a: made.append(name))
+    fake = type("Ctx", (), {"handle": 1})()
+    open_list, closed = (engine.GradientList.__new__(engine.GradientList) for _ in range(2))
+    for li in (open_list, closed):
+        li.ctx, li.tensors, li.handle = fake, [], C.c_void_p(64)
+    closed.close()
+    eng = engine.ComputeEngine.__new__(engine.ComputeEngine)
+    try:
+        with pytest.raises(engine.FtError, match="closed"):
+            eng.clip_grad_global_norm(fake, open_list, 1.0, out=closed)
+        eng.clip_grad_global_norm(fake, open_list, 1.0)
+    finally:
+        open_list.close()
+    assert made == ["ft_grad_list_destroy", "ft_clip_grad_global_norm", "ft_grad_list_destroy"]
