@@ -51,6 +51,7 @@ class CudaContext:
             raise FtError(-1, "no CUDA device: the cuda engine has no CPU fallback")
         _lib.load()
         self.device = torch.device("cuda", device)
+        self.device_index = device
         torch.cuda.set_device(self.device)
         self.stream = torch.cuda.current_stream(self.device)
         handle = C.c_void_p()
@@ -268,6 +269,14 @@ def _require(cond: bool, msg: str) -> None:
         raise FtError(1, msg)
 
 
+def _buffer(ctx, t, nbytes: int, what: str) -> int:
+    """The address of a tensor's buffer, which has to hold `nbytes` on the context's device."""
+    s = t.storage
+    if s.get_device() != ctx.device_index or s.nbytes < nbytes:
+        raise FtError(1, f"{what} has a buffer of {s.nbytes} bytes on {s.device}, {nbytes} on cuda:{ctx.device_index} are needed")
+    return s.data_ptr()
+
+
 _TYPE_CODE = {DType.F32: _lib.FT_TYPE_F32, DType.FP16: _lib.FT_TYPE_F16}
 
 
@@ -280,11 +289,9 @@ class GradientList:
         self.ctx, self.tensors, self.handle = ctx, list(tensors), None
         for i, t in enumerate(self.tensors):
             _require(t.dtype in _TYPE_CODE, f"GradientList: tensor {i} is {t.dtype}, expected F32 or FP16")
-            _require(t.storage.device == ctx.device, f"GradientList: tensor {i} is on {t.storage.device}")
-            _require(t.size_in_bytes() <= t.storage.numel() * t.storage.element_size(),
-                     f"GradientList: tensor {i} is larger than its buffer")
         n = len(self.tensors)
-        ptrs = (C.c_void_p * n)(*[t.storage.data_ptr() for t in self.tensors])
+        ptrs = (C.c_void_p * n)(*[_buffer(ctx, t, t.size_in_bytes(), f"GradientList: tensor {i}")
+                                  for i, t in enumerate(self.tensors)])
         counts = (C.c_size_t * n)(*[t.numel() for t in self.tensors])
         types = (C.c_int * n)(*[_TYPE_CODE[t.dtype] for t in self.tensors])
         handle = C.c_void_p()
@@ -492,14 +499,14 @@ class ComputeEngine:
     def linear_cross_entropy_workspace(self, ctx, hidden, weight, grad_hidden=None, grad_weight=None,
                                        vocab_piece=0, vocab_major=False) -> int:
         """Bytes of workspace that a call with these tensors needs in the context's GEMM mode."""
-        p = self._linear_ce_params(hidden, weight, grad_hidden, grad_weight, 1.0, vocab_piece, int(vocab_major))
+        p, *_ = self._linear_ce_params(hidden, weight, grad_hidden, grad_weight, 1.0, vocab_piece, int(vocab_major))
         n = C.c_size_t()
         call("ft_linear_cross_entropy_workspace", ctx.handle, weight.ptr, C.byref(p), grad_hidden is not None,
              grad_weight is not None, C.byref(n))
         return n.value
 
     # A call of one row takes the device less time than a few dozen lines of Python take the host, so
-    # these check in straight lines (19 us a call with loops over the operands, 16 so).
+    # these check in straight lines (19 us a call with loops over the operands, 16 so; 1.4 more for the buffers).
     @staticmethod
     def _linear_ce_type(t, name) -> int:
         if t.dtype is DType.F32:
@@ -528,19 +535,31 @@ class ComputeEngine:
             _require(grad_weight.numel() == h * vocab, "linear_cross_entropy: grad_weight has the wrong size")
         _require(0 <= vocab_piece < 1 << 32, "linear_cross_entropy: vocab_piece is out of range")
         _require(max(rows, h, vocab) < 1 << 32, "linear_cross_entropy: a dimension is out of range")
-        return FtLinearCeParams(rows, h, vocab, vocab_major, hidden_type, weight_type, grad_hidden_type,
-                                grad_weight_type, vocab_piece, grad_scale)
+        # and the bytes of hidden, weight and their gradients
+        values, columns = rows * h, h * vocab
+        return (FtLinearCeParams(rows, h, vocab, vocab_major, hidden_type, weight_type, grad_hidden_type, grad_weight_type,
+                                 vocab_piece, grad_scale), rows, values * (4 - 2 * hidden_type), columns * (4 - 2 * weight_type),
+                values * (4 - 2 * grad_hidden_type), columns * (4 - 2 * grad_weight_type))
 
     def _linear_ce(self, ctx, hidden, weight, targets, weights, row_loss, grad_hidden, grad_weight, grad_scale,
                    vocab_piece, workspace, vocab_major):
-        p = self._linear_ce_params(hidden, weight, grad_hidden, grad_weight, grad_scale, vocab_piece, vocab_major)
-        _require(targets.dtype is DType.U32 and targets.numel() == p.rows, "linear_cross_entropy: one U32 target per row")
-        _require(row_loss.dtype is DType.F32 and row_loss.numel() == p.rows, "linear_cross_entropy: one F32 loss per row")
-        _require(weights is None or (weights.dtype is DType.F32 and weights.numel() == p.rows),
+        p, rows, x_bytes, w_bytes, gh_bytes, gw_bytes = self._linear_ce_params(
+            hidden, weight, grad_hidden, grad_weight, grad_scale, vocab_piece, vocab_major)
+        _require(targets.dtype is DType.U32 and targets.numel() == rows, "linear_cross_entropy: one U32 target per row")
+        _require(row_loss.dtype is DType.F32 and row_loss.numel() == rows, "linear_cross_entropy: one F32 loss per row")
+        _require(weights is None or (weights.dtype is DType.F32 and weights.numel() == rows),
                  "linear_cross_entropy: one F32 weight per row")
-        ref, w = C.byref(p), weight.storage.data_ptr()
-        gh = None if grad_hidden is None else grad_hidden.storage.data_ptr()
-        gw = None if grad_weight is None else grad_weight.storage.data_ptr()
+        ref = C.byref(p)
+        x = _buffer(ctx, hidden, x_bytes, "linear_cross_entropy: hidden")
+        w = _buffer(ctx, weight, w_bytes, "linear_cross_entropy: weight")
+        y = _buffer(ctx, targets, 4 * rows, "linear_cross_entropy: targets")
+        a = None if weights is None else _buffer(ctx, weights, 4 * rows, "linear_cross_entropy: weights")
+        loss = _buffer(ctx, row_loss, 4 * rows, "linear_cross_entropy: row_loss")
+        gh = gw = None
+        if grad_hidden is not None:
+            gh = _buffer(ctx, grad_hidden, gh_bytes, "linear_cross_entropy: grad_hidden")
+        if grad_weight is not None:
+            gw = _buffer(ctx, grad_weight, gw_bytes, "linear_cross_entropy: grad_weight")
         if workspace is None:
             n = C.c_size_t()
             call("ft_linear_cross_entropy_workspace", ctx.handle, w, ref, grad_hidden is not None, grad_weight is not None,
@@ -548,16 +567,14 @@ class ComputeEngine:
             held = ctx.temporary(n.value)
             space, size = held.data_ptr(), n.value
         else:
-            held = workspace.storage
-            space, size = held.data_ptr(), held.numel() * held.element_size()
-        call("ft_linear_cross_entropy", ctx.handle, hidden.storage.data_ptr(), w, targets.storage.data_ptr(),
-             None if weights is None else weights.storage.data_ptr(), row_loss.storage.data_ptr(), gh, gw, space, size, ref)
+            space, size = _buffer(ctx, workspace, 0, "linear_cross_entropy: workspace"), workspace.storage.nbytes
+        call("ft_linear_cross_entropy", ctx.handle, x, w, y, a, loss, gh, gw, space, size, ref)
 
     # ---- trainer/lib.rs:328-343: the norm over all gradients, and the clip by it
     def global_grad_norm(self, ctx, grads: GradientList, norm_out, grad_scale=1.0):
         """norm_out (F32, 4 values): {norm, 1 or 0 when it is not finite, grad_scale, unused}."""
         _require(norm_out.dtype is DType.F32 and norm_out.numel() >= 4, "global_grad_norm: norm_out holds 4 F32 values")
-        call("ft_global_grad_norm", ctx.handle, grads.handle, float(grad_scale), norm_out.ptr)
+        call("ft_global_grad_norm", ctx.handle, grads.handle, float(grad_scale), _buffer(ctx, norm_out, 16, "global_grad_norm: norm_out"))
 
     def clip_grad_global_norm(self, ctx, grads: GradientList, max_norm, norm_out=None, grad_scale=1.0,
                               out: Optional[GradientList] = None):
@@ -569,7 +586,8 @@ class ComputeEngine:
         # (a NULL list of outputs would mean: in place)
         _require(out is None or bool(out.handle), "clip_grad_global_norm: the list of outputs is closed")
         call("ft_clip_grad_global_norm", ctx.handle, grads.handle, out.handle if out is not None else None,
-             float(grad_scale), float(max_norm), norm_out.ptr if norm_out is not None else None)
+             float(grad_scale), float(max_norm),
+             None if norm_out is None else _buffer(ctx, norm_out, 16, "clip_grad_global_norm: norm_out"))
 
     # ---- misc.rs:20-34
     def argmax_rows(self, ctx, input, out_idx):

@@ -17,6 +17,49 @@ def eng(cuda_ctx):
     return ComputeEngine(cuda_ctx)
 
 
+@pytest.mark.parametrize("what", ["hidden", "weight", "targets", "weights", "row_loss", "grad_hidden", "grad_weight", "workspace", "norm_out"])
+def test_buffers_that_are_too_small_or_elsewhere(monkeypatch, what):
+    """A tensor whose buffer is a byte short or on another device never reaches the library."""
+    from ferrotensor_b200 import engine
+    from ferrotensor_b200.engine import DType, FtError, UnifiedTensor
+    calls = []
+    monkeypatch.setattr(engine, "call", lambda name, *a: calls.append(name))
+    ctx = type("Ctx", (), {"handle": 1, "device_index": -1})()      # (-1: what a tensor on the CPU gives)
+    eng = engine.ComputeEngine.__new__(engine.ComputeEngine)
+
+    def tensor(name, shape, kind=DType.F32):
+        n = int(np.prod(shape)) * kind.size_bytes() - (name == short)
+        storage = torch.empty(n, dtype=torch.uint8)
+        if name == far:
+            storage = type("Elsewhere", (), dict(nbytes=n, device="cuda:1", get_device=lambda self: 1, data_ptr=lambda self: 256))()
+        return UnifiedTensor(storage, shape, kind)
+
+    def run():
+        if what == "norm_out":
+            lists = engine.GradientList.__new__(engine.GradientList)
+            lists.ctx, lists.tensors, lists.handle = ctx, [], None
+            eng.global_grad_norm(ctx, lists, tensor("norm_out", [4]))
+            eng.clip_grad_global_norm(ctx, lists, 1.0, tensor("norm_out", [4]))
+            return
+        t = {n: tensor(n, s, k) for n, s, k in (("hidden", [3, 8], DType.FP16), ("weight", [8, 5], DType.F32), ("targets", [3], DType.U32),
+                                                ("weights", [3], DType.F32), ("row_loss", [3], DType.F32), ("grad_hidden", [3, 8], DType.F32),
+                                                ("grad_weight", [8, 5], DType.FP16), ("workspace", [64], DType.U32))}
+        eng.linear_cross_entropy(ctx, **t)
+
+    short = far = None
+    run()
+    assert calls.pop() in ("ft_linear_cross_entropy", "ft_clip_grad_global_norm")
+    calls.clear()
+    if what != "workspace":                                        # (its size is the library's to judge)
+        short = what
+        with pytest.raises(FtError, match=what):
+            run()
+    short, far = None, what
+    with pytest.raises(FtError, match=what):
+        run()
+    assert not calls
+
+
 @gpu
 @pytest.mark.parametrize("mode", ["F16", "F16X2"])
 @pytest.mark.parametrize("vocab_major", [False, True])
