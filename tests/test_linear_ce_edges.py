@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_linear_ce import F16, F32, MODES, SKIP, _bounds, _call, _check, _make, _truth
+from tests.test_linear_ce import F16, F32, MODES, SKIP, _bounds, _call, _check, _make, _targets, _truth, _ut
 
 gpu = pytest.mark.gpu
 
@@ -269,3 +269,35 @@ def test_f16_products_over_a_million_rows(cuda_ctx, eng):
     got = _call(cuda_ctx, eng, "F16", x, w, y, a, 1.0, True, (F32, F32))
     rel = 2.0 ** -11 + 2.0 ** -14 + 128 * 2.0 ** -23 + (t / 2048 + 64) * 2.0 ** -24
     assert ((got[2].double() - dW).abs() <= rel * dW.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+def test_losses_without_row_weights(cuda_ctx, eng, mode):
+    """No gradient asked for: the rows' weights may be left out, and change nothing."""
+    for t in (1, 16, 100, 300):
+        x, w, y, a = _make(t, 64, 900, (F16, F16), True, "half", 9)
+        with_weights = _call(cuda_ctx, eng, mode, x, w, y, a, 1.0, True, want="none")[0]
+        from ferrotensor_b200.engine import GemmMode
+        cuda_ctx.set_gemm_mode(GemmMode[mode])
+        loss = torch.full((t,), 9.0, device="cuda")
+        try:
+            eng.linear_cross_entropy_bt(cuda_ctx, _ut(x), _ut(w), _ut(_targets(y)), None, _ut(loss))
+            cuda_ctx.synchronize()
+        finally:
+            cuda_ctx.set_gemm_mode(GemmMode.F32)
+        assert torch.equal(loss, with_weights)
+
+
+@gpu
+@pytest.mark.parametrize("types,gtypes", [((F32, F32), (F32, F32)), ((F16, F16), (F16, F16)), ((F32, F16), (F32, F16))])
+@pytest.mark.parametrize("vocab_major", [False, True])
+@pytest.mark.parametrize("rows,hidden,mask", [(700, 320, "half"), (257, 896, "none"), (900, 264, "prompts"), (513, 576, "last")])
+def test_gradient_made_in_place_over_several_row_tiles(cuda_ctx, eng, types, gtypes, vocab_major, rows, hidden, mask):
+    """The split mode with more than one tile of rows, some of them empty behind the last supervised row."""
+    s = 512.0 if F16 in gtypes else 1.0
+    x, w, y, a = _make(rows, hidden, 2100, types, vocab_major, mask, 900 + rows)
+    x[y == SKIP] = float("nan")
+    q = _truth(x, w, y, a, s, vocab_major)
+    got = _call(cuda_ctx, eng, "F16X2", x, w, y, a, s, vocab_major, gtypes)
+    _check(got, q, _bounds(q, "F16X2", types, gtypes), vocab_major)
