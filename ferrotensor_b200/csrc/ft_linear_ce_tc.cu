@@ -91,8 +91,7 @@ struct TcProduct {
   int stage_tx;                     // what the tile's CTAs load into one
   int terms;                        // plane pairs, the small ones first
   int a_plane[3], b_plane[3];
-  int a_mn0, b_mn0, k0;             // where M, N and K begin in the operands' tensors...
-  int a_has_k0, b_has_k0;           // ... and which of them k0 applies to
+  int b_mn0, b_k0;                  // where N and K begin in B's tensor
   // EPI_STATS, EPI_GRAD
   Rows rw;
   float2* part;                     // [parts of a tile * column tiles][part_ld]: {maximum in log2 units, sum}
@@ -380,11 +379,10 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (elect_one()) {
       uint32_t stage = 0, phase = 0;
-      const int ak0 = g.a_has_k0 ? g.k0 : 0, bk0 = g.b_has_k0 ? g.k0 : 0;
       for (int u = pair; u < units && !*abort_flag; u += npairs) {
         const Unit un = decode_unit(u, tiles_m, tiles_n, g);
         const int kb0 = k_begin(un.sp), kb1 = k_begin(un.sp + 1);
-        const int am = g.a_mn0 + un.mt * TM + (int)rank * 128;
+        const int am = un.mt * TM + (int)rank * 128;
         const int bn = g.b_mn0 + un.nt * tile_n + (PAIR ? (int)rank * (tile_n / 2) : 0);
         const int b_cols = PAIR ? tile_n / 2 : tile_n;
         for (int s0 = kb0; s0 < kb1 && !*abort_flag; s0 += slice) {
@@ -397,15 +395,15 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               const uint32_t bar = lead_full + stage * 8;
               if (rank == 0) mbar_expect_tx(bar_full + stage * 8, (uint32_t)g.stage_tx);
               if constexpr (A_MN) {
-                load_3d<PAIR>(sa, &map_a, bar, am, ak0 + kb * BK, pa);
-                load_3d<PAIR>(sa + 8192, &map_a, bar, am + 64, ak0 + kb * BK, pa);
+                load_3d<PAIR>(sa, &map_a, bar, am, kb * BK, pa);
+                load_3d<PAIR>(sa + 8192, &map_a, bar, am + 64, kb * BK, pa);
               } else {
-                load_3d<PAIR>(sa, &map_a, bar, ak0 + kb * BK, am, pa);
+                load_3d<PAIR>(sa, &map_a, bar, kb * BK, am, pa);
               }
               if constexpr (B_MN) {
-                for (int c = 0; c < b_cols; c += 64) load_3d<PAIR>(sb + c * 128, &map_b, bar, bn + c, bk0 + kb * BK, pb);
+                for (int c = 0; c < b_cols; c += 64) load_3d<PAIR>(sb + c * 128, &map_b, bar, bn + c, g.b_k0 + kb * BK, pb);
               } else {
-                load_3d<PAIR>(sb, &map_b, bar, bk0 + kb * BK, bn, pb);
+                load_3d<PAIR>(sb, &map_b, bar, g.b_k0 + kb * BK, bn, pb);
               }
               if (++stage == stages) { stage = 0; phase ^= 1; }
             }
@@ -1605,7 +1603,7 @@ int tc_path(FtContext* ctx, const Problem& q, const Tensors& t, void* ws) {
     p.splits = std::min(pl.splits, ft_cdiv(cols, pl.by_exp ? TILE : BK));
     p.n_fast = 1; p.band = 1;
     set_terms(p, pl.g_planes, pl.w_planes);
-    p.k0 = v0; p.b_has_k0 = 1;
+    p.b_k0 = v0;
     p.out_type = FT_TYPE_F32; p.accumulate = v0 > 0;
     p.part = pl.part; p.part_ld = pl.Tp;
     p.unpacked = unpacked ? 1 : 0;
