@@ -64,7 +64,6 @@ struct Rows {
   float* lse;
   float* at_target;   // p - 1 at the target, from the loss: -(1 - e^-loss) is exact where 1 - p is small
   float* base;        // E: the point R that the row's sums are scaled against, in log2 units
-  float2* kept;       // E: {value, reference point} of the target
 };
 
 struct Problem {
@@ -114,7 +113,6 @@ inline Rows carve_rows(Carver& c, int T) {
   r.lse = c.take<float>(T);
   r.at_target = c.take<float>(T);
   r.base = c.take<float>(T);
-  r.kept = c.take<float2>(T);
   return r;
 }
 

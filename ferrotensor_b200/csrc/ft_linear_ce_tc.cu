@@ -15,7 +15,8 @@
 // that maximum), and the
 // product E W is drained from tensor memory once a tile of K and scaled there, in f32, by the
 // row's 2^(ref - R).  R is the row's maximum when its first piece was done; the rest of the
-// normaliser and the one-hot term, -w W(:, y), are applied by the pass that unpacks the rows.
+// normaliser and the target's term, w (p - 1) W(:, y), which E leaves out, are applied by the pass that
+// unpacks the rows.
 // That saves a third of the multiplications of a frozen head's gradient.
 //
 // Planes: an f16 operand, and an f32 one in FT_GEMM_F16, is one f16 plane.  FT_GEMM_F16X2 carries an
@@ -236,7 +237,7 @@ __device__ __forceinline__ void stage_f16(uint8_t* st, int lane, int part, const
 // cost a 32-byte sector for every 2 bytes; with many rows (R = 32) all warps walk down K together,
 // so that DRAM reads a row of W once for all targets in it (with a row a warp, 4096 rows x 2048
 // read 540 MB for 100 MB of W and the products waited for them: 390 against 277 us).
-// With g.wy the columns are kept, for the one-hot term of dh.
+// With g.wy the columns are kept, for the target's term of dh.
 __device__ __forceinline__ void target_dots(const TcProduct& g, int r0, int r1, int worker, int workers, float scale, int lane) {
   const int rows = r1 - r0;
   int R = 1;
@@ -581,16 +582,17 @@ k_ce_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           mask_columns(c0, v);
           const float ref = finite_max(run_m);
           if (y < 32u) {
+            // The target has no part in E: its whole gradient, p - 1, is applied from the loss.  (Both parts, p by
+            // E W and -1 later, would leave a sure row's gradient to the last bits of their sums.)
             float z = 0.f;
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (y == (uint32_t)k) z = v[k];
-            const float e = E_SCALE * ex2((z - ref) * c2);
-            float kept = __half2float(__float2half_rn(e));         // as the product will see it
-            if (TWO) kept += __half2float(__float2half_rn(e - kept));
-            kept *= 1.f / E_SCALE;
+              if (y == (uint32_t)k) {
+                z = v[k];
+                v[k] = -INFINITY;
+              }
             g.rw.picked[row] = z * c2;
-            g.rw.kept[row] = make_float2(kept, ref * c2);
+            run_s += ex2((z - ref) * c2);
           }
           run_s += exponentials(v, ref, c2);
 #pragma unroll
@@ -909,12 +911,9 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
         row_loss[unpacked_rows ? row : rw.source[row]] = loss;
         if (!unpacked_rows) rw.at_target[row] = expm1f(-loss);
         if (acc) {
-          // the gradient at the target, p - 1, is -(1 - e^-loss), exact for a row that is sure of its
-          // target; what E W holds of it already goes off
+          // the gradient at the target, p - 1, is -(1 - e^-loss), exact for a row that is sure of it
           const float w = rw.weight[row] * rw.head->w_unscale;
-          float b = 0.f;
-          if (rw.target[row] < (uint32_t)vocab) b = expm1f(-loss) - rw.kept[row].x * ex2(rw.kept[row].y - rw.lse[row]);
-          rw.stat[row] = make_float2(w * ex2(rw.base[row] - rw.lse[row]), w * b);
+          rw.stat[row] = make_float2(w * ex2(rw.base[row] - rw.lse[row]), w * rw.at_target[row]);
         }
       }
     }
@@ -929,8 +928,8 @@ k_ce_join(const float2* __restrict__ part, int part_ld, int parts, Rows rw, int 
   }
 }
 
-// E -> g in place, both planes, for a vocabulary that is one piece: g = w (2^(ref - lse) 2^-14 E - onehot), with the
-// gradient at the target as k_ce_join has it, and zero rows up to a K block of dW.
+// E -> g in place, both planes, for a vocabulary that is one piece: g = w 2^(ref - lse) 2^-14 E, with the
+// gradient at the target, where E is zero, as k_ce_join has it, and zero rows up to a K block of dW.
 // One read and one write of E against a second product for the logits (makes_g_in_place).  With one plane it would round g's values twice, so FT_GEMM_F16 has no use for it.
 __global__ void __launch_bounds__(256)
 k_ce_normalise(__half* __restrict__ e, size_t plane, int ld, const float2* __restrict__ part, int part_ld, Rows rw, int cols,
@@ -1260,7 +1259,7 @@ k_ce_finish(const float2* __restrict__ part, int part_ld, int parts, Rows rw, in
       float b = 0.f;
       if (rw.target[at] < (uint32_t)vocab) {
         loss = loss_of(ref, l2, rw.picked[at], rw.exact[at]);
-        b = expm1f(-loss) - rw.kept[at].x * ex2(rw.kept[at].y - lse2);
+        b = expm1f(-loss);
       }
       onehot[i] = w * b;
       lse_of[i] = lse2;

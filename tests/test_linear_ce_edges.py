@@ -301,3 +301,13 @@ def test_gradient_made_in_place_over_several_row_tiles(cuda_ctx, eng, types, gty
     q = _truth(x, w, y, a, s, vocab_major)
     got = _call(cuda_ctx, eng, "F16X2", x, w, y, a, s, vocab_major, gtypes)
     _check(got, q, _bounds(q, "F16X2", types, gtypes), vocab_major)
+
+
+@gpu
+@pytest.mark.parametrize("offset", [200.0, 1000.0])
+@pytest.mark.parametrize("mode", ["F16", "F16X2"])
+@pytest.mark.parametrize("size", [(75, 100, 395, 0), (184, 492, 337, 0), (179, 144, 920, 0), (721, 752, 408, 0), (304, 60, 664, 300), (1100, 144, 920, 0)])
+def test_sure_rows_beside_large_weights(cuda_ctx, eng, mode, offset, size):
+    """A coordinate in which every weight is 32, the others near 0.1: dh there is a sum that comes to almost
+    nothing, of which the target's own share must not be in two parts."""
+    _sure_case(cuda_ctx, eng, mode, offset, size, ("hidden", "both"))
