@@ -220,7 +220,7 @@ __device__ __forceinline__ Outcome decide(double squares, float grad_scale, floa
 
 // Every block joins the partial sums itself (the same order everywhere), block 0 publishes.
 // out == NULL: measure only.  TI, TO: the types of all chunks; void: each chunk's own.  (The four pairs
-// of types in one body spill 300 to 700 bytes a thread, so only lists of both types take it.)
+// of types in one body spill 180 bytes a thread, so only lists of both types take it.)
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(LIST_THREADS, SCALE_BLOCKS_PER_SM)
 k_list_scale(const Chunk* __restrict__ chunks, const Chunk* __restrict__ out, int count,

@@ -12,12 +12,10 @@
 // cheaper, g is made of E in place).  dh alone does not need that.  The pass that finds the
 // statistics writes E = 2^(z2 - ref + 14) for each column tile (z2 in log2 units, ref the row's maximum in
 // that tile: E has f16's full precision whatever the row's normaliser turns out to be, down to 2^-28 of
-// that maximum), and the
-// product E W is drained from tensor memory once a tile of K and scaled there, in f32, by the
-// row's 2^(ref - R).  R is the row's maximum when its first piece was done; the rest of the
-// normaliser and the target's term, w (p - 1) W(:, y), which E leaves out, are applied by the pass that
-// unpacks the rows.
-// That saves a third of the multiplications of a frozen head's gradient.
+// that maximum), and the product E W is drained from tensor memory once a tile of K and scaled there,
+// in f32, by the row's 2^(ref - R).  R is the row's maximum when its first piece was done; the rest of
+// the normaliser and the target's term, w (p - 1) W(:, y), which E leaves out, are applied by the pass
+// that unpacks the rows.  That saves a third of the multiplications of a frozen head's gradient.
 //
 // Planes: an f16 operand, and an f32 one in FT_GEMM_F16, is one f16 plane.  FT_GEMM_F16X2 carries an
 // f32 operand and g (or E) as two planes, hi = f16(x) and lo = f16(x - hi), of which the products
@@ -75,7 +73,7 @@ constexpr float E_SCALE = 16384.f;
 // of K with two planes.  With one plane its sums, which run over rows or the vocabulary and have no limit to
 // their length, are taken over 2048 at most (128 groups of 16: 2^-16 of the sum is cut off; a million rows
 // in one sum lose 0.4%): where there are more, by the instance in slices (2048 of 4096 rows x 896 x 151936,
-// whole call: 2.01 -> 2.02 ms).
+// whole call: 2.01 -> 2.03 ms).
 constexpr int slice_of(int epi, bool two) { return epi == EPI_FACTOR ? TILE / BK : two ? 8 : 0; }
 constexpr int ONE_PLANE_SLICE = 32;
 

@@ -211,8 +211,8 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  *   row_loss[t] = lse_t - z[t, targets[t]]
  *   g[t, v]     = grad_scale * weights[t] * (exp(z[t, v] - lse_t) - (v == targets[t]))
  *   grad_hidden = g W^T,   grad_weight = hidden^T g (in the layout of the weight)
- * targets[t] == FT_MASKED_CE_SKIP gives zero loss and a zero gradient, whatever the row holds
- * (its hidden values are not read); another target >= vocab gives zero loss and the gradient
+ * targets[t] == FT_MASKED_CE_SKIP gives zero loss and a zero gradient, and what the row's hidden
+ * values and weight hold affects nothing (they may be read); another target >= vocab gives zero loss and the gradient
  * without its one-hot term, as ft_masked_cross_entropy_weighted does.
  *   hidden      [rows, hidden]  hidden_type
  *   weight      weight_type, [hidden, vocab] as ft_matmul's b, or with weight_vocab_major
@@ -227,6 +227,12 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  * cuts off the low bits of every group of 16 products (at most 2^-23 of the sum so far), so sums over
  * rows and over the vocabulary pass through it 2048 terms at a time and are joined by f32 adds, in
  * FT_GEMM_F16X2 all sums 512 terms at a time; FT_GEMM_F16 takes a logit's `hidden` terms at once.
+ * The tensor cores' f16 forms of f32 operands, and of g, are scaled by a power of two each, so that
+ * the largest finite value (of the weight, of the rows, or of each row where no grad_weight is wanted;
+ * for g the largest |grad_scale * weights|) is near 2^14: no value is held closer than to 2^-38 of
+ * it, so an f32 weight with one value of 1e30 beside ordinary ones has none of these left in FT_GEMM_F16 and
+ * FT_GEMM_F16X2.  Infinite f32 values, and those they meet, give NaN in FT_GEMM_F16X2 (their two halves
+ * do); else they act as in f32: a weight of -inf that makes a logit -inf takes its column out.
  * Calls of at most 16 rows may be computed on f32 FMA in any mode, where that is the faster way.
  * The vocabulary is worked through in pieces of vocab_piece columns (0: chosen by size), of which
  * only one piece of g exists at a time (with 0, at most 16 rows may have all their logits kept
@@ -278,7 +284,8 @@ int ft_adamw_update(FtContext* ctx, float* w, const float* g, float* m, float* v
  * is released when the context's next list is created, or with the context, before which all
  * its lists have to be destroyed.
  * norm_out: device f32[4] = {norm, applied, factor, unused}, as ft_model_apply_gradients:
- *   norm    = |grad_scale| * sqrt(sum of all squares), squares and sums in f64
+ *   norm    = |grad_scale| * sqrt(sum of all squares), squares and sums in f64 (f16 values: exact f32
+ *             squares, summed by eights in f32 and from there in f64)
  *   applied = 1, or 0 when the norm is not finite in f32
  *   factor  = grad_scale, times max_norm / (norm + 1e-6) when norm > max_norm > 0
  * ft_global_grad_norm only measures (factor = grad_scale).  ft_clip_grad_global_norm also writes
