@@ -212,8 +212,8 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  *   g[t, v]     = grad_scale * weights[t] * (exp(z[t, v] - lse_t) - (v == targets[t]))
  *   grad_hidden = g W^T,   grad_weight = hidden^T g (in the layout of the weight)
  * targets[t] == FT_MASKED_CE_SKIP gives zero loss and a zero gradient, and what the row's hidden
- * values and weight hold affects nothing (they may be read); another target >= vocab gives zero loss and the gradient
- * without its one-hot term, as ft_masked_cross_entropy_weighted does.
+ * values and weight hold affects nothing (they may be read); another target >= vocab gives zero
+ * loss and the gradient without its one-hot term, as ft_masked_cross_entropy_weighted does.
  *   hidden      [rows, hidden]  hidden_type
  *   weight      weight_type, [hidden, vocab] as ft_matmul's b, or with weight_vocab_major
  *               [vocab, hidden] as ft_matmul_bt's
@@ -230,17 +230,16 @@ int ft_masked_cross_entropy_weighted(FtContext* ctx, const float* logits,
  * The tensor cores' f16 forms of f32 operands, and of g, are scaled by a power of two each, so that
  * the largest finite value (of the weight, of the rows, or of each row where no grad_weight is wanted;
  * for g the largest |grad_scale * weights|) is near 2^14: no value is held closer than to 2^-38 of
- * it, so an f32 weight with one value of 1e30 beside ordinary ones has none of these left in FT_GEMM_F16 and
- * FT_GEMM_F16X2.  Infinite f32 values, and those they meet, give NaN in FT_GEMM_F16X2 (their two halves
+ * it, so an f32 weight with one value of 1e30 beside ordinary ones has none of these left in
+ * FT_GEMM_F16 and FT_GEMM_F16X2.  Infinite f32 values, and those they meet, give NaN in FT_GEMM_F16X2 (their two halves
  * do); else they act as in f32: a weight of -inf that makes a logit -inf takes its column out.
  * Calls of at most 16 rows may be computed on f32 FMA in any mode, where that is the faster way.
  * The vocabulary is worked through in pieces of vocab_piece columns (0: chosen by size), of which
  * only one piece of g exists at a time (with 0, at most 16 rows may have all their logits kept
  * there, 64 bytes a column); workspace holds it and must have the bytes that
  * ft_linear_cross_entropy_workspace gives for the same arguments, context and GEMM mode (of the
- * weight it looks at the alignment alone).  The
- * call allocates nothing, keeps nothing there for a later call, and may be captured into a
- * graph; calls that overlap on the GPU need workspaces of their own.  Outputs may overlap no
+ * weight it looks at the alignment alone).  The call allocates nothing, keeps nothing there for a
+ * later call, and may be captured into a graph; calls that overlap on the GPU need workspaces of their own.  Outputs may overlap no
  * input, no other output and not the workspace.
  * Limits: rows <= 2^24, hidden <= 2^16, vocab <= 2^24. */
 typedef struct FtLinearCeParams {
